@@ -417,6 +417,93 @@ int qfa_attn_bwd_f32(const int8_t *qc, const float *sq, const int8_t *zq, const 
  */
 int64_t qfa_attn_bwd_split_workspace_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Nk, int D, int causal, int f32);
 
+/*
+ * RMSNorm of every head's row and the position rotation, in one pass, for one or two tensors (queries and keys; k nullable):
+ *     y = rot(x * w / sqrt(mean(x^2) + eps)),   rot: (a, b) -> (a cos - b sin, b cos + a sin) on `rotated` elements of a row
+ * Everything in fp32, rounded once.  No counterpart in the reference, whose operators take queries and keys as they come.
+ *   x, y       [B,H,N,D] of dtype, D in {64, 128, 256}, 16-byte aligned, strides (batch, head, token) multiples of 16 bytes
+ *   weight     nullable (no norm); [D], or [H,D] where weight_per_head; of w_dtype (QFA_F32 or dtype), for both tensors the same type
+ *   cos, sin   [rope_rows, rotated / 2] float, dense, 16-byte aligned; rotated a multiple of 16 up to D.  NULL with rotated 0: no rotation
+ *   interleaved  pairs (2i, 2i + 1) instead of (i, i + rotated / 2)
+ *   positions  nullable; token n of sequence b has position positions[b * spb + n * spn] + step * n (step 0 or 1; without
+ *              positions: step * n).  The rotated elements of a token whose position is not in [0, rope_rows) are NaN.
+ */
+typedef struct {
+  const void *x, *weight;
+  void *y;            /* backward: dx */
+  const void *dy;     /* backward only */
+  void *dweight;      /* backward only, nullable: [D] or [H,D] of w_dtype */
+  int64_t H, sx[3], sy[3], sdy[3];
+  int weight_per_head;
+} qfa_norm_rope_tensor;
+
+int qfa_norm_rope(const qfa_norm_rope_tensor *q, const qfa_norm_rope_tensor *k, const float *cos, const float *sin, int64_t rope_rows,
+                  int rotated, int interleaved, const int32_t *positions, int64_t spb, int64_t spn, int step, float eps, int dtype,
+                  int w_dtype, int64_t B, int64_t N, int D, void *stream);
+
+/*
+ * Its gradient:  g = rot^T(dy),  dweight = sum over rows of g x r,  dx = r (g w) - x r^3 mean(g w x),  r = 1 / sqrt(mean(x^2) + eps).
+ * dx goes to y.  workspace: qfa_norm_rope_bwd_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant (not needed where no
+ * dweight is asked for); the sums are added up in a fixed order.  weight_per_head as of the tensors: where the two differ, the sum of
+ * what either needs alone (Hk 0).
+ */
+int64_t qfa_norm_rope_bwd_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t Hk, int D, int weight_per_head);
+
+int qfa_norm_rope_bwd(const qfa_norm_rope_tensor *q, const qfa_norm_rope_tensor *k, const float *cos, const float *sin, int64_t rope_rows,
+                      int rotated, int interleaved, const int32_t *positions, int64_t spb, int64_t spn, int step, float eps, int dtype,
+                      int w_dtype, int64_t B, int64_t N, int D, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * A paged INT8 cache of keys and values: codes [pages,H,page_size,D], scale (of scale_dtype) and zero point [pages,H,page_size], dense.
+ * Position p of sequence b is row p % page_size of page page_table[b * stb + (p / page_size) * stw].  page_size: a power of two
+ * from 16 on; D in {64, 128, 256}; the codes 16-byte aligned.  No counterpart in the reference, whose K = V tensor is in one piece.
+ */
+typedef struct {
+  int8_t *k_codes; void *k_scale; int8_t *k_zero;
+  int8_t *v_codes; void *v_scale; int8_t *v_zero;
+  int64_t pages, H;
+  int page_size, D, scale_dtype;
+} qfa_paged_cache;
+
+/*
+ * Quantizes tokens into the cache: token n < counts[b] (counts NULL: all N) of sequence b goes to position starts[b] + n, its
+ * values by the arithmetic of qfa_quant_per_token, its keys likewise after qfa_norm_rope's norm (k_weight nullable: none) and rotation by
+ * that position (cos and sin NULL: none), which stay in fp32 in between.  A token has no place, and is not written, where its position is
+ * negative, past the page table's width or (rotated) past rope_rows, or its page is not in [0, pages).  The places of a call's
+ * tokens must differ: no page that is written may stand twice in the table.
+ *   k, v [B,H,N,D] of dtype, with strides as in qfa_quant_per_token
+ */
+int qfa_paged_append(const qfa_paged_cache *cache, const void *k, const void *v, int dtype, int64_t skb, int64_t skh, int64_t skn, int64_t svb,
+                     int64_t svh, int64_t svn, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts,
+                     const int32_t *counts, const void *k_weight, int w_dtype, int weight_per_head, float eps, const float *cos, const float *sin,
+                     int64_t rope_rows, int rotated, int interleaved, int64_t B, int64_t N, void *stream);
+
+/*
+ * Rows of the cache as the values that they stand for, (code - zero point) * scale, rounded to dtype: k_out, v_out [B,H,N,D] dense =
+ * positions starts[b] + n, n < counts[b]; zeros for the others and for tokens without a place.
+ */
+int qfa_paged_read(const qfa_paged_cache *cache, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts,
+                   const int32_t *counts, void *k_out, void *v_out, int dtype, int64_t B, int64_t N, void *stream);
+
+/*
+ * Attention of the tokens at the end of every sequence on its pages:
+ *     O = softmax(sm_scale * Q^ K^^T) V^,   Q^, K^, V^ = scale * (codes - zero_point) per token
+ * with qfa_attn_fwd_cache's arithmetic.  Token n < counts[b] sees the keys j <= starts[b] + n (causal 0: j < starts[b] + counts[b]);
+ * tokens from counts[b] on, and tokens that see no key, get zeros.  Keys past the table's width or on a page that is not in
+ * [0, pages) are hidden.  What hidden rows of the cache hold is irrelevant.
+ *   q [B,H,N,D] of q_dtype with strides as in qfa_attn_fwd; H a multiple of the cache's heads: query head h reads key head
+ *     h / (H / cache->H).  o [B,H,N,D] of q_dtype, dense.
+ *   prefix  the first `prefix` keys are the same for all sequences: they are read once, from sequence 0's pages.
+ *   workspace  qfa_attn_paged_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant; one for each call under way.
+ * The lengths are read on the device: a captured call follows them.  Keys are dealt to workgroups evenly over the whole batch, so
+ * the last bits of a sequence's O depend on the lengths of the others; a call repeated gives the same bits.
+ */
+int64_t qfa_attn_paged_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
+
+int qfa_attn_paged(const qfa_paged_cache *cache, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn, const int32_t *page_table,
+                   int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, void *o, int64_t B, int64_t H, int64_t N,
+                   int64_t prefix, float sm_scale, int causal, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

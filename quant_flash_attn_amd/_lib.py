@@ -21,6 +21,19 @@ _lock = threading.Lock()
 _lib = None
 _host = None
 
+
+class NormRopeTensor(ctypes.Structure):
+    """qfa_norm_rope_tensor"""
+    _fields_ = [("x", c_void_p), ("weight", c_void_p), ("y", c_void_p), ("dy", c_void_p), ("dweight", c_void_p), ("H", c_int64),
+                ("sx", c_int64 * 3), ("sy", c_int64 * 3), ("sdy", c_int64 * 3), ("weight_per_head", c_int)]
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """qfa_paged_cache"""
+    _fields_ = [("k_codes", c_void_p), ("k_scale", c_void_p), ("k_zero", c_void_p), ("v_codes", c_void_p), ("v_scale", c_void_p),
+                ("v_zero", c_void_p), ("pages", c_int64), ("H", c_int64), ("page_size", c_int), ("D", c_int), ("scale_dtype", c_int)]
+
+
 # argument lists mirror include/qfa.h one to one
 _P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
 _SIGNATURES = {
@@ -61,6 +74,13 @@ _SIGNATURES = {
     "qfa_attn_bwd_split_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _I, _I]),
     "qfa_attn_bwd_f32_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I]),
     "qfa_attn_bwd_f32": (c_int, [_P] * 13 + [_L] + [_P] * 3 + [_I, _L, _L, _L, _L, _I] + [_L] * 24 + [_F, _I, _P]),
+    "qfa_norm_rope": (c_int, [_P] * 4 + [_L, _I, _I, _P, _L, _L, _I, _F, _I, _I, _L, _L, _I, _P]),
+    "qfa_norm_rope_bwd_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _I]),
+    "qfa_norm_rope_bwd": (c_int, [_P] * 4 + [_L, _I, _I, _P, _L, _L, _I, _F, _I, _I, _L, _L, _I, _P, _L, _P]),
+    "qfa_paged_append": (c_int, [_P, _P, _P, _I] + [_L] * 6 + [_P, _L, _L, _L, _P, _P, _P, _I, _I, _F, _P, _P, _L, _I, _I, _L, _L, _P]),
+    "qfa_paged_read": (c_int, [_P, _P, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _P]),
+    "qfa_attn_paged_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _L]),
+    "qfa_attn_paged": (c_int, [_P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _L, _L, _L, _L, _F, _I, _P, _L, _P]),
     "qfa_attn_bwd": (c_int, [_P] * 13 + [_L] + [_P] * 3 + [_I, _L, _L, _L, _L, _I] + [_L] * 24 + [_F, _I, _P]),
 }
 

@@ -4,7 +4,7 @@
 #include <stdio.h>
 #include <string.h>
 
-#include "qfa_host.h"
+#include "qfa_check.h"
 
 namespace qfa {
 
@@ -26,17 +26,6 @@ int check_launch(const char *what) {
 }
 
 static constexpr int64_t kMaxTokens = 1LL << 28;   // longest sequence (Nq, Nk) the attention entry points take
-static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-static bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
-static bool is_float_dtype(int d) { return d == QFA_F32 || d == QFA_F16 || d == QFA_BF16; }
-static int elem_size(int d) { return d == QFA_F32 ? 4 : 2; }
-
-// strides (elements) of a [B,H,N,D] tensor with element size `es`: positive, 16-byte multiples,
-// and the token stride must at least span a row
-static bool strides_ok(int64_t sb, int64_t sh, int64_t sn, int D, int es) {
-  if (sb <= 0 || sh <= 0 || sn < D) return false;
-  return (sb * es) % 16 == 0 && (sh * es) % 16 == 0 && (sn * es) % 16 == 0;
-}
 
 }  // namespace qfa
 

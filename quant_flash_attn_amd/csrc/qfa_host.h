@@ -179,4 +179,60 @@ struct CacheAttnArgs {
 int launch_cache_fwd(const CacheAttnArgs &a, hipStream_t st);
 int64_t cache_workspace_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Nk, int D);
 
+// RMSNorm of every head's row and the position rotation (qfa_norm_rope.hip), after validation.  Strides: batch, head, token.
+struct NormRopeArgs {
+  struct Tensor {
+    const void *x, *w;      // w: nullable (no norm)
+    void *y;                // backward: dx
+    const void *dy;         // backward only
+    void *dw;               // backward, nullable: of w's type
+    int64_t H, sx[3], sy[3], sg[3];
+    int per_head;           // w is [H, D]
+  } t[2];                   // t[1].H 0: one tensor
+  const float *cos, *sin;
+  const int32_t *pos;       // nullable: position = step * n
+  int64_t rows, spb, spn, B, N;
+  int half, step, interleaved, D, dtype, w_f32;
+  float eps;
+  void *workspace;
+};
+int launch_norm_rope(const NormRopeArgs &a, bool back, hipStream_t st);
+int64_t norm_rope_bwd_workspace_bytes(int64_t tokens, int64_t H0, int64_t H1, int D, bool per_head);
+
+// A paged INT8 cache and its rows' places, after validation
+struct PagedCachePtrs {
+  int8_t *k_codes; void *k_scale; int8_t *k_zero;
+  int8_t *v_codes; void *v_scale; int8_t *v_zero;
+};
+struct PagedRowsArgs {
+  PagedCachePtrs cache;
+  const int32_t *page_table, *starts, *counts;   // counts: nullable
+  int64_t pages, H, width, stb, stw, B, N;
+  int page_log2, scale_dtype, D, dtype;
+  const void *k, *v;        // append
+  int64_t sk[3], sv[3];
+  const void *w;            // nullable
+  const float *cos, *sin;
+  int64_t rope_rows;
+  int half, interleaved, w_f32, w_per_head;
+  float eps;
+  void *k_out, *v_out;      // read: dense [B, H, N, D]
+};
+int launch_paged_rows(const PagedRowsArgs &a, bool read, hipStream_t st);
+
+// Attention of the queries at the end of every sequence on its pages (qfa_paged_attn.hip), after validation
+struct PagedAttnArgs {
+  PagedCachePtrs cache;
+  const int32_t *page_table, *starts, *counts;
+  int64_t pages, Hk, width, stb, stw, B, H, N, prefix;
+  int page_log2, scale_dtype, D, q_dtype, causal;
+  const void *q;
+  void *o;                  // dense [B, H, N, D]
+  int64_t sq[3];
+  float sm_scale;
+  void *workspace;
+};
+int launch_paged_attn(const PagedAttnArgs &a, hipStream_t st);
+int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
+
 }  // namespace qfa

@@ -1,0 +1,488 @@
+// Attention of the queries at the end of every sequence of a batch on the pages of an INT8 cache:
+//     O = softmax(sm_scale * Q^ K^^T) V^,   X^ = scale * (codes - zero_point) per token,
+// with the arithmetic of the kernel for a cache in one piece (qfa_cache.hip): queries quantized per token here, Q K^T on INT8
+// MFMA with the exact zero-point term, V as its exact codes in binary16, softmax statistics and sums in fp32.
+//
+// Bound by reading the cache once (2 D + 6 bytes per key and key head).  A workgroup = 4 waves = 16 rows (queries times the
+// query heads that share a key head) of one sequence and key head, and a piece of its keys (qfa_paged_work.h); 32-key tiles are
+// dealt to the waves, each with its own online softmax.  A tile lives in registers, double-buffered, as there.  A page holds 16
+// keys or a multiple, so the two halves of a tile lie in one page each: their pages' numbers are fetched 32 tiles ahead, one
+// lane per half, and read out of the lanes as scalars, so that no load of keys waits for the page table.
+//
+// What the mask hides may hold anything (pages that were never written): its scores are replaced, its probability is zero and
+// zero wins over whatever its scale holds.
+#include <type_traits>
+
+#include "qfa_host.h"
+#include "qfa_merge.h"
+#include "qfa_paged_work.h"
+#include "qfa_quant_row.h"
+#include "qfa_skv_common.h"
+
+namespace qfa {
+
+struct PagedAttnKernelArgs {
+  PagedWork work;
+  const void *q; const int8_t *kc; const void *ks; const int8_t *kz; const int8_t *vc; const void *vs; const int8_t *vz;
+  void *o;
+  const int32_t *page_table;
+  int64_t pages, stb, stw, sqb, sqh, sqn;
+  int width, page_log2, q_dtype;
+  float sm_scale_log2;
+};
+
+constexpr int PAGED_ROWS = 16;
+constexpr int paged_wgs_per_cu(int D) { return D == 256 ? 1 : 2; }
+// log2 of the largest p' at a new reference, and the p' past which the reference moves (see CACHE_P_REF in qfa_cache.hip)
+constexpr float PAGED_P_REF = 7.0f, PAGED_P_MAX = 0x1p10f;
+
+__device__ __forceinline__ i32x4 paged_mfma_i8(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+
+template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, paged_wgs_per_cu(D)) void paged_rows_kernel(PagedAttnKernelArgs a) {
+  constexpr int KM = D / 64;    // 64-wide k-steps of the score product
+  constexpr int DB = D / 16;    // 16-row blocks of O^T
+  constexpr int VB = D / 16;    // bytes of a V row per lane
+  constexpr int VD = VB / 4;    // ... in dwords
+  constexpr int LPT = D / 8, TPP = 256 / LPT;   // quantizer: lanes per token, tokens per pass
+  // LDS: query codes and constants, per-wave token constants; the merge of the four waves overlays them
+  constexpr int OFF_ST = 16 * D, OFF_TC = OFF_ST + 3 * 16 * 4, MERGE = 4 * 16 * (D + 2) * 4;
+  constexpr int TC = 512 + 128;   // per wave: [64] x (scale, zero point operand), exponents of the 32 values' scales
+  constexpr int TOTAL = MERGE > OFF_TC + 4 * TC ? MERGE : OFF_TC + 4 * TC;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[TOTAL];
+
+  const PagedDeal<SHARED, PAGED_ROWS, SKV_TILE> deal(a.work);
+  unsigned x = blockIdx.x * deal.each;
+  if (x >= deal.total) return;
+  const unsigned x_end = min(x + deal.each, deal.total);
+  const int tid = threadIdx.x, lane = tid % 64, q16 = lane % 16, G = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+
+  struct Tile {
+    i32x4 k[2][KM];
+    unsigned v[8][VD];
+    unsigned sc, zp;   // scale (its bits) and zero point: lanes 0-31 of key lane, lanes 32-63 of value lane - 32
+    int ok;            // bit per half: its page exists
+  };
+  const int k_off = q16 * D + 16 * G, v_off = 4 * G * D + VB * q16;
+  const S *sc_base = reinterpret_cast<const S *>(lane < 32 ? a.ks : a.vs);
+  const int8_t *zp_base = lane < 32 ? a.kz : a.vz;
+  const int page_halves_log2 = a.page_log2 - 4;
+  const i32x4 ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
+  unsigned *tc = reinterpret_cast<unsigned *>(smem + OFF_TC + wave * TC);
+
+  for (auto item = deal.find(x);;) {
+    const int item_tiles = (int)deal.tiles(item.p, item.rb), ntiles = (int)min((unsigned)item_tiles - item.at, x_end - x);
+    const int t0 = deal.begin() / SKV_TILE + (int)item.at;
+    const int my_tiles = ntiles > wave ? (ntiles - wave + 3) / 4 : 0;
+    const int seq = SHARED ? 0 : item.p;   // whose pages
+    const int nrows = min(PAGED_ROWS, deal.rows - PAGED_ROWS * item.rb);
+
+    // pages of this wave's tiles: lane 2 i + half of tile i of 32
+    auto pages_from = [&](int i0) __attribute__((always_inline)) -> int {
+      const int i = i0 + lane / 2, half = 2 * (t0 + wave + 4 * i) + lane % 2, at = half >> page_halves_log2;
+      int id = -1;
+      if (i < my_tiles && at < a.width) id = a.page_table[seq * a.stb + at * a.stw];
+      return id >= 0 && id < a.pages ? id : -1;
+    };
+    int pg = pages_from(0), pg_next = my_tiles > 32 ? pages_from(32) : -1;
+    // (every load is issued whether the tile exists or not -- a missing one has an empty descriptor and fetches nothing)
+    auto load = [&](Tile &t, int i) __attribute__((always_inline)) {
+      if (i > 0 && i % 32 == 0) {
+        pg = pg_next;
+        pg_next = i + 32 < my_tiles ? pages_from(i + 32) : -1;
+      }
+      const int tile = t0 + wave + 4 * i;
+      t.ok = 0;
+      int64_t first[2];   // first row of the half among all rows
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        const int id = __builtin_amdgcn_readlane(pg, 2 * (i % 32) + rb);
+        const bool ok = id >= 0;
+        t.ok |= ok ? 1 << rb : 0;
+        first[rb] = (((int64_t)(ok ? id : 0) * a.work.Hk + item.h) << a.page_log2) + (((2 * tile + rb) & ((1 << page_halves_log2) - 1)) << 4);
+        const rsrc_t rk = make_rsrc(a.kc + first[rb] * D, ok ? 16 * D : 0), rv = make_rsrc(a.vc + first[rb] * D, ok ? 16 * D : 0);
+#pragma unroll
+        for (int m = 0; m < KM; ++m)
+          t.k[rb][m] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off, 64 * m, 0));
+#pragma unroll
+        for (int e = 4 * rb; e < 4 * rb + 4; ++e) {
+          const int soff = (e % 4) * D;
+          if constexpr (VD == 4) {
+            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off, soff, 0));
+#pragma unroll
+            for (int y = 0; y < 4; ++y) t.v[e][y] = w[y];
+          } else if constexpr (VD == 2) {
+            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_off, soff, 0));
+            t.v[e][0] = w[0];
+            t.v[e][1] = w[1];
+          } else {
+            t.v[e][0] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rv, v_off, soff, 0);
+          }
+        }
+      }
+      const int64_t at = (lane % 32 < 16 ? first[0] : first[1]) + lane % 16;
+      if constexpr (sizeof(S) == 4) t.sc = __builtin_bit_cast(unsigned, sc_base[at]);
+      else t.sc = __builtin_bit_cast(unsigned short, sc_base[at]);
+      t.zp = (unsigned)(unsigned char)zp_base[at];
+    };
+
+    Tile ta, tb;
+    load(ta, 0);
+
+    // ---- the block's queries, quantized: codes to LDS, a = scale * sm_scale * log2(e), zero point and c = sum - D * zp
+    float *st_a = reinterpret_cast<float *>(smem + OFF_ST);
+    int *st_z = reinterpret_cast<int *>(smem + OFF_ST + 64), *st_c = reinterpret_cast<int *>(smem + OFF_ST + 128);
+#pragma unroll
+    for (int p = 0; p < (16 + TPP - 1) / TPP; ++p) {
+      const int tok = p * TPP + tid / LPT, sub = tid % LPT;
+      const auto r = deal.row(item.p, item.h, PAGED_ROWS * item.rb + min(tok, nrows - 1));
+      const int64_t off = r.b * a.sqb + r.qh * a.sqh + r.i * a.sqn + sub * 8;
+      float v[8];
+      if (a.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(a.q) + off, v);
+      else if (a.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(a.q) + off, v);
+      else Load8<_Float16>::run(static_cast<const _Float16 *>(a.q) + off, v);
+      const QuantRow<8> row = quant_row<LPT, false, 8>(v, true);
+      if (tok < 16) {
+        *reinterpret_cast<u32x2 *>(smem + tok * D + sub * 8) = u32x2{row.codes[0], row.codes[1]};
+        if (sub == 0) {
+          const float f = row.scale * a.sm_scale_log2;
+          st_a[tok] = f < 0x1p-126f ? 0x1p-126f : f;   // (not zero: the mask's -inf is multiplied by it)
+          st_z[tok] = (int)row.zp;
+          st_c[tok] = row.sum - D * (int)row.zp;
+        }
+      }
+    }
+    __syncthreads();
+    i32x4 qf[KM];
+#pragma unroll
+    for (int m = 0; m < KM; ++m) qf[m] = *reinterpret_cast<const i32x4 *>(smem + q16 * D + 64 * m + 16 * G);
+    const float a_i = st_a[q16];
+    const int zq = st_z[q16], c_i = st_c[q16];
+    // last key of this lane's row; a row that is not there, or brings no token, goes along with the others and is not looked at
+    const int block_end = deal.end(item.p, item.rb) - 1, lo = deal.begin();
+    int lim = block_end;
+    if (q16 < nrows) {
+      const auto r = deal.row(item.p, item.h, PAGED_ROWS * item.rb + q16);
+      const int k = deal.last_key(r);
+      if (r.i < deal.tokens(r.b)) lim = k;
+    }
+    int first_lim = lim;
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) first_lim = min(first_lim, __shfl_xor(first_lim, off, 64));
+    first_lim = __builtin_amdgcn_readfirstlane(first_lim);
+
+    f32x4 oacc[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float ref = NO_KEY, l_run = 0.f, w_run = 0.f;   // p = 2^(a_i * u - ref)
+
+    auto tile = [&](const Tile &t, int i, auto masked_tag) __attribute__((always_inline)) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      const int key0 = (t0 + wave + 4 * i) * SKV_TILE;
+      // token constants: K (scale, zp as an integer), V (scale, the binary16 number 1152 + zp)
+      {
+        u32x2 w;
+        w[0] = __builtin_bit_cast(unsigned, scale_to_f32<S>(t.sc));
+        w[1] = lane < 32 ? (unsigned)(int)(signed char)t.zp : (0x6400u | (t.zp ^ 0x80u));
+        *reinterpret_cast<u32x2 *>(tc + 2 * lane) = w;
+      }
+      // ---- scores of keys 16rb + 4G + v
+      f32x4 f[2];
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        i32x4 s = {0, 0, 0, 0}, rk = {0, 0, 0, 0};
+#pragma unroll
+        for (int m = 0; m < KM; ++m) {
+          s = paged_mfma_i8(t.k[rb][m], qf[m], s);
+          rk = paged_mfma_i8(t.k[rb][m], ones, rk);
+        }
+        const u32x4 c0 = *reinterpret_cast<const u32x4 *>(tc + 2 * (16 * rb + 4 * G)),
+                    c1 = *reinterpret_cast<const u32x4 *>(tc + 2 * (16 * rb + 4 * G) + 4);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const unsigned scw = v < 2 ? c0[2 * v] : c1[2 * v - 4], zw = v < 2 ? c0[2 * v + 1] : c1[2 * v - 3];
+          const int dot = s[v] - __mul24(zq, rk[v]) - __mul24((int)zw, c_i);
+          float u = (float)dot * __builtin_bit_cast(float, scw);
+          const int key = key0 + 16 * rb + 4 * G + v;
+          if (MASKED && (key > lim || key < lo || !(t.ok >> rb & 1))) u = -INFINITY;
+          f[rb][v] = u;
+        }
+      }
+      // ---- p and its row sum, p' = p * scale_j and the largest of them
+      float ps[8], mx = 0.f, l_new = 0.f;
+      unsigned zz[4];   // the binary16 numbers 1152 + zero point
+      u32x4 cv[4];      // keys 16(x/2) + 4G + 2(x%2) + {0, 1}: scale, 1152 + zero point, and again
+#pragma unroll
+      for (int y = 0; y < 4; ++y) cv[y] = *reinterpret_cast<const u32x4 *>(tc + 2 * (32 + 16 * (y / 2) + 4 * G + 2 * (y % 2)));
+      auto probs = [&]() __attribute__((always_inline)) {
+        mx = 0.f;
+        l_new = l_run;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const unsigned s0 = cv[y][0], z0 = cv[y][1], s1 = cv[y][2], z1 = cv[y][3];   // (a bit cast of a vector's element takes element 0)
+          zz[y] = z0 | (z1 << 16);
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, f[y / 2][2 * (y % 2)], -ref));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, f[y / 2][2 * (y % 2) + 1], -ref));
+          l_new += p0 + p1;
+          if (MASKED) {   // what is hidden may hold any scale
+            ps[2 * y] = mul_zero_wins(p0, __builtin_bit_cast(float, s0));
+            ps[2 * y + 1] = mul_zero_wins(p1, __builtin_bit_cast(float, s1));
+          } else {
+            ps[2 * y] = p0 * __builtin_bit_cast(float, s0);
+            ps[2 * y + 1] = p1 * __builtin_bit_cast(float, s1);
+          }
+          mx = fmaxf(mx, fmaxf(fabsf(ps[2 * y]), fabsf(ps[2 * y + 1])));
+        }
+      };
+      // a new reference, common to the four lanes of a row: log2 of the tile's largest p' (and p itself within fp32), but for the
+      // scale's mantissa
+      auto move = [&]() __attribute__((always_inline)) -> float {
+        float *tl = reinterpret_cast<float *>(tc + 128);
+        if (lane >= 32) tl[lane - 32] = __builtin_floorf(__builtin_amdgcn_logf(fabsf((*reinterpret_cast<const f32x2 *>(tc + 2 * lane))[0])));
+        float t_max = -INFINITY, u = -INFINITY;
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+          const f32x4 ls = *reinterpret_cast<const f32x4 *>(tl + 16 * rb + 4 * G);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            t_max = fmaxf(t_max, MASKED && !(f[rb][v] > -INFINITY) ? -INFINITY : __builtin_fmaf(a_i, f[rb][v], ls[v]));
+            u = fmaxf(u, f[rb][v]);
+          }
+        }
+        t_max = fmaxf(t_max - PAGED_P_REF, __builtin_fmaf(a_i, u, -100.0f));
+        t_max = fmaxf(t_max, __shfl_xor(t_max, 16, 64));
+        t_max = fmaxf(t_max, __shfl_xor(t_max, 32, 64));
+        t_max = fmaxf(t_max, ref);
+        const float alpha = __builtin_amdgcn_exp2f(ref - t_max);
+        ref = t_max;
+        return alpha;
+      };
+      if (i == 0) move();   // (nothing summed yet)
+      probs();
+      if (i != 0 && __builtin_amdgcn_ballot_w64(mx > PAGED_P_MAX || !(l_new <= 0x1p100f)) != 0) {
+        const float alpha = move();
+        l_run *= alpha;
+        w_run *= alpha;
+#pragma unroll
+        for (int j = 0; j < DB; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) oacc[j][v] *= alpha;
+        probs();
+      }
+      l_run = l_new;
+      // ---- p' as binary16, offset term
+      u32x4 pf;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const unsigned pp = pack_h2(ps[2 * y], ps[2 * y + 1]);
+        pf[y] = pp;
+        w_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pp), __builtin_bit_cast(f16x2, zz[y]), w_run, false);
+      }
+      // ---- O^T += (1152 + codes)^T . P'^T
+#pragma unroll
+      for (int j = 0; j < DB; ++j) {
+        u32x4 vf;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          constexpr unsigned pick = 0x0c040c00u;
+          vf[e] = __builtin_amdgcn_perm(t.v[2 * e + 1][j / 4], t.v[2 * e][j / 4], pick + (unsigned)(j % 4) * 0x00010001u) ^ 0x64806480u;
+        }
+        oacc[j] = mfma_h16(vf, pf, oacc[j]);
+      }
+    };
+    auto run = [&](const Tile &t, int i) __attribute__((always_inline)) {
+      const int key0 = (t0 + wave + 4 * i) * SKV_TILE;
+      if (key0 + SKV_TILE - 1 > first_lim || key0 < lo || t.ok != 3) tile(t, i, std::true_type{});
+      else tile(t, i, std::false_type{});
+    };
+    for (int i = 0; i < my_tiles; i += 2) {
+      load(tb, i + 1);
+      run(ta, i);
+      load(ta, i + 2);
+      if (i + 1 < my_tiles) run(tb, i + 1);
+    }
+
+    // ---- merge of the four waves, through LDS: [wave][row][D] and (m, l) behind
+    float l_tot = l_run + __shfl_xor(l_run, 16, 64), w_tot = w_run + __shfl_xor(w_run, 16, 64);
+    l_tot += __shfl_xor(l_tot, 32, 64);
+    w_tot += __shfl_xor(w_tot, 32, 64);
+    __syncthreads();   // query codes and token constants are done with
+    float *mg = reinterpret_cast<float *>(smem), *ml = mg + 4 * 16 * D;
+    if (q16 < nrows) {
+      float *dst = mg + (wave * 16 + q16) * D;
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int j = 0; j < DB; j += 4) {
+          f32x4 y;
+#pragma unroll
+          for (int z = 0; z < 4; ++z) y[z] = oacc[j + z][v] - w_tot;
+          *reinterpret_cast<f32x4 *>(dst + VB * (4 * G + v) + j) = y;
+        }
+      if (G == 0) {
+        ml[2 * (wave * 16 + q16)] = ref;
+        ml[2 * (wave * 16 + q16) + 1] = l_tot;
+      }
+    }
+    __syncthreads();
+    const bool whole = item.at == 0 && ntiles == item_tiles;
+    const int64_t slot = ((int64_t)blockIdx.x * 2 + (item.at == 0 ? 1 : 0)) * PAGED_ROWS;
+    for (int y = tid; y < nrows * (D / 4); y += 256) {
+      const int q = y / (D / 4), d = 4 * (y % (D / 4)), r = PAGED_ROWS * item.rb + q;
+      float m = NO_KEY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) m = fmaxf(m, ml[2 * (16 * w + q)]);
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float s = __builtin_amdgcn_exp2f(ml[2 * (16 * w + q)] - m);
+        l += ml[2 * (16 * w + q) + 1] * s;
+        const f32x4 z = *reinterpret_cast<const f32x4 *>(mg + (16 * w + q) * D + d);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += z[e] * s;
+      }
+      if (whole && !a.work.whole) {
+        const auto row = deal.row(item.p, item.h, r);
+        const bool none = row.i >= deal.tokens(row.b) || l == 0.f;
+        const float inv = none ? 0.f : 1.0f / l;
+        const f32x4 out = none ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+        const int64_t off = (((int64_t)row.b * a.work.Hk * a.work.G + row.qh) * a.work.N + row.i) * D;
+        store4(static_cast<char *>(a.o) + off * (a.q_dtype == QFA_F32 ? 4 : 2), a.q_dtype, d, out);
+      } else {
+        const int64_t to = whole ? ((int64_t)item.p * a.work.Hk + item.h) * deal.rows + r : slot + q;
+        float *po = whole ? a.work.whole : a.work.slots, *pml = whole ? a.work.whole_ml : a.work.slots_ml;
+        *reinterpret_cast<f32x4 *>(po + to * D + d) = acc;
+        if (d == 0) *reinterpret_cast<f32x2 *>(pml + 2 * to) = f32x2{m, l};
+      }
+    }
+    x += (unsigned)ntiles;
+    if (x >= x_end) return;
+    deal.next(item);
+    __syncthreads();   // the merge is read
+  }
+}
+
+// O of one row from its pieces: a workgroup per row, D/4 lanes of four columns times 1024/D groups of pieces.  Rows that are in
+// one piece have been stored (no shared prefix); rows that see no key become zeros.
+struct PagedMergeArgs {
+  PagedWork own, shared;   // shared.grid 0: none
+  void *o;
+  int o_dtype;
+};
+struct PagedMerge { float m, l; f32x4 acc; };
+// the pieces of one row in one launch, dealt to `groups` groups
+template <bool SHARED, int D> __device__ __forceinline__ bool paged_pieces(const PagedWork &work, int p, int h, int r, int group, int groups, PagedMerge &x) {
+  const PagedDeal<SHARED, PAGED_ROWS, SKV_TILE> deal(work);
+  const int rb = r / PAGED_ROWS, d = 4 * (threadIdx.x % (D / 4));
+  const unsigned n = deal.tiles(p, rb);
+  if (n == 0) return true;
+  const unsigned first = deal.first_tile(p, h, rb), w0 = first / deal.each, w1 = (first + n - 1) / deal.each;
+  if (w0 == w1 && !work.whole) return false;   // stored
+  for (unsigned w = w0 + group; w <= w1; w += groups) {
+    const int64_t at = w0 == w1 ? ((int64_t)p * work.Hk + h) * deal.rows + r
+                                : ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * PAGED_ROWS + r % PAGED_ROWS;
+    const float *po = w0 == w1 ? work.whole : work.slots, *pml = w0 == w1 ? work.whole_ml : work.slots_ml;
+    const f32x2 ml = *reinterpret_cast<const f32x2 *>(pml + 2 * at);
+    if (ml[1] == 0.f) continue;
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(po + at * D + d);
+    const float m_new = fmaxf(x.m, ml[0]), s0 = __builtin_amdgcn_exp2f(x.m - m_new), s1 = __builtin_amdgcn_exp2f(ml[0] - m_new);
+    x.m = m_new;
+    x.l = x.l * s0 + ml[1] * s1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.acc[e] = x.acc[e] * s0 + y[e] * s1;
+  }
+  return true;
+}
+
+template <int D> __global__ __launch_bounds__(256) void paged_merge_kernel(PagedMergeArgs a) {
+  constexpr int CL = D / 4, SG = 256 / CL;
+  __shared__ float red[SG][D + 4];
+  const int tid = threadIdx.x, d = 4 * (tid % CL), sg = tid / CL;
+  const int rows = a.own.N * a.own.G;
+  const int bh = (int)(blockIdx.x / (unsigned)rows), r = (int)(blockIdx.x % (unsigned)rows), b = bh / a.own.Hk, h = bh % a.own.Hk;
+  const int i = r / a.own.G, qh = h * a.own.G + r % a.own.G;
+  PagedMerge x = {NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+  const int n = a.own.counts ? max(0, min(a.own.counts[b], a.own.N)) : a.own.N;
+  if (i < n) {
+    if (!paged_pieces<false, D>(a.own, b, h, r, sg, SG, x)) return;
+    if (a.shared.grid > 0) paged_pieces<true, D>(a.shared, 0, h, b * rows + r, sg, SG, x);
+  }
+  *reinterpret_cast<f32x4 *>(&red[sg][d]) = x.acc;
+  if (tid % CL == 0) {
+    red[sg][D] = x.m;
+    red[sg][D + 1] = x.l;
+  }
+  __syncthreads();
+  if (sg > 0) return;
+  float m = NO_KEY, l = 0.f;
+#pragma unroll
+  for (int s = 0; s < SG; ++s) m = fmaxf(m, red[s][D]);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < SG; ++s) {
+    const float w = __builtin_amdgcn_exp2f(red[s][D] - m);
+    l += red[s][D + 1] * w;
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(&red[s][d]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += y[e] * w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const int64_t off = (((int64_t)b * a.own.Hk * a.own.G + qh) * a.own.N + i) * D;
+  store4(static_cast<char *>(a.o) + off * (a.o_dtype == QFA_F32 ? 4 : 2), a.o_dtype, d, f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv});
+}
+
+// bytes of a launch's slots, and of its whole items
+static int64_t slots_bytes(int D) { return 2LL * 256 * paged_wgs_per_cu(D) * PAGED_ROWS * (D + 2) * 4; }
+static int64_t whole_bytes(int64_t rows, int D) { return (rows * (D + 2) * 4 + 15) / 16 * 16; }
+int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t, int64_t N, int D, int64_t prefix) {
+  return prefix > 0 ? 2 * (slots_bytes(D) + whole_bytes(B * H * N, D)) : slots_bytes(D);
+}
+
+template <typename S, int D> static int launch_sd(const PagedAttnArgs &x, hipStream_t st) {
+  PagedAttnKernelArgs a;
+  a.q = x.q; a.kc = x.cache.k_codes; a.ks = x.cache.k_scale; a.kz = x.cache.k_zero;
+  a.vc = x.cache.v_codes; a.vs = x.cache.v_scale; a.vz = x.cache.v_zero; a.o = x.o; a.page_table = x.page_table;
+  a.pages = x.pages; a.stb = x.stb; a.stw = x.stw; a.sqb = x.sq[0]; a.sqh = x.sq[1]; a.sqn = x.sq[2];
+  a.width = (int)x.width; a.page_log2 = x.page_log2; a.q_dtype = x.q_dtype;
+  a.sm_scale_log2 = x.sm_scale * kLog2e;
+  const int grid = 256 * paged_wgs_per_cu(D);
+  const int64_t rows = x.B * x.H * x.N, slots = 2LL * grid * PAGED_ROWS;
+  PagedWork w[2];
+  float *mem = static_cast<float *>(x.workspace);
+  for (int i = 0; i < 2; ++i) {
+    w[i] = {x.starts, x.counts, (int)x.B, (int)x.Hk, (int)(x.H / x.Hk), (int)x.N, x.causal, (int)x.prefix,
+            (int)(x.width << x.page_log2), x.prefix > 0 || i == 0 ? grid : 0, 8, nullptr, nullptr, nullptr, nullptr};
+    if (w[i].grid == 0) continue;
+    w[i].slots = mem;
+    w[i].slots_ml = mem + slots * D;
+    mem += slots_bytes(D) / 4;
+    if (x.prefix > 0) {
+      w[i].whole = mem;
+      w[i].whole_ml = mem + rows * D;
+      mem += whole_bytes(rows, D) / 4;
+    }
+  }
+  if (w[1].grid) {
+    a.work = w[1];
+    paged_rows_kernel<S, D, true><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
+    if (int e = check_launch("qfa_attn_paged (prefix)")) return e;
+  }
+  a.work = w[0];
+  paged_rows_kernel<S, D, false><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
+  if (int e = check_launch("qfa_attn_paged")) return e;
+  const PagedMergeArgs m = {w[0], w[1], x.o, x.q_dtype};
+  paged_merge_kernel<D><<<dim3((unsigned)rows), dim3(256), 0, st>>>(m);
+  return check_launch("qfa_attn_paged (merge)");
+}
+template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
+  if (x.scale_dtype == QFA_F32) return launch_sd<float, D>(x, st);
+  if (x.scale_dtype == QFA_F16) return launch_sd<_Float16, D>(x, st);
+  return launch_sd<__bf16, D>(x, st);
+}
+int launch_paged_attn(const PagedAttnArgs &x, hipStream_t st) {
+  if (x.D == 64) return launch_d<64>(x, st);
+  if (x.D == 128) return launch_d<128>(x, st);
+  return launch_d<256>(x, st);
+}
+
+}  // namespace qfa

@@ -56,6 +56,13 @@ struct Api {
   QFA_ENTRY(qfa_attn_fwd_cache_lse);
   QFA_ENTRY(qfa_dout_normalise_workspace_bytes);
   QFA_ENTRY(qfa_dout_normalise_cast);
+  QFA_ENTRY(qfa_norm_rope);
+  QFA_ENTRY(qfa_norm_rope_bwd_workspace_bytes);
+  QFA_ENTRY(qfa_norm_rope_bwd);
+  QFA_ENTRY(qfa_paged_append);
+  QFA_ENTRY(qfa_paged_read);
+  QFA_ENTRY(qfa_attn_paged_workspace_bytes);
+  QFA_ENTRY(qfa_attn_paged);
 #undef QFA_ENTRY
 };
 Api api;
@@ -92,6 +99,13 @@ void init(const py::dict &address) {
   QFA_ENTRY(qfa_attn_fwd_cache_lse);
   QFA_ENTRY(qfa_dout_normalise_workspace_bytes);
   QFA_ENTRY(qfa_dout_normalise_cast);
+  QFA_ENTRY(qfa_norm_rope);
+  QFA_ENTRY(qfa_norm_rope_bwd_workspace_bytes);
+  QFA_ENTRY(qfa_norm_rope_bwd);
+  QFA_ENTRY(qfa_paged_append);
+  QFA_ENTRY(qfa_paged_read);
+  QFA_ENTRY(qfa_attn_paged_workspace_bytes);
+  QFA_ENTRY(qfa_attn_paged);
 #undef QFA_ENTRY
 }
 
@@ -424,9 +438,9 @@ void refuse_tangents(std::initializer_list<const Tensor *> ts) {
 // A call that is being traced goes through the dispatcher, which records the operator as one node of the graph (what the
 // function below does by itself is invisible there but for its allocations); others save themselves that round trip.
 template <typename F> struct Traced;
-template <typename... A> struct Traced<Tensor(A...)> {
-  static Tensor call(const char *name, A... args) {
-    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Tensor(A...)>().call(args...);
+template <typename R, typename... A> struct Traced<R(A...)> {
+  static R call(const char *name, A... args) {
+    return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<R(A...)>().call(args...);
   }
 };
 
@@ -888,6 +902,8 @@ Tensor shared(const Tensor &q, const Tensor &kv_fp16, const Tensor &codes, const
   return shared_op(q, kv_fp16, codes, scale, zp, sm, max_q);
 }
 
+#include "qfa_torch_paged.inc"
+
 }  // namespace
 
 // (no backend key: the operators attach their autograd nodes themselves)
@@ -897,6 +913,11 @@ TORCH_LIBRARY(quant_flash_attn_amd, m) {
         "Tensor v_codes, Tensor v_scale, Tensor v_zero_point, bool causal, float sm_scale) -> Tensor", &cache_op);
   m.def("shared_kv(Tensor q, Tensor kv_fp16, Tensor codes, Tensor scale, Tensor zero_point, float sm_scale, int max_q) -> Tensor",
         &shared_op);
+  m.def("norm_rope(Tensor x, Tensor? weight, Tensor? cos, Tensor? sin, Tensor? positions, float eps, bool interleaved) -> Tensor", &norm_rope_op);
+  m.def("norm_rope_pair(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor? cos, Tensor? sin, Tensor? positions, float eps, "
+        "bool interleaved) -> (Tensor, Tensor)", &norm_rope_pair_op);
+  m.def("paged(Tensor q, Tensor k_codes, Tensor k_scale, Tensor k_zero_point, Tensor v_codes, Tensor v_scale, Tensor v_zero_point, "
+        "Tensor page_table, Tensor starts, Tensor? counts, bool causal, float sm_scale, int prefix_len) -> Tensor", &paged_attn_op);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -919,4 +940,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   }, nogil());
   m.def("normalised_dout", &normalised_dout, nogil());
   m.def("shared", &shared, nogil());
+  m.def("norm_rope", &norm_rope, nogil());
+  m.def("norm_rope_pair", &norm_rope_pair, nogil());
+  m.def("paged_append", &paged_append, nogil());
+  m.def("paged_read", &paged_read, nogil());
+  m.def("paged_attn", &paged_attn, nogil());
 }
