@@ -15,26 +15,14 @@
 
 #include "qfa_host.h"
 #include "qfa_merge.h"
-#include "qfa_paged_work.h"
+#include "qfa_paged_attn.h"
 #include "qfa_quant_row.h"
 #include "qfa_skv_common.h"
 
 namespace qfa {
 
-struct PagedAttnKernelArgs {
-  PagedWork work;
-  const void *q; const int8_t *kc; const void *ks; const int8_t *kz; const int8_t *vc; const void *vs; const int8_t *vz;
-  void *o;
-  const int32_t *page_table;
-  int64_t pages, stb, stw, sqb, sqh, sqn;
-  int width, page_log2, q_dtype;
-  float sm_scale_log2;
-};
-
 constexpr int PAGED_ROWS = 16;
 constexpr int paged_wgs_per_cu(int D) { return D == 256 ? 1 : 2; }
-// log2 of the largest p' at a new reference, and the p' past which the reference moves (see CACHE_P_REF in qfa_cache.hip)
-constexpr float PAGED_P_REF = 7.0f, PAGED_P_MAX = 0x1p10f;
 
 __device__ __forceinline__ i32x4 paged_mfma_i8(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
@@ -50,10 +38,13 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
   constexpr int TOTAL = MERGE > OFF_TC + 4 * TC ? MERGE : OFF_TC + 4 * TC;
   __shared__ __attribute__((aligned(16))) unsigned char smem[TOTAL];
 
-  const PagedDeal<SHARED, PAGED_ROWS, SKV_TILE> deal(a.work);
-  unsigned x = blockIdx.x * deal.each;
-  if (x >= deal.total) return;
-  const unsigned x_end = min(x + deal.each, deal.total);
+  typedef PagedDeal<SHARED, true> Deal;
+  Deal deal(a.work, PAGED_ROWS, SKV_TILE);
+  unsigned x;
+  typename Deal::Item item;
+  if (!deal.find(x, item)) return;
+  const unsigned x_end = min((blockIdx.x + 1) * deal.each, deal.total);
+  if (x >= x_end) return;
   const int tid = threadIdx.x, lane = tid % 64, q16 = lane % 16, G = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
 
@@ -70,8 +61,8 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
   const i32x4 ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
   unsigned *tc = reinterpret_cast<unsigned *>(smem + OFF_TC + wave * TC);
 
-  for (auto item = deal.find(x);;) {
-    const int item_tiles = (int)deal.tiles(item.p, item.rb), ntiles = (int)min((unsigned)item_tiles - item.at, x_end - x);
+  for (;;) {
+    const int ntiles = (int)min(item.tiles - item.at, x_end - x);
     const int t0 = deal.begin() / SKV_TILE + (int)item.at;
     const int my_tiles = ntiles > wave ? (ntiles - wave + 3) / 4 : 0;
     const int seq = SHARED ? 0 : item.p;   // whose pages
@@ -126,6 +117,27 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
       t.zp = (unsigned)(unsigned char)zp_base[at];
     };
 
+    // the block's queries are requested beside the pages, and quantized while the first keys are on their way
+    constexpr int PASSES = (16 + TPP - 1) / TPP;
+    float qv[PASSES][8];
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+      const int tok = p * TPP + tid / LPT, sub = tid % LPT;
+      const auto r = deal.row(item.p, item.h, PAGED_ROWS * item.rb + min(tok, nrows - 1));
+      const int64_t off = r.b * a.sqb + r.qh * a.sqh + r.i * a.sqn + sub * 8;
+      if (a.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(a.q) + off, qv[p]);
+      else if (a.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(a.q) + off, qv[p]);
+      else Load8<_Float16>::run(static_cast<const _Float16 *>(a.q) + off, qv[p]);
+    }
+    // last key of this lane's row; a row that is not there, or brings no token, goes along with the others and is not looked at
+    const int block_end = deal.end(item.s, item.rb) - 1, lo = deal.begin();
+    int lim = block_end;
+    if (q16 < nrows) {
+      const auto r = deal.row(item.p, item.h, PAGED_ROWS * item.rb + q16);
+      const PagedSeq s = SHARED ? deal.load(r.b) : item.s;
+      if (r.i < s.tokens) lim = deal.last_key(r, s);
+    }
+
     Tile ta, tb;
     load(ta, 0);
 
@@ -133,15 +145,9 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
     float *st_a = reinterpret_cast<float *>(smem + OFF_ST);
     int *st_z = reinterpret_cast<int *>(smem + OFF_ST + 64), *st_c = reinterpret_cast<int *>(smem + OFF_ST + 128);
 #pragma unroll
-    for (int p = 0; p < (16 + TPP - 1) / TPP; ++p) {
+    for (int p = 0; p < PASSES; ++p) {
       const int tok = p * TPP + tid / LPT, sub = tid % LPT;
-      const auto r = deal.row(item.p, item.h, PAGED_ROWS * item.rb + min(tok, nrows - 1));
-      const int64_t off = r.b * a.sqb + r.qh * a.sqh + r.i * a.sqn + sub * 8;
-      float v[8];
-      if (a.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(a.q) + off, v);
-      else if (a.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(a.q) + off, v);
-      else Load8<_Float16>::run(static_cast<const _Float16 *>(a.q) + off, v);
-      const QuantRow<8> row = quant_row<LPT, false, 8>(v, true);
+      const QuantRow<8> row = quant_row<LPT, false, 8>(qv[p], true);
       if (tok < 16) {
         *reinterpret_cast<u32x2 *>(smem + tok * D + sub * 8) = u32x2{row.codes[0], row.codes[1]};
         if (sub == 0) {
@@ -158,14 +164,6 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
     for (int m = 0; m < KM; ++m) qf[m] = *reinterpret_cast<const i32x4 *>(smem + q16 * D + 64 * m + 16 * G);
     const float a_i = st_a[q16];
     const int zq = st_z[q16], c_i = st_c[q16];
-    // last key of this lane's row; a row that is not there, or brings no token, goes along with the others and is not looked at
-    const int block_end = deal.end(item.p, item.rb) - 1, lo = deal.begin();
-    int lim = block_end;
-    if (q16 < nrows) {
-      const auto r = deal.row(item.p, item.h, PAGED_ROWS * item.rb + q16);
-      const int k = deal.last_key(r);
-      if (r.i < deal.tokens(r.b)) lim = k;
-    }
     int first_lim = lim;
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) first_lim = min(first_lim, __shfl_xor(first_lim, off, 64));
@@ -325,7 +323,11 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
       }
     }
     __syncthreads();
-    const bool whole = item.at == 0 && ntiles == item_tiles;
+    const bool whole = item.at == 0 && ntiles == (int)item.tiles;
+    if (!SHARED && item.at == 0 && tid == 0) {   // where the pieces are, for those who join them
+      a.work.first[2 * deal.item_index(item.p, item.h, item.rb)] = item.first;
+      a.work.first[2 * deal.item_index(item.p, item.h, item.rb) + 1] = deal.each;
+    }
     const int64_t slot = ((int64_t)blockIdx.x * 2 + (item.at == 0 ? 1 : 0)) * PAGED_ROWS;
     for (int y = tid; y < nrows * (D / 4); y += 256) {
       const int q = y / (D / 4), d = 4 * (y % (D / 4)), r = PAGED_ROWS * item.rb + q;
@@ -343,7 +345,7 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
       }
       if (whole && !a.work.whole) {
         const auto row = deal.row(item.p, item.h, r);
-        const bool none = row.i >= deal.tokens(row.b) || l == 0.f;
+        const bool none = row.i >= item.s.tokens || l == 0.f;   // (not of a shared prefix)
         const float inv = none ? 0.f : 1.0f / l;
         const f32x4 out = none ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
         const int64_t off = (((int64_t)row.b * a.work.Hk * a.work.G + row.qh) * a.work.N + row.i) * D;
@@ -356,128 +358,169 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
       }
     }
     x += (unsigned)ntiles;
-    if (x >= x_end) return;
-    deal.next(item);
+    if (x >= x_end || !deal.next(x, x_end, item)) return;
     __syncthreads();   // the merge is read
   }
 }
 
-// O of one row from its pieces: a workgroup per row, D/4 lanes of four columns times 1024/D groups of pieces.  Rows that are in
-// one piece have been stored (no shared prefix); rows that see no key become zeros.
+// O from the pieces of its rows: a workgroup joins up to 16 rows of one sequence and key head, D/4 lanes of four columns each; with
+// fewer rows than 1024/D the pieces of a row are dealt to several groups of lanes, which meet in LDS.  Rows that lie in one piece
+// have been stored already (no shared prefix); rows that see no key become zeros.
 struct PagedMergeArgs {
   PagedWork own, shared;   // shared.grid 0: none
   void *o;
-  int o_dtype;
+  int o_dtype, chunks, chunk_rows;   // chunks of rows of a sequence and key head, a power of two that divides a block
 };
-struct PagedMerge { float m, l; f32x4 acc; };
-// the pieces of one row in one launch, dealt to `groups` groups
-template <bool SHARED, int D> __device__ __forceinline__ bool paged_pieces(const PagedWork &work, int p, int h, int r, int group, int groups, PagedMerge &x) {
-  const PagedDeal<SHARED, PAGED_ROWS, SKV_TILE> deal(work);
-  const int rb = r / PAGED_ROWS, d = 4 * (threadIdx.x % (D / 4));
-  const unsigned n = deal.tiles(p, rb);
-  if (n == 0) return true;
-  const unsigned first = deal.first_tile(p, h, rb), w0 = first / deal.each, w1 = (first + n - 1) / deal.each;
-  if (w0 == w1 && !work.whole) return false;   // stored
-  for (unsigned w = w0 + group; w <= w1; w += groups) {
-    const int64_t at = w0 == w1 ? ((int64_t)p * work.Hk + h) * deal.rows + r
-                                : ((int64_t)w * 2 + (w == w0 ? 1 : 0)) * PAGED_ROWS + r % PAGED_ROWS;
-    const float *po = w0 == w1 ? work.whole : work.slots, *pml = w0 == w1 ? work.whole_ml : work.slots_ml;
-    const f32x2 ml = *reinterpret_cast<const f32x2 *>(pml + 2 * at);
-    if (ml[1] == 0.f) continue;
-    const f32x4 y = *reinterpret_cast<const f32x4 *>(po + at * D + d);
-    const float m_new = fmaxf(x.m, ml[0]), s0 = __builtin_amdgcn_exp2f(x.m - m_new), s1 = __builtin_amdgcn_exp2f(ml[0] - m_new);
+// Where a row's pieces are
+struct PagedPieces {
+  unsigned w0 = 1, w1 = 0;       // workgroups that have one (none)
+  int64_t whole = -1;            // row among the items in one piece
+  int in_block = 0;
+  __device__ __forceinline__ PagedPieces(unsigned first, unsigned each, unsigned n, int64_t whole_row, int in_block_) {
+    if (n == 0) return;
+    w0 = first / each;
+    w1 = (first + n - 1) / each;
+    in_block = in_block_;
+    if (w0 == w1) whole = whole_row;
+  }
+};
+struct PagedSum { float m, l; f32x4 acc; };
+template <int D> __device__ __forceinline__ void paged_add(const PagedWork &work, const PagedPieces &at, int d, int group, int groups, PagedSum &x) {
+  const float *po = at.whole >= 0 ? work.whole : work.slots, *pml = at.whole >= 0 ? work.whole_ml : work.slots_ml;
+#pragma unroll 4
+  for (unsigned w = at.w0 + group; w <= at.w1; w += groups) {
+    const int64_t i = at.whole >= 0 ? at.whole : ((int64_t)w * 2 + (w == at.w0 ? 1 : 0)) * work.br + at.in_block;
+    const f32x2 ml = *reinterpret_cast<const f32x2 *>(pml + 2 * i);
+    const f32x4 y = *reinterpret_cast<const f32x4 *>(po + i * D + d);
+    const float m_new = ml[1] == 0.f ? x.m : fmaxf(x.m, ml[0]);   // (a piece that saw no key: its sums are zero)
+    const float s0 = __builtin_amdgcn_exp2f(x.m - m_new), s1 = ml[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m_new);
     x.m = m_new;
     x.l = x.l * s0 + ml[1] * s1;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x.acc[e] = x.acc[e] * s0 + y[e] * s1;
+    for (int e = 0; e < 4; ++e) x.acc[e] = x.acc[e] * s0 + mul_zero_wins(s1, y[e]);
   }
-  return true;
 }
 
 template <int D> __global__ __launch_bounds__(256) void paged_merge_kernel(PagedMergeArgs a) {
-  constexpr int CL = D / 4, SG = 256 / CL;
-  __shared__ float red[SG][D + 4];
-  const int tid = threadIdx.x, d = 4 * (tid % CL), sg = tid / CL;
-  const int rows = a.own.N * a.own.G;
-  const int bh = (int)(blockIdx.x / (unsigned)rows), r = (int)(blockIdx.x % (unsigned)rows), b = bh / a.own.Hk, h = bh % a.own.Hk;
-  const int i = r / a.own.G, qh = h * a.own.G + r % a.own.G;
-  PagedMerge x = {NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
-  const int n = a.own.counts ? max(0, min(a.own.counts[b], a.own.N)) : a.own.N;
-  if (i < n) {
-    if (!paged_pieces<false, D>(a.own, b, h, r, sg, SG, x)) return;
-    if (a.shared.grid > 0) paged_pieces<true, D>(a.shared, 0, h, b * rows + r, sg, SG, x);
-  }
-  *reinterpret_cast<f32x4 *>(&red[sg][d]) = x.acc;
-  if (tid % CL == 0) {
-    red[sg][D] = x.m;
-    red[sg][D + 1] = x.l;
-  }
-  __syncthreads();
-  if (sg > 0) return;
-  float m = NO_KEY, l = 0.f;
+  constexpr int CL = D / 4, SLOTS = 256 / CL;
+  __shared__ float red[SLOTS][D + 4];
+  const int tid = threadIdx.x, d = 4 * (tid % CL), slot = tid / CL;
+  const PagedDeal<false, false> own(a.own, a.own.br, a.own.tk);
+  const int bh = (int)(blockIdx.x / (unsigned)a.chunks), chunk = (int)(blockIdx.x % (unsigned)a.chunks), b = bh / a.own.Hk, h = bh % a.own.Hk;
+  const int r0 = chunk * a.chunk_rows, n = min(a.chunk_rows, own.rows - r0), rb = r0 / own.BR;
+  const unsigned *note = a.own.first + 2 * own.item_index(b, h, rb), first = note[0], each = max(note[1], 1u);   // (nobody's, without tiles)
+  const PagedSeq seq = own.load(b);
+  const PagedPieces mine(first, each, own.tiles(seq, rb), (int64_t)bh * own.rows + r0, r0 % own.BR);
+  if (!a.own.whole && mine.whole >= 0) return;   // stored
+  const int groups = n >= SLOTS ? 1 : SLOTS / n;   // of pieces
+  for (int first = 0; first < n; first += SLOTS) {
+    const int k = groups == 1 ? first + slot : slot % n, group = groups == 1 ? 0 : slot / n;   // row of the chunk
+    const bool live = k < n && group < groups;
+    const int r = r0 + min(k, n - 1), i = r / a.own.G;
+    PagedSum x = {NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+    if (live && i < seq.tokens) {
+      PagedPieces p = mine;
+      p.in_block += r - r0;
+      if (p.whole >= 0) p.whole += r - r0;
+      paged_add<D>(a.own, p, d, group, groups, x);
+      if (a.shared.grid > 0) {
+        const PagedDeal<true, false> all(a.shared, a.shared.br, a.shared.tk);
+        const int rs = b * own.rows + r, item = h * all.blocks + rs / all.BR;
+        const unsigned u = all.units({0, 0}, 0);
+        const PagedPieces q((unsigned)item * u + (unsigned)a.shared.extra, all.each, all.tiles({0, 0}, 0), (int64_t)h * all.rows + rs, rs % all.BR);
+        paged_add<D>(a.shared, q, d, group, groups, x);
+      }
+    }
+    if (groups > 1) {
+      *reinterpret_cast<f32x4 *>(&red[slot][d]) = x.acc;
+      if (tid % CL == 0) {
+        red[slot][D] = x.m;
+        red[slot][D + 1] = x.l;
+      }
+      __syncthreads();
+      if (slot >= n) return;
+      x = {NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+      for (int g = 0; g < groups; ++g) x.m = fmaxf(x.m, red[g * n + slot][D]);
+      for (int g = 0; g < groups; ++g) {
+        const float s = __builtin_amdgcn_exp2f(red[g * n + slot][D] - x.m);
+        x.l += red[g * n + slot][D + 1] * s;
+        const f32x4 y = *reinterpret_cast<const f32x4 *>(&red[g * n + slot][d]);
 #pragma unroll
-  for (int s = 0; s < SG; ++s) m = fmaxf(m, red[s][D]);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int s = 0; s < SG; ++s) {
-    const float w = __builtin_amdgcn_exp2f(red[s][D] - m);
-    l += red[s][D + 1] * w;
-    const f32x4 y = *reinterpret_cast<const f32x4 *>(&red[s][d]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += y[e] * w;
+        for (int e = 0; e < 4; ++e) x.acc[e] += y[e] * s;
+      }
+    } else if (!live) {
+      return;
+    }
+    const float inv = x.l == 0.f ? 0.f : 1.0f / x.l;
+    const int64_t off = (((int64_t)b * a.own.Hk * a.own.G + h * a.own.G + r % a.own.G) * a.own.N + i) * D;
+    store4(static_cast<char *>(a.o) + off * (a.o_dtype == QFA_F32 ? 4 : 2), a.o_dtype, d,
+           f32x4{x.acc[0] * inv, x.acc[1] * inv, x.acc[2] * inv, x.acc[3] * inv});
   }
-  const float inv = l == 0.f ? 0.f : 1.0f / l;
-  const int64_t off = (((int64_t)b * a.own.Hk * a.own.G + qh) * a.own.N + i) * D;
-  store4(static_cast<char *>(a.o) + off * (a.o_dtype == QFA_F32 ? 4 : 2), a.o_dtype, d, f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv});
 }
 
+// Rows of a block in a launch over problems of that many rows: one block of 16, the tiles' 64 or 128 beyond
+static int block_rows(int64_t rows) { return rows <= PAGED_ROWS ? PAGED_ROWS : rows <= 64 ? 64 : 128; }
+static int work_grid(int br, int D) { return br == PAGED_ROWS ? 256 * paged_wgs_per_cu(D) : paged_tile_grid(D); }
 // bytes of a launch's slots, and of its whole items
-static int64_t slots_bytes(int D) { return 2LL * 256 * paged_wgs_per_cu(D) * PAGED_ROWS * (D + 2) * 4; }
+static int64_t slots_bytes(int br, int D) { return 2LL * work_grid(br, D) * br * (D + 2) * 4; }
 static int64_t whole_bytes(int64_t rows, int D) { return (rows * (D + 2) * 4 + 15) / 16 * 16; }
-int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t, int64_t N, int D, int64_t prefix) {
-  return prefix > 0 ? 2 * (slots_bytes(D) + whole_bytes(B * H * N, D)) : slots_bytes(D);
+static int64_t first_bytes(int64_t B, int64_t Hk, int64_t rows) { return (8 * B * Hk * ((rows + block_rows(rows) - 1) / block_rows(rows)) + 15) / 16 * 16; }
+int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix) {
+  const int64_t rows = N * (H / Hk), own = slots_bytes(block_rows(rows), D) + first_bytes(B, Hk, rows);
+  return prefix > 0 ? own + slots_bytes(block_rows(B * rows), D) + 2 * whole_bytes(B * H * N, D) : own;
 }
 
-template <typename S, int D> static int launch_sd(const PagedAttnArgs &x, hipStream_t st) {
+template <typename S, int D> static int launch_rows(const PagedAttnKernelArgs &a, bool shared, hipStream_t st) {
+  if (shared) paged_rows_kernel<S, D, true><<<dim3((unsigned)a.work.grid), dim3(256), 0, st>>>(a);
+  else paged_rows_kernel<S, D, false><<<dim3((unsigned)a.work.grid), dim3(256), 0, st>>>(a);
+  return check_launch(shared ? "qfa_attn_paged (prefix)" : "qfa_attn_paged");
+}
+template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
   PagedAttnKernelArgs a;
   a.q = x.q; a.kc = x.cache.k_codes; a.ks = x.cache.k_scale; a.kz = x.cache.k_zero;
   a.vc = x.cache.v_codes; a.vs = x.cache.v_scale; a.vz = x.cache.v_zero; a.o = x.o; a.page_table = x.page_table;
   a.pages = x.pages; a.stb = x.stb; a.stw = x.stw; a.sqb = x.sq[0]; a.sqh = x.sq[1]; a.sqn = x.sq[2];
   a.width = (int)x.width; a.page_log2 = x.page_log2; a.q_dtype = x.q_dtype;
   a.sm_scale_log2 = x.sm_scale * kLog2e;
-  const int grid = 256 * paged_wgs_per_cu(D);
-  const int64_t rows = x.B * x.H * x.N, slots = 2LL * grid * PAGED_ROWS;
+  const int G = (int)(x.H / x.Hk);
+  const int64_t rows = x.B * x.H * x.N, problem[2] = {x.N * G, x.B * x.N * G};
   PagedWork w[2];
   float *mem = static_cast<float *>(x.workspace);
   for (int i = 0; i < 2; ++i) {
-    w[i] = {x.starts, x.counts, (int)x.B, (int)x.Hk, (int)(x.H / x.Hk), (int)x.N, x.causal, (int)x.prefix,
-            (int)(x.width << x.page_log2), x.prefix > 0 || i == 0 ? grid : 0, 8, nullptr, nullptr, nullptr, nullptr};
-    if (w[i].grid == 0) continue;
+    const int br = block_rows(problem[i]), grid = x.prefix > 0 || i == 0 ? work_grid(br, D) : 0;
+    w[i] = {x.starts, x.counts, (int)x.B, (int)x.Hk, G, (int)x.N, x.causal, (int)x.prefix, (int)(x.width << x.page_log2), grid, br,
+            br == PAGED_ROWS ? SKV_TILE : PAGED_TILE, br == PAGED_ROWS ? 8 : 4, nullptr, nullptr, nullptr, nullptr, nullptr};
+    if (grid == 0) continue;
+    if (i == 0) {
+      w[i].first = reinterpret_cast<unsigned *>(mem);
+      mem += first_bytes(x.B, x.Hk, problem[0]) / 4;
+    }
     w[i].slots = mem;
-    w[i].slots_ml = mem + slots * D;
-    mem += slots_bytes(D) / 4;
+    w[i].slots_ml = mem + 2LL * grid * br * D;
+    mem += slots_bytes(br, D) / 4;
     if (x.prefix > 0) {
       w[i].whole = mem;
       w[i].whole_ml = mem + rows * D;
       mem += whole_bytes(rows, D) / 4;
     }
   }
-  if (w[1].grid) {
-    a.work = w[1];
-    paged_rows_kernel<S, D, true><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
-    if (int e = check_launch("qfa_attn_paged (prefix)")) return e;
+  for (int i = 1; i >= 0; --i) {
+    if (w[i].grid == 0) continue;
+    a.work = w[i];
+    int e;
+    if (w[i].br > PAGED_ROWS) e = launch_paged_tile(a, i == 1, D, x.scale_dtype, w[i].br / 32, st);
+    else if (x.scale_dtype == QFA_F32) e = launch_rows<float, D>(a, i == 1, st);
+    else if (x.scale_dtype == QFA_F16) e = launch_rows<_Float16, D>(a, i == 1, st);
+    else e = launch_rows<__bf16, D>(a, i == 1, st);
+    if (e) return e;
   }
-  a.work = w[0];
-  paged_rows_kernel<S, D, false><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
-  if (int e = check_launch("qfa_attn_paged")) return e;
-  const PagedMergeArgs m = {w[0], w[1], x.o, x.q_dtype};
-  paged_merge_kernel<D><<<dim3((unsigned)rows), dim3(256), 0, st>>>(m);
+  // rows per workgroup: few, whose pieces many lanes share, while that leaves no more than 4096 workgroups
+  int chunk_rows = 1;
+  while (chunk_rows < 16 && x.B * x.Hk * ((problem[0] + chunk_rows - 1) / chunk_rows) > 4096) chunk_rows *= 2;
+  const int chunks = (int)((problem[0] + chunk_rows - 1) / chunk_rows);
+  const PagedMergeArgs m = {w[0], w[1], x.o, x.q_dtype, chunks, chunk_rows};
+  paged_merge_kernel<D><<<dim3((unsigned)(x.B * x.Hk * chunks)), dim3(256), 0, st>>>(m);
   return check_launch("qfa_attn_paged (merge)");
-}
-template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
-  if (x.scale_dtype == QFA_F32) return launch_sd<float, D>(x, st);
-  if (x.scale_dtype == QFA_F16) return launch_sd<_Float16, D>(x, st);
-  return launch_sd<__bf16, D>(x, st);
 }
 int launch_paged_attn(const PagedAttnArgs &x, hipStream_t st) {
   if (x.D == 64) return launch_d<64>(x, st);

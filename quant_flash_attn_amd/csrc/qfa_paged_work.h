@@ -1,10 +1,16 @@
 // How the keys of a batch of sequences of any lengths are dealt to a fixed number of workgroups.
 //
 // The lengths are on the device and the host does not wait for them (a captured graph is replayed while they grow), so the
-// division is made here, by every workgroup for itself.  All tiles of keys that the call has to look at are numbered through:
-// sequence by sequence, in it head by head, in it block of rows by block of rows, in it key tile by key tile.  Workgroup w
-// takes the tiles [w * each, (w + 1) * each): every one the same number, whatever the lengths.  Where that cuts an item (one
-// sequence, head and block of rows), the pieces' unnormalised results go to the workgroups' slots and a second kernel joins them.
+// division is made here, by every workgroup for itself.  All work of the call is numbered through in units: sequence by sequence,
+// in it head by head, in it block of rows by block of rows -- an item --, and of an item first a few units for its start and end,
+// then one for every tile of its keys.  Workgroup w takes the units [w * each, (w + 1) * each): every one the same number, whatever
+// the lengths.  Where that cuts an item, the pieces' unnormalised results go to the workgroups' slots and a second kernel joins them.
+// (Without the units for an item's start, a workgroup that gets many short sequences takes several times as long as the others: a
+// start costs the time of about eight tiles.)
+//
+// Every load that another one waits for costs about a microsecond at a workgroup's start, and so do a few thousand bytes of code
+// that no cache holds yet: the lengths of 64 sequences are loaded once, a sequence in each lane, and read out of the lanes from
+// there on; where an item begins is left in memory for the kernel that joins the pieces.
 //
 // Rows of a sequence are its queries times the query heads that share a key head: row = query * G + head % G.
 #pragma once
@@ -19,121 +25,177 @@ struct PagedWork {
   const int32_t *starts, *counts;   // counts: nullable
   int B, Hk, G, N, causal;
   int prefix, capacity;             // keys; what the page table has room for
-  int grid, least;                  // workgroups; the fewest tiles that one of them takes
-  float *slots, *slots_ml;          // [2 * grid][block rows][D] and (m in log2 units, l): of a piece that does not begin its item, one that does
+  int grid;                         // workgroups (0: this launch is not made)
+  int br, tk;                       // rows of a block, keys of a tile: powers of two
+  int extra;                        // units of an item beside its tiles, and the fewest units that a workgroup takes
+  unsigned *first;                  // [items] the unit of an item's first tile, [items] that one's units per workgroup (own keys)
+  float *slots, *slots_ml;          // [2 * grid][br][D] and (m in log2 units, l): of a piece that does not begin its item, one that does
   float *whole, *whole_ml;          // nullable: items in one piece, [problem, head, row] (null: they are normalised and stored)
 };
 
-template <bool SHARED, int BR, int TK> struct PagedDeal {
+// A sequence's position of its first new token, and how many it brings
+struct PagedSeq { int start, tokens; };
+
+// inclusive sum over the wave's lanes (the last one has all of it)
+__device__ __forceinline__ unsigned wave_scan(unsigned x) {
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true);   // row_shr 1, 2, 4, 8
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);  // the row before's last lane, to rows 1 and 3
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);  // the lower half's last lane, to the upper half
+  return x;
+}
+
+// ONE: a problem has a single block of rows
+template <bool SHARED, bool ONE> struct PagedDeal {
   const PagedWork &a;
+  const int BR, TK;                 // work.br and work.tk, constants in the kernels that are made for them
   int rows, blocks, problems;       // rows and blocks of rows of a problem
-  unsigned total, each;
-  __device__ __forceinline__ int tokens(int p) const { return a.counts ? max(0, min(a.counts[p], a.N)) : a.N; }
+  unsigned total, each;             // units of the call, of a workgroup
+  int held;                         // the 64 sequences from here on are in the lanes
+  PagedSeq lanes;
+  __device__ __forceinline__ PagedSeq load(int p) const {
+    const int i = min(p, a.B - 1), n = a.counts ? max(0, min(a.counts[i], a.N)) : a.N;
+    return {a.starts[i], n};
+  }
+  // sequence p, uniform over the wave
+  __device__ __forceinline__ PagedSeq seq(int p) {
+    if (SHARED) return {0, 0};
+    if ((p & ~63) != held) {
+      held = p & ~63;
+      lanes = load(held + threadIdx.x % 64);
+    }
+    return {__builtin_amdgcn_readlane(lanes.start, p & 63), __builtin_amdgcn_readlane(lanes.tokens, p & 63)};
+  }
   // the keys of a block of rows end here
-  __device__ __forceinline__ int end(int p, int rb) const {
+  __device__ __forceinline__ int end(const PagedSeq &s, int rb) const {
     if (SHARED) return min(a.prefix, a.capacity);
-    const int n = tokens(p), first = rb * BR / a.G;
-    if (first >= n) return 0;
-    const int64_t last = a.causal ? min(((rb + 1) * BR - 1) / a.G, n - 1) : n - 1;
-    return (int)max((int64_t)0, min((int64_t)a.starts[p] + last + 1, (int64_t)a.capacity));
+    if (s.tokens == 0) return 0;
+    int last = s.tokens - 1;
+    if (!ONE) {
+      if (rb * BR / a.G > last) return 0;
+      if (a.causal) last = min(((rb + 1) * BR - 1) / a.G, last);
+    }
+    return (int)max((int64_t)0, min((int64_t)s.start + last + 1, (int64_t)a.capacity));
   }
   __device__ __forceinline__ int begin() const { return SHARED ? 0 : a.prefix; }
-  __device__ __forceinline__ unsigned tiles(int p, int rb) const {
-    const int e = end(p, rb), b = begin();
+  __device__ __forceinline__ unsigned tiles(const PagedSeq &s, int rb) const {
+    const int e = end(s, rb), b = begin();
     return e > b ? (unsigned)((e + TK - 1) / TK - b / TK) : 0u;
   }
-  __device__ __forceinline__ unsigned tiles_of_problem(int p) const {   // of one head
-    if (SHARED || !a.causal) return (unsigned)blocks * tiles(p, 0) - (SHARED ? 0u : missing(p));
-    unsigned s = 0;
-    for (int rb = 0; rb < blocks; ++rb) s += tiles(p, rb);
-    return s;
+  __device__ __forceinline__ unsigned units(const PagedSeq &s, int rb) const {
+    const unsigned n = tiles(s, rb);
+    return n ? n + (unsigned)a.extra : 0u;
   }
-  // not causal: all blocks see the same keys, but for those behind the last token
-  __device__ __forceinline__ unsigned missing(int p) const {
-    const int n = tokens(p), with = (n * a.G + BR - 1) / BR;
-    return (unsigned)(blocks - with) * tiles(p, 0);
+  __device__ __forceinline__ unsigned units_of_head(const PagedSeq &s) const {
+    if (ONE) return units(s, 0);
+    if (SHARED) return (unsigned)blocks * units(s, 0);
+    if (!a.causal) return (unsigned)((s.tokens * a.G + BR - 1) / BR) * units(s, 0);   // (all blocks with a token see the same keys)
+    unsigned sum = 0;
+    for (int rb = 0; rb < blocks; ++rb) sum += units(s, rb);
+    return sum;
   }
-  // (every wave adds up for itself: 64 problems at a time, nothing to wait for but their lengths)
-  __device__ __forceinline__ unsigned below(int p, unsigned x) const { return p < problems ? x : 0u; }
-  __device__ __forceinline__ PagedDeal(const PagedWork &a_) : a(a_) {
+  __device__ __forceinline__ void divide() { each = max((unsigned)a.extra, (total + a.grid - 1) / a.grid); }
+  __device__ __forceinline__ PagedDeal(const PagedWork &a_, int br, int tk) : a(a_), BR(br), TK(tk) {
     rows = (SHARED ? a.B : 1) * a.N * a.G;
-    blocks = (rows + BR - 1) / BR;
+    blocks = ONE ? 1 : (rows + BR - 1) / BR;
     problems = SHARED ? 1 : a.B;
-    unsigned sum = 0;
-    for (int p = threadIdx.x % 64; p < problems; p += 64) sum += tiles_of_problem(p);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    total = __builtin_amdgcn_readfirstlane((int)(sum * (unsigned)a.Hk));
-    each = max((unsigned)a.least, (total + a.grid - 1) / a.grid);
-  }
-  // Number of the first tile of an item
-  __device__ __forceinline__ unsigned first_tile(int p, int h, int rb) const {
-    unsigned sum = 0;
-    for (int i = threadIdx.x % 64; i < p; i += 64) sum += tiles_of_problem(i);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    sum = sum * (unsigned)a.Hk + (unsigned)h * tiles_of_problem(p);
-    for (int i = 0; i < rb; ++i) sum += tiles(p, i);
-    return __builtin_amdgcn_readfirstlane((int)sum);
-  }
-  // The item that tile x < total belongs to, and which of its tiles it is
-  struct Item { int p, h, rb; unsigned at; };
-  __device__ __forceinline__ Item find(unsigned x) const {
-    const int lane = threadIdx.x % 64;
-    unsigned before = 0;
-    Item it = {0, 0, 0, 0u};
-    for (int base = 0; base < problems; base += 64) {
-      const unsigned mine = base + lane < problems ? tiles_of_problem(base + lane) * (unsigned)a.Hk : 0u;
-      unsigned sum = mine;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const unsigned y = __shfl_up(sum, off, 64);
-        if (lane >= off) sum += y;
-      }
-      const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > x);
-      if (past != 0) {
-        const int l = __builtin_ctzll(past);
-        it.p = base + l;
-        it.at = x - before - __builtin_amdgcn_readlane((int)(sum - mine), l);
-        break;
-      }
-      before += __builtin_amdgcn_readlane((int)sum, 63);
+    held = 0;
+    if (SHARED) {
+      total = units_of_head({0, 0}) * (unsigned)a.Hk;
+      divide();
     }
-    const unsigned per_head = __builtin_amdgcn_readfirstlane((int)tiles_of_problem(it.p));
-    it.h = (int)(it.at / per_head);
-    it.at -= (unsigned)it.h * per_head;
-    for (unsigned t; it.rb < blocks - 1 && it.at >= (t = tiles(it.p, it.rb)); ++it.rb) it.at -= t;
-    it.p = __builtin_amdgcn_readfirstlane(it.p);
-    it.h = __builtin_amdgcn_readfirstlane(it.h);
-    it.rb = __builtin_amdgcn_readfirstlane(it.rb);
-    it.at = __builtin_amdgcn_readfirstlane((int)it.at);
-    return it;
   }
-  // the next item that has tiles (there is one)
-  __device__ __forceinline__ void next(Item &it) const {
+  // An item, its sequence, which of its `tiles` tiles is the next, and the unit of its first one
+  struct Item { int p, h, rb; unsigned at, tiles, first; PagedSeq s; };
+  // Divides the work and finds unit blockIdx.x * each.  False: there is no such unit.  (x moves on to an item's first tile.)
+  __device__ __forceinline__ bool find(unsigned &x, Item &it) {
+    unsigned in = 0;   // which unit of the problem
+    it.p = 0;
+    it.s = {0, 0};
+    if (SHARED) {
+      x = blockIdx.x * each;
+      if (x >= total) return false;
+      in = x;
+    } else {
+      const int lane = threadIdx.x % 64;
+      lanes = load(lane);
+      unsigned mine = lane < problems ? units_of_head(lanes) * (unsigned)a.Hk : 0u, sum = wave_scan(mine);
+      total = (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
+      for (int base = 64; base < problems; base += 64) {
+        const unsigned u = base + lane < problems ? units_of_head(load(base + lane)) * (unsigned)a.Hk : 0u;
+        total += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(u), 63);
+      }
+      divide();
+      x = blockIdx.x * each;
+      if (x >= total) return false;
+      unsigned before = 0;
+      for (;;) {
+        const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > x);
+        if (past != 0) {
+          const int l = __builtin_ctzll(past);
+          it.p = held + l;
+          in = x - before - (unsigned)__builtin_amdgcn_readlane((int)(sum - mine), l);
+          break;
+        }
+        before += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);   // (x < total: a later sequence has it)
+        held += 64;
+        lanes = load(held + lane);
+        mine = held + lane < problems ? units_of_head(lanes) * (unsigned)a.Hk : 0u;
+        sum = wave_scan(mine);
+      }
+      it.s = seq(it.p);
+    }
+    const unsigned per_head = __builtin_amdgcn_readfirstlane((int)units_of_head(it.s));
+    it.h = __builtin_amdgcn_readfirstlane((int)(in / per_head));
+    in -= (unsigned)it.h * per_head;
+    it.rb = 0;
+    if (!ONE) {
+      if (SHARED || !a.causal) {
+        it.rb = (int)(in / units(it.s, 0));
+        in -= (unsigned)it.rb * units(it.s, 0);
+      } else {
+        for (unsigned t; it.rb < blocks - 1 && in >= (t = units(it.s, it.rb)); ++it.rb) in -= t;
+      }
+      it.rb = __builtin_amdgcn_readfirstlane(it.rb);
+    }
+    in = __builtin_amdgcn_readfirstlane((int)in);
+    it.tiles = __builtin_amdgcn_readfirstlane((int)tiles(it.s, it.rb));
+    it.first = x - in + (unsigned)a.extra;
+    if (in < (unsigned)a.extra) x = it.first;
+    it.at = x - it.first;
+    return x < total;
+  }
+  // the next item that has tiles, behind unit x where the last one ended; false: that is not this workgroup's
+  __device__ __forceinline__ bool next(unsigned &x, unsigned x_end, Item &it) {
+    x += (unsigned)a.extra;
+    if (x >= x_end) return false;
+    it.first = x;
     it.at = 0;
-    do {
-      if (++it.rb == blocks) {
+    do {   // (x_end is at most the last item's end: there is one)
+      if (ONE || ++it.rb == blocks) {
         it.rb = 0;
         if (++it.h == a.Hk) {
           it.h = 0;
-          ++it.p;
+          it.s = seq(++it.p);
         }
       }
-    } while (tiles(it.p, it.rb) == 0);
+      it.tiles = __builtin_amdgcn_readfirstlane((int)tiles(it.s, it.rb));
+    } while (it.tiles == 0);
+    return true;
   }
+  __device__ __forceinline__ int item_index(int p, int h, int rb) const { return (p * a.Hk + h) * blocks + rb; }
   // Row r of problem p: its sequence, query and query head (of key head h)
   struct Row { int b, i, qh; };
   __device__ __forceinline__ Row row(int p, int h, int r) const {
     const int per = a.N * a.G, b = SHARED ? r / per : p, in = SHARED ? r - b * per : r;
-    const int i = in / a.G;
+    const int i = a.N == 1 ? 0 : in / a.G;
     return {b, i, h * a.G + in - i * a.G};
   }
-  // The last key that a row sees (-1 and below: none)
-  __device__ __forceinline__ int last_key(const Row &r) const {
-    const int n = tokens(r.b);
-    if (r.i >= n) return -1;
-    const int64_t k = (int64_t)a.starts[r.b] + (a.causal ? r.i : n - 1);
+  // The last key that a row sees (-1 and below: none).  s: its sequence
+  __device__ __forceinline__ int last_key(const Row &r, const PagedSeq &s) const {
+    const int64_t k = (int64_t)s.start + (a.causal ? r.i : s.tokens - 1);
     return (int)max((int64_t)-1, min(k, (int64_t)(SHARED ? a.prefix : a.capacity) - 1));
   }
 };
