@@ -68,6 +68,8 @@ static int check_cache(const char *who, const qfa_paged_cache *c) {
   if (!is_float_dtype(c->scale_dtype)) return set_error(QFA_EINVAL, "%s: scale_dtype %d is not QFA_F32/F16/BF16", who, c->scale_dtype);
   if (c->pages <= 0 || c->H <= 0) return set_error(QFA_EINVAL, "%s: pages and H must be positive", who);
   if (!head_dim_ok(c->D)) return set_error(QFA_EUNSUPPORTED, "%s: head_dim %d not in {64, 128, 256}", who, c->D);
+  if ((double)c->pages * (double)c->H * (double)c->page_size > 4294967295.0)
+    return set_error(QFA_EUNSUPPORTED, "%s: a cache holds fewer than 2^32 rows of keys", who);
   if (c->page_size < 16 || c->page_size > (1 << 20) || (c->page_size & (c->page_size - 1)))
     return set_error(QFA_EUNSUPPORTED, "%s: page size %d: a power of two from 16 on is needed", who, c->page_size);
   return 0;

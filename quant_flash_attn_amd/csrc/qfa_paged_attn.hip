@@ -11,8 +11,6 @@
 //
 // What the mask hides may hold anything (pages that were never written): its scores are replaced, its probability is zero and
 // zero wins over whatever its scale holds.
-#include <type_traits>
-
 #include "qfa_host.h"
 #include "qfa_merge.h"
 #include "qfa_paged_attn.h"
@@ -174,8 +172,7 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
     for (int i = 0; i < DB; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float ref = NO_KEY, l_run = 0.f, w_run = 0.f;   // p = 2^(a_i * u - ref)
 
-    auto tile = [&](const Tile &t, int i, auto masked_tag) __attribute__((always_inline)) {
-      constexpr bool MASKED = decltype(masked_tag)::value;
+    auto tile = [&](const Tile &t, int i) __attribute__((always_inline)) {
       const int key0 = (t0 + wave + 4 * i) * SKV_TILE;
       // token constants: K (scale, zp as an integer), V (scale, the binary16 number 1152 + zp)
       {
@@ -200,11 +197,16 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
         for (int v = 0; v < 4; ++v) {
           const unsigned scw = v < 2 ? c0[2 * v] : c1[2 * v - 4], zw = v < 2 ? c0[2 * v + 1] : c1[2 * v - 3];
           const int dot = s[v] - __mul24(zq, rk[v]) - __mul24((int)zw, c_i);
-          float u = (float)dot * __builtin_bit_cast(float, scw);
-          const int key = key0 + 16 * rb + 4 * G + v;
-          if (MASKED && (key > lim || key < lo || !(t.ok >> rb & 1))) u = -INFINITY;
-          f[rb][v] = u;
+          f[rb][v] = (float)dot * __builtin_bit_cast(float, scw);
         }
+      }
+      if (key0 + SKV_TILE - 1 > first_lim || key0 < lo || t.ok != 3) {
+        const int last = lim - key0 - 4 * G, first = lo - key0 - 4 * G;   // (this lane's keys are key0 + 4 G + 16 rb + v)
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (16 * rb + v > last || 16 * rb + v < first || !(t.ok >> rb & 1)) f[rb][v] = -INFINITY;
       }
       // ---- p and its row sum, p' = p * scale_j and the largest of them
       float ps[8], mx = 0.f, l_new = 0.f;
@@ -222,13 +224,8 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
           const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, f[y / 2][2 * (y % 2)], -ref));
           const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, f[y / 2][2 * (y % 2) + 1], -ref));
           l_new += p0 + p1;
-          if (MASKED) {   // what is hidden may hold any scale
-            ps[2 * y] = mul_zero_wins(p0, __builtin_bit_cast(float, s0));
-            ps[2 * y + 1] = mul_zero_wins(p1, __builtin_bit_cast(float, s1));
-          } else {
-            ps[2 * y] = p0 * __builtin_bit_cast(float, s0);
-            ps[2 * y + 1] = p1 * __builtin_bit_cast(float, s1);
-          }
+          ps[2 * y] = mul_zero_wins(p0, __builtin_bit_cast(float, s0));   // (what is hidden may hold any scale)
+          ps[2 * y + 1] = mul_zero_wins(p1, __builtin_bit_cast(float, s1));
           mx = fmaxf(mx, fmaxf(fabsf(ps[2 * y]), fabsf(ps[2 * y + 1])));
         }
       };
@@ -243,7 +240,7 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
           const f32x4 ls = *reinterpret_cast<const f32x4 *>(tl + 16 * rb + 4 * G);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            t_max = fmaxf(t_max, MASKED && !(f[rb][v] > -INFINITY) ? -INFINITY : __builtin_fmaf(a_i, f[rb][v], ls[v]));
+            t_max = fmaxf(t_max, !(f[rb][v] > -INFINITY) ? -INFINITY : __builtin_fmaf(a_i, f[rb][v], ls[v]));
             u = fmaxf(u, f[rb][v]);
           }
         }
@@ -288,16 +285,11 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
         oacc[j] = mfma_h16(vf, pf, oacc[j]);
       }
     };
-    auto run = [&](const Tile &t, int i) __attribute__((always_inline)) {
-      const int key0 = (t0 + wave + 4 * i) * SKV_TILE;
-      if (key0 + SKV_TILE - 1 > first_lim || key0 < lo || t.ok != 3) tile(t, i, std::true_type{});
-      else tile(t, i, std::false_type{});
-    };
     for (int i = 0; i < my_tiles; i += 2) {
       load(tb, i + 1);
-      run(ta, i);
+      tile(ta, i);
       load(ta, i + 2);
-      if (i + 1 < my_tiles) run(tb, i + 1);
+      if (i + 1 < my_tiles) tile(tb, i + 1);
     }
 
     // ---- merge of the four waves, through LDS: [wave][row][D] and (m, l) behind
@@ -465,9 +457,12 @@ static int work_grid(int br, int D) { return br == PAGED_ROWS ? 256 * paged_wgs_
 static int64_t slots_bytes(int br, int D) { return 2LL * work_grid(br, D) * br * (D + 2) * 4; }
 static int64_t whole_bytes(int64_t rows, int D) { return (rows * (D + 2) * 4 + 15) / 16 * 16; }
 static int64_t first_bytes(int64_t B, int64_t Hk, int64_t rows) { return (8 * B * Hk * ((rows + block_rows(rows) - 1) / block_rows(rows)) + 15) / 16 * 16; }
+static int64_t quantized_bytes(int64_t rows, int D) { return (rows * D + 4 * rows + rows + 15) / 16 * 16; }
 int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix) {
   const int64_t rows = N * (H / Hk), own = slots_bytes(block_rows(rows), D) + first_bytes(B, Hk, rows);
-  return prefix > 0 ? own + slots_bytes(block_rows(B * rows), D) + 2 * whole_bytes(B * H * N, D) : own;
+  // (16 rows or fewer are quantized by those who use them)
+  const int64_t q = rows > PAGED_ROWS || (prefix > 0 && B * rows > PAGED_ROWS) ? quantized_bytes(B * H * N, D) : 0;
+  return prefix > 0 ? own + q + slots_bytes(block_rows(B * rows), D) + 2 * whole_bytes(B * H * N, D) : own + q;
 }
 
 template <typename S, int D> static int launch_rows(const PagedAttnKernelArgs &a, bool shared, hipStream_t st) {
@@ -476,7 +471,7 @@ template <typename S, int D> static int launch_rows(const PagedAttnKernelArgs &a
   return check_launch(shared ? "qfa_attn_paged (prefix)" : "qfa_attn_paged");
 }
 template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
-  PagedAttnKernelArgs a;
+  PagedAttnKernelArgs a = {};
   a.q = x.q; a.kc = x.cache.k_codes; a.ks = x.cache.k_scale; a.kz = x.cache.k_zero;
   a.vc = x.cache.v_codes; a.vs = x.cache.v_scale; a.vz = x.cache.v_zero; a.o = x.o; a.page_table = x.page_table;
   a.pages = x.pages; a.stb = x.stb; a.stw = x.stw; a.sqb = x.sq[0]; a.sqh = x.sq[1]; a.sqn = x.sq[2];
@@ -503,6 +498,16 @@ template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
       w[i].whole_ml = mem + rows * D;
       mem += whole_bytes(rows, D) / 4;
     }
+  }
+  if (w[0].br > PAGED_ROWS || (w[1].grid > 0 && w[1].br > PAGED_ROWS)) {   // many rows: quantized once, every piece of keys needs them
+    int8_t *codes = reinterpret_cast<int8_t *>(mem), *zero = codes + rows * (D + 4);
+    float *scale = reinterpret_cast<float *>(codes + rows * D);
+    // (one token each: a sequence's heads as tokens of one head, which fill the quantizer's workgroups)
+    const bool one = x.N == 1;
+    if (int e = launch_quant(x.q, x.q_dtype, codes, scale, nullptr, 0, zero, nullptr, x.B, one ? 1 : x.H, one ? x.H : x.N, D, x.sq[0], one ? x.sq[2] : x.sq[1],
+                             one ? x.sq[1] : x.sq[2], x.H * x.N * D, one ? D : x.N * D, D, st))
+      return e;
+    a.q_codes = codes; a.q_scale = scale; a.q_zero = zero;
   }
   for (int i = 1; i >= 0; --i) {
     if (w[i].grid == 0) continue;

@@ -10,12 +10,9 @@
 // A wave takes 32 rows.  Four waves side by side (128 rows) take both blocks of 32 keys of a tile, two (64 rows) share them with the
 // other two and meet in LDS at the end.  The next tile's codes are on their way in registers while a tile is worked on; pieces of
 // the keys are dealt as qfa_paged_work.h says.
-#include <type_traits>
-
 #include "qfa_host.h"
 #include "qfa_merge.h"
 #include "qfa_paged_attn.h"
-#include "qfa_quant_row.h"
 #include "qfa_skv_tile.h"
 
 namespace qfa {
@@ -25,10 +22,9 @@ template <int D, int QW> struct PagedTileGeom {
   static constexpr int CPR = D / 16, SLAB = TK * 32 + 128;
   static constexpr int SIDE = CPR * SLAB;               // one side's expanded tile
   static constexpr int CONST_K = 2 * SIDE, CONST_V = CONST_K + TK * 4, CONST_L = CONST_V + TK * 4;   // scales of both, log2 of V's
-  static constexpr int BUF = CONST_L + TK * 4;
-  static constexpr int QROW = 2 * D + 16;               // a query row on its way into operands
+  static constexpr int CONST_X = CONST_L + TK * 4, BUF = CONST_X + TK * 4;
   static constexpr int MERGE = (D / 2 + 2) * 256;       // partial result of a wave
-  static_assert(BR * QROW <= 2 * BUF && (KW - 1) * QW * MERGE <= 2 * BUF, "what overlays the tiles");
+  static_assert((KW - 1) * QW * MERGE <= 2 * BUF, "what overlays the tiles");
 };
 
 // A thread's share of one side of a tile: N chunks of 16 codes with their rows' zero points
@@ -39,14 +35,13 @@ template <int D> struct PagedChunks {
   unsigned z[N];
 };
 
-template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(PagedAttnKernelArgs a, int scale_dtype) {
+template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(PagedAttnKernelArgs a_, int scale_dtype) {
   typedef PagedTileGeom<D, QW> GM;
   typedef PagedChunks<D> Chunks;
   constexpr int TK = GM::TK, NB = GM::NB, KW = GM::KW, BR = GM::BR, DB = D / 32, KD = D / 16, SLAB = GM::SLAB;
-  constexpr int LPT = D / 8, TPP = 256 / LPT;   // quantizer: lanes per row, rows per pass
   __shared__ __attribute__((aligned(256))) unsigned char smem[2 * GM::BUF];
-  __shared__ float row_a[BR];
 
+  const PagedAttnKernelArgs &a = a_;
   typedef PagedDeal<SHARED, false> Deal;
   Deal deal(a.work, BR, TK);
   unsigned x;
@@ -63,7 +58,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
   // a thread's chunks: 4 columns of chunks by 4 rows per 16 lanes, as SkvTileStage has them
   // (made again where it is needed, from a lane that is opaque there: kept over the tiles it would cost registers that are not there)
   constexpr int CH = GM::CPR / 4;
-  const int quarter_mask = (1 << page_quarters_log2) - 1;
+  const unsigned quarter_mask = (1u << page_quarters_log2) - 1;
   auto opaque = [](int y) __attribute__((always_inline)) -> int {
     asm volatile("" : "+v"(y));
     return y;
@@ -78,134 +73,122 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
     const int slot = (wave + item.h) % QW;   // (turned by the head: waves without rows should not all sit on the same SIMD)
     const bool active = 32 * slot < nrows;
 
-    // pages of 16 tiles: lane 4 t + quarter
-    auto pages_from = [&](int first) __attribute__((always_inline)) -> int {
-      const int l = opaque(lane), t = first + l / 4, quarter = 4 * (t0 + t) + l % 4, at = quarter >> page_quarters_log2;
-      int id = -1;
-      if (t < nt && at < a.width) id = a.page_table[seq * a.stb + at * a.stw];
-      return id >= 0 && id < a.pages ? id : -1;
+    // pages of 16 tiles (lane 4 t + quarter): requested, and made into their first rows among all pages' rows (counted in 32 bits, see
+    // qfa_paged_api.cpp) where that is needed.  A page that is not there: some other one's rows, hidden
+    int pg;
+    unsigned first_row = 0;
+    uint64_t pages_ok = 0;
+    auto request_pages = [&](int t) __attribute__((always_inline)) {
+      const int l = opaque(lane);
+      pg = a.page_table[seq * a.stb + min((4 * (t0 + t) + l) >> page_quarters_log2, a.width - 1) * a.stw];
     };
-    int pg = pages_from(0);
+    auto take_pages = [&](int t) __attribute__((always_inline)) {
+      const int l = opaque(lane), quarter = 4 * (t0 + t) + l;
+      const bool ok = 4 * t + l < 4 * nt && quarter >> page_quarters_log2 < a.width && pg >= 0 && pg < a.pages;
+      pages_ok = __builtin_amdgcn_ballot_w64(ok);
+      first_row = (((unsigned)(ok ? pg : 0) * (unsigned)a.work.Hk + (unsigned)item.h) << a.page_log2) + (((unsigned)quarter & quarter_mask) << 4);
+    };
     Chunks ck, cv;
-    unsigned sc;       // wave 0: scales of the keys, wave 1: of the values
+    unsigned sc;       // even waves: scales of the keys, odd ones: of the values (each of a pair writes the same)
     unsigned ok_next;  // quarters of the tile on its way whose pages are there
-    // request tile t (of a page that is not there: of some other; its keys are hidden)
+    // request tile t
     auto issue = [&](int t) __attribute__((always_inline)) {
-      if (t > 0 && t % 16 == 0) pg = pages_from(t);
-      ok_next = (unsigned)(__builtin_amdgcn_ballot_w64(pg >= 0) >> (4 * (t % 16))) & 15u;
-      const int tile = t0 + t, l = opaque(lane), in = chunk_row(l) % 16, off = in * D + 16 * chunk_col(l);
+      if (t % 16 == 0) {
+        if (t > 0) request_pages(t);
+        take_pages(t);
+      }
+      ok_next = (unsigned)(pages_ok >> (4 * (t % 16))) & 15u;
+      const int l = opaque(lane);
+      const unsigned scale_row = (unsigned)__shfl((int)first_row, 4 * (t % 16) + l / 16, 64) + l % 16;
+      const unsigned in = (unsigned)chunk_row(l) % 16, off = in * D + 16 * (unsigned)chunk_col(l);
 #pragma unroll
       for (int i = 0; i < Chunks::N; ++i) {
         // (chunk i lies STEP rows further: the same row of its 16, another quarter)
         static_assert(Chunks::STEP % 16 == 0, "a thread's chunks differ in the quarter");
         const int quarter = (wave * Chunks::RPW + Chunks::STEP * i) / 16;
-        const int id = __builtin_amdgcn_readlane(pg, 4 * (t % 16) + quarter);
-        const int64_t at = (((int64_t)max(id, 0) * a.work.Hk + item.h) << a.page_log2) + (((4 * tile + quarter) & quarter_mask) << 4);
-        const rsrc_t rk = make_rsrc(a.kc + at * D, 16 * D), rv = make_rsrc(a.vc + at * D, 16 * D);
-        ck.w[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, off, 0, 0));
-        cv.w[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, off, 0, 0));
-        ck.z[i] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(make_rsrc(a.kz + at, 16), in, 0, 0);
-        cv.z[i] = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(make_rsrc(a.vz + at, 16), in, 0, 0);
+        const unsigned at = (unsigned)__builtin_amdgcn_readlane((int)first_row, 4 * (t % 16) + quarter);
+        const int8_t *k = a.kc + (uint64_t)at * D, *v = a.vc + (uint64_t)at * D, *zk = a.kz + at, *zv = a.vz + at;
+        asm("" : "+s"(k), "+s"(v), "+s"(zk), "+s"(zv));   // (scalar bases: else the lanes' 64-bit addresses are kept)
+        ck.w[i] = *reinterpret_cast<const u32x4 *>(k + off);
+        cv.w[i] = *reinterpret_cast<const u32x4 *>(v + off);
+        ck.z[i] = (unsigned char)zk[in];
+        cv.z[i] = (unsigned char)zv[in];
       }
-      if (wave < 2) {
-        const int id = __shfl(pg, 4 * (t % 16) + l / 16, 64);
-        const int64_t at = (((int64_t)max(id, 0) * a.work.Hk + item.h) << a.page_log2) + (((4 * tile + l / 16) & quarter_mask) << 4) + l % 16;
-        const void *p = wave == 0 ? a.ks : a.vs;
-        asm("" : "+s"(p));
-        sc = scale_dtype == QFA_F32 ? static_cast<const unsigned *>(p)[at] : static_cast<const unsigned short *>(p)[at];
-      }
+      const void *p = wave % 2 == 0 ? a.ks : a.vs;
+      sc = scale_dtype == QFA_F32 ? static_cast<const unsigned *>(p)[scale_row] : static_cast<const unsigned short *>(p)[scale_row];
     };
-    auto expand = [&](unsigned char *side, const Chunks &c, int chunk_lds) __attribute__((always_inline)) {
+    request_pages(0);
+    // one chunk of the tile on its way, as binary16 integers code - zero point, into buf (i: the keys' chunks, then the values')
+    auto commit_chunk = [&](unsigned char *buf, int lds, int i) __attribute__((always_inline)) {
+      const Chunks &c = i < Chunks::N ? ck : cv;
+      const int n = i % Chunks::N;
+      const unsigned nz = 0xe400u | (c.z[n] ^ 0x80u), nz2 = nz | nz << 16;   // -(1152 + zero_point), twice
+      const f16x2 neg = __builtin_bit_cast(f16x2, nz2);
+      unsigned char *side = buf + (i < Chunks::N ? 0 : GM::SIDE) + n * (Chunks::STEP * 32);
 #pragma unroll
-      for (int i = 0; i < Chunks::N; ++i) {
-        const unsigned nz = 0xe400u | (c.z[i] ^ 0x80u), nz2 = nz | nz << 16;   // -(1152 + zero_point), twice
-        const f16x2 neg = __builtin_bit_cast(f16x2, nz2);
-        u32x4 e[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const u32x4 m = expand_codes(c.w[i][2 * k], c.w[i][2 * k + 1]);
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const unsigned my = m[y];
-            e[k][y] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, my) + neg);
-          }
-        }
-        *reinterpret_cast<u32x4 *>(side + chunk_lds + i * (Chunks::STEP * 32)) = e[0];
-        *reinterpret_cast<u32x4 *>(side + (chunk_lds ^ 16) + i * (Chunks::STEP * 32)) = e[1];
-      }
-    };
-    auto commit = [&](unsigned char *buf) __attribute__((always_inline)) {
-      const int l = opaque(lane), chunk_lds = skv_tile_off<SLAB>(chunk_row(l), chunk_col(l), 0);
-      expand(buf, ck, chunk_lds);
-      expand(buf + GM::SIDE, cv, chunk_lds);
-      if (wave < 2) {
-        const float f = scale_dtype == QFA_F32 ? __builtin_bit_cast(float, sc) : scale_dtype == QFA_F16 ? lo_to_f32<_Float16>(sc) : lo_to_f32<__bf16>(sc);
-        *reinterpret_cast<float *>(buf + (wave == 0 ? GM::CONST_K : GM::CONST_V) + l * 4) = f;
-        if (wave == 1) *reinterpret_cast<float *>(buf + GM::CONST_L + l * 4) = __builtin_floorf(__builtin_amdgcn_logf(fabsf(f)));
-      }
-    };
-
-    // ---- the block's queries: quantized, code - zero point as binary16 rows in LDS, a = scale * sm_scale * log2(e).  Four passes'
-    // rows are requested together
-    const int tid_q = opaque(tid), sub = tid_q % LPT;
-    constexpr int PASSES = BR / TPP, TOGETHER = PASSES < 4 ? PASSES : 4;
-    // last key of this lane's row; a row that is not there, or brings no token, goes along with the others and is not looked at
-    const int block_end = deal.end(item.s, item.rb) - 1, lo = deal.begin();
-    int lim = block_end;
-    const int row_q = 32 * slot + tid_q % 32;
-    if (row_q < nrows) {
-      const auto r = deal.row(item.p, item.h, BR * item.rb + row_q);
-      const PagedSeq s = SHARED ? deal.load(r.b) : item.s;
-      if (r.i < s.tokens) lim = deal.last_key(r, s);
-    }
-    for (int p0 = 0; p0 < PASSES && p0 * TPP < nrows; p0 += TOGETHER) {
-      float v[TOGETHER][8];
-#pragma unroll
-      for (int p = 0; p < TOGETHER; ++p) {
-        const auto r = deal.row(item.p, item.h, BR * item.rb + min((p0 + p) * TPP + tid_q / LPT, nrows - 1));
-        const int64_t off = r.b * a.sqb + r.qh * a.sqh + r.i * a.sqn + sub * 8;
-        if (a.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(a.q) + off, v[p]);
-        else if (a.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(a.q) + off, v[p]);
-        else Load8<_Float16>::run(static_cast<const _Float16 *>(a.q) + off, v[p]);
-      }
-      if (p0 == 0) issue(0);   // (behind the first rows, which the pages do not wait for)
-#pragma unroll
-      for (int p = 0; p < TOGETHER; ++p) {
-        const int q = (p0 + p) * TPP + tid_q / LPT;
-        const QuantRow<8> row = quant_row<LPT, false, 8>(v[p], true);
-        const u32x4 m = expand_codes(row.codes[0], row.codes[1]);
-        const _Float16 neg = (_Float16)(-1152.0f - row.zp);
-        const f16x2 neg2 = {neg, neg};
+      for (int k = 0; k < 2; ++k) {
+        const u32x4 m = expand_codes(c.w[n][2 * k], c.w[n][2 * k + 1]);
         u32x4 e;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           const unsigned my = m[y];
-          e[y] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, my) + neg2);
+          e[y] = __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, my) + neg);
         }
-        *reinterpret_cast<u32x4 *>(smem + q * GM::QROW + sub * 16) = e;
-        if (sub == 0) {
-          const float f = row.scale * a.sm_scale_log2;
-          row_a[q] = f < 0x1p-126f ? 0x1p-126f : f;   // (not zero: the mask's -inf is multiplied by it)
-        }
+        *reinterpret_cast<u32x4 *>(side + (k == 0 ? lds : lds ^ 16)) = e;
       }
+    };
+    auto commit_scales = [&](unsigned char *buf, int l) __attribute__((always_inline)) {
+      const float f = scale_dtype == QFA_F32 ? __builtin_bit_cast(float, sc) : scale_dtype == QFA_F16 ? lo_to_f32<_Float16>(sc) : lo_to_f32<__bf16>(sc);
+      *reinterpret_cast<float *>(buf + (wave % 2 == 0 ? GM::CONST_K : GM::CONST_V) + l * 4) = f;
+      // (log2 of the keys' scales goes where nobody reads it)
+      *reinterpret_cast<float *>(buf + (wave % 2 == 0 ? GM::CONST_X : GM::CONST_L) + l * 4) = __builtin_floorf(__builtin_amdgcn_logf(fabsf(f)));
+    };
+    auto commit = [&](unsigned char *buf) __attribute__((always_inline)) {
+      const int l = opaque(lane), lds = skv_tile_off<SLAB>(chunk_row(l), chunk_col(l), 0);
+#pragma unroll
+      for (int i = 0; i < 2 * Chunks::N; ++i) commit_chunk(buf, lds, i);
+      commit_scales(buf, l);
+    };
+
+    // ---- this lane's row: half of its codes, as binary16 integers code - zero point (k-step m, k-group g holds columns
+    // 16m + 8g + {0..7}), and a = scale * sm_scale * log2(e).  Rows past the last are zeros.
+    const int row_q = 32 * slot + opaque(lr), block_end = deal.end(item.s, item.rb) - 1, lo = deal.begin();
+    int lim = block_end;   // last key of the row; one that is not there, or brings no token, goes along with the others and is not looked at
+    u32x2 qc[KD];
+    float a_i = 0x1p-126f, zq = 0.f;
+    const bool have = row_q < nrows;
+    {
+      const auto r = deal.row(item.p, item.h, BR * item.rb + min(row_q, nrows - 1));
+      const PagedSeq s = SHARED ? deal.load(r.b) : item.s;
+      const int64_t at = ((int64_t)r.b * a.work.Hk * a.work.G + r.qh) * a.work.N + r.i;
+      const int8_t *codes = a.q_codes + at * D + 8 * g;
+#pragma unroll
+      for (int m = 0; m < KD; ++m) qc[m] = *reinterpret_cast<const u32x2 *>(codes + 16 * m);
+      const float f = a.q_scale[at] * a.sm_scale_log2;
+      zq = (float)a.q_zero[at];
+      if (have) a_i = f < 0x1p-126f ? 0x1p-126f : f;   // (not zero: the mask's -inf is multiplied by it)
+      if (have && r.i < s.tokens) lim = deal.last_key(r, s);
     }
-    __syncthreads();
+    issue(0);
     u32x4 qf[KD];
-    float a_i = 0.f;
-    if (active) {   // (rows past the last hold what is there: their columns of the products are nobody's)
+    {
+      const _Float16 neg = (_Float16)(-1152.0f - zq);
+      const f16x2 neg2 = {neg, neg};
 #pragma unroll
-      for (int m = 0; m < KD; ++m) qf[m] = *reinterpret_cast<const u32x4 *>(smem + (32 * slot + lr) * GM::QROW + 32 * m + 16 * g);
-      a_i = 32 * slot + lr < nrows ? row_a[32 * slot + lr] : 0x1p-126f;
-      if (32 * slot + lr >= nrows) {
+      for (int m = 0; m < KD; ++m) {
+        const unsigned w0 = qc[m][0], w1 = qc[m][1];
+        const u32x4 e = expand_codes(w0, w1);
 #pragma unroll
-        for (int m = 0; m < KD; ++m) qf[m] = u32x4{0u, 0u, 0u, 0u};
+        for (int y = 0; y < 4; ++y) {
+          const unsigned ey = e[y];
+          qf[m][y] = have ? __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, ey) + neg2) : 0u;
+        }
       }
     }
     int first_lim = lim;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) first_lim = min(first_lim, __shfl_xor(first_lim, off, 64));
     first_lim = __builtin_amdgcn_readfirstlane(first_lim);
-    __syncthreads();   // the queries are read
     commit(smem);
     unsigned ok = ok_next;
     if (nt > 1) issue(1);
@@ -217,124 +200,193 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[db][v] = 0.f;
     float ref = NO_KEY, l_run = 0.f;   // p = 2^(a_i * u - ref)
-    bool begun = false;
-
-    // rows kr .. kr + 31 of the tile in buf, whose first key is key0: scores in s
-    auto scores = [&](const unsigned char *buf, int kr, f32x16 &s) __attribute__((always_inline)) {
-      constexpr int AHEAD = KD < 8 ? KD : 8;   // fragments requested together (their registers are free until the probabilities)
+    // ---- Rows kr .. kr + 31 of the tile in buf, and their scores in code units in four steps
+    constexpr int KS = KD / 4;   // k-steps of a step, and of the fragments requested together
+    auto request = [&](const unsigned char *buf, int kr, int step, u32x4 (&kf)[KS]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int v = 0; v < 16; ++v) s[v] = 0.f;
+      for (int m = 0; m < KS; ++m) kf[m] = rd.rows(buf + kr * 32, step * KS + m);
+    };
+    auto scores = [&](f32x16 &s, int step, const u32x4 (&kf)[KS]) __attribute__((always_inline)) {
+      if (step == 0) {
 #pragma unroll
-      for (int m0 = 0; m0 < KD; m0 += AHEAD) {
-        u32x4 kf[AHEAD];
+        for (int v = 0; v < 16; ++v) s[v] = 0.f;
+      }
 #pragma unroll
-        for (int m = 0; m < AHEAD; ++m) kf[m] = rd.rows(buf + kr * 32, m0 + m);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int m = 0; m < KS; ++m) s = mfma_h(kf[m], qf[step * KS + m], s);
+    };
+    auto all_scores = [&](const unsigned char *buf, int kr, f32x16 &s) __attribute__((always_inline)) {
+      u32x4 kf[4][KS];
 #pragma unroll
-        for (int m = 0; m < AHEAD; ++m) s = mfma_h(kf[m], qf[m0 + m], s);
+      for (int i = 0; i < 4; ++i) request(buf, kr, i, kf[i]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) scores(s, i, kf[i]);
+    };
+    // Scales of keys 8 aa + 4 g + {0..3} of rows kr .. and of their values
+    struct Scales { f32x4 k, v; };
+    auto scales = [&](const unsigned char *buf, int kr, int aa) __attribute__((always_inline)) -> Scales {
+      const unsigned char *at = buf + 16 * g + kr * 4 + 32 * aa;
+      return {*reinterpret_cast<const f32x4 *>(at + GM::CONST_K), *reinterpret_cast<const f32x4 *>(at + GM::CONST_V)};
+    };
+    // Those keys' scores times their scales; hidden keys become -inf.  (A branch of its own around the mask and nothing else: with a
+    // masked and an unmasked copy of the whole tile the compiler keeps the accumulators twice.)
+    auto scale = [&](const Scales &c, int kr, int key0, unsigned okb, bool masked, f32x16 &s, int aa) __attribute__((always_inline)) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) s[4 * aa + v] *= c.k[v];
+      if (masked) {
+        const int at0 = key0 + kr + 8 * aa + opaque(4 * g), last = lim - at0, first = lo - at0;
+        const bool page = okb >> (kr / 16 + aa / 2) & 1;
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (v > last || v < first || !page) s[4 * aa + v] = -INFINITY;
       }
     };
-    auto block = [&](const unsigned char *buf, int kr, int key0, unsigned okb, f32x16 &s, auto masked_tag) __attribute__((always_inline)) {
-      constexpr bool MASKED = decltype(masked_tag)::value;
-      const int at0 = key0 + kr + 4 * g, last = lim - at0, first = lo - at0;   // (this lane's keys are at0 + 8 aa + v)
+    // p' = p * scale as binary16, the sum of p, the largest p' as bits (of a negative scale: larger than any limit)
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    struct Probs { u32x4 f[2]; float sum; u16x2 top; };
+    auto probs = [&](const Scales &c, const f32x16 &s, Probs &r, int aa) __attribute__((always_inline)) {
+      if (aa == 0) {
+        r.sum = 0.f;
+        r.top = u16x2{0, 0};
+      }
+      const f32x4 sv = c.v;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, s[4 * aa + 2 * y], -ref)),
+                    p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, s[4 * aa + 2 * y + 1], -ref));
+        r.sum += p0 + p1;
+        const float x0 = mul_zero_wins(p0, sv[2 * y]), x1 = mul_zero_wins(p1, sv[2 * y + 1]);   // (what is hidden may hold any scale)
+        const unsigned w = pack_h2(x0, x1);
+        r.top = __builtin_elementwise_max(r.top, __builtin_bit_cast(u16x2, w));
+        r.f[aa / 2][2 * (aa % 2) + y] = w;
+      }
+    };
+    // A new reference, common to the two lanes of a row (see PAGED_P_REF): the factor for what has been summed up
+    auto move = [&](const unsigned char *buf, int kr, const f32x16 &s) __attribute__((always_inline)) -> float {
+      float t = -INFINITY, u = -INFINITY;
 #pragma unroll
       for (int aa = 0; aa < 4; ++aa) {
-        const f32x4 sk = *reinterpret_cast<const f32x4 *>(buf + GM::CONST_K + (kr + 8 * aa + 4 * g) * 4);
+        const f32x4 ls = *reinterpret_cast<const f32x4 *>(buf + GM::CONST_L + (kr + 8 * aa + 4 * g) * 4);
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          s[4 * aa + v] *= sk[v];
-          if (MASKED && (8 * aa + v > last || 8 * aa + v < first || !(okb >> (kr / 16 + aa / 2) & 1))) s[4 * aa + v] = -INFINITY;
+          const float y = s[4 * aa + v];
+          t = fmaxf(t, !(y > -INFINITY) ? -INFINITY : __builtin_fmaf(a_i, y, ls[v]));
+          u = fmaxf(u, y);
         }
       }
-      float sum, mx;
-      u32x4 pf[2];
-      auto probs = [&]() __attribute__((always_inline)) {
-        sum = 0.f;
-        mx = 0.f;
-        const unsigned char *at = buf + GM::CONST_V + opaque(kr + 4 * g) * 4;   // (opaque: read again for each use, not kept)
-#pragma unroll
-        for (int aa = 0; aa < 4; ++aa) {
-          const f32x4 sv = *reinterpret_cast<const f32x4 *>(at + 32 * aa);
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, s[4 * aa + 2 * y], -ref)),
-                        p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, s[4 * aa + 2 * y + 1], -ref));
-            sum += p0 + p1;
-            // (what is hidden may hold any scale)
-            const float x0 = MASKED ? mul_zero_wins(p0, sv[2 * y]) : p0 * sv[2 * y], x1 = MASKED ? mul_zero_wins(p1, sv[2 * y + 1]) : p1 * sv[2 * y + 1];
-            mx = __builtin_fmaxf(mx, __builtin_fmaxf(fabsf(x0), fabsf(x1)));
-            pf[aa / 2][2 * (aa % 2) + y] = pack_h2(x0, x1);
-          }
-        }
-      };
-      // a new reference, common to the two lanes of a row: see PAGED_P_REF
-      auto move = [&]() __attribute__((always_inline)) -> float {
-        float t = -INFINITY, u = -INFINITY;
-#pragma unroll
-        for (int aa = 0; aa < 4; ++aa) {
-          const f32x4 ls = *reinterpret_cast<const f32x4 *>(buf + GM::CONST_L + (kr + 8 * aa + 4 * g) * 4);
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const float y = s[4 * aa + v];
-            t = fmaxf(t, MASKED && !(y > -INFINITY) ? -INFINITY : __builtin_fmaf(a_i, y, ls[v]));
-            u = fmaxf(u, y);
-          }
-        }
-        t = fmaxf(max_across_halves(fmaxf(t - PAGED_P_REF, __builtin_fmaf(a_i, u, -100.0f))), ref);
-        const float alpha = __builtin_amdgcn_exp2f(ref - t);
-        ref = t;
-        return alpha;
-      };
-      if (!begun) {
-        move();
-        begun = true;
-      }
-      probs();
-      if (__builtin_amdgcn_ballot_w64(mx > PAGED_P_MAX || !(l_run + sum <= 0x1p100f)) != 0) {
-        const float alpha = move();
+      t = fmaxf(max_across_halves(fmaxf(t - PAGED_P_REF, __builtin_fmaf(a_i, u, -100.0f))), ref);
+      const float alpha = __builtin_amdgcn_exp2f(ref - t);
+      ref = t;
+      return alpha;
+    };
+    // The reference moves where some p' (or the sum) has become too large; what was made of it is made again
+    auto check = [&](const unsigned char *buf, int kr, const f32x16 &s, Probs &r) __attribute__((always_inline)) {
+      if (__builtin_amdgcn_ballot_w64(max((unsigned)r.top[0], (unsigned)r.top[1]) > PAGED_P_MAX_BITS || !(l_run + r.sum <= 0x1p100f)) != 0) {
+        const float alpha = move(buf, kr, s);
         l_run *= alpha;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
           for (int v = 0; v < 16; ++v) acc[db][v] *= alpha;
-        probs();
-      }
-      l_run += sum;
-      __builtin_amdgcn_sched_barrier(0);
-      // (columns are requested two products ahead, and not earlier: their registers are needed by then)
-      const unsigned char *p = buf + GM::SIDE + kr * 32;
-      u32x4 vf[2][2] = {{rd.cols(p, 0, 0), rd.cols(p, 0, 1)}, {}};
 #pragma unroll
-      for (int db = 0; db < DB; ++db) {
-        if (db + 1 < DB) {
-          vf[(db + 1) % 2][0] = rd.cols(p, db + 1, 0);
-          vf[(db + 1) % 2][1] = rd.cols(p, db + 1, 1);
+        for (int aa = 0; aa < 4; ++aa) probs(scales(buf, kr, aa), s, r, aa);
+      }
+      l_run += r.sum;
+    };
+    // A tile.  The matrix products of one block of keys run beside the probabilities of the other one, the last ones beside what
+    // makes the next tile out of codes: four steps each, written down in the order in which they are to be issued.  (Left alone, the
+    // compiler puts every kind in a row of its own, a load, a wait and a product at a time, and two waves per SIMD do not fill that.)
+    auto fence = []() __attribute__((always_inline)) { __builtin_amdgcn_sched_barrier(0); };
+    auto tile = [&](const unsigned char *buf, unsigned char *nbuf, int key0, unsigned okb, bool masked) __attribute__((always_inline)) {
+      const int kr = 32 * NB * kw;
+      f32x16 s0, s1;
+      Probs r0, r1;
+      u32x4 kf[2][KS], vf[2][2];
+      // columns 32 db .. of the values of rows kr ..
+      auto columns = [&](int row, int db) __attribute__((always_inline)) {
+        if (db < DB) {
+          const unsigned char *p = buf + GM::SIDE + row * 32;
+          vf[db % 2][0] = rd.cols(p, db, 0);
+          vf[db % 2][1] = rd.cols(p, db, 1);
         }
-        __builtin_amdgcn_sched_barrier(0);
+      };
+      auto product = [&](const Probs &r, int db) __attribute__((always_inline)) {
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) acc[db] = mfma_h(vf[db % 2][hh], pf[hh], acc[db]);
+        for (int hh = 0; hh < 2; ++hh) acc[db] = mfma_h(vf[db % 2][hh], r.f[hh], acc[db]);
+      };
+      // all products with r, and `step` in four parts beside them
+      auto products = [&](const Probs &r, int row, auto step) __attribute__((always_inline)) {
+        constexpr int PER = DB > 4 ? DB / 4 : 1, EVERY = DB < 4 ? 4 / DB : 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+          for (int x = 0; x < PER; ++x) {
+            if (j % EVERY != 0) continue;
+            const int db = j / EVERY * PER + x;
+            columns(row, db + 1);
+            product(r, db);
+          }
+          step(j);
+          fence();
+        }
+      };
+      Scales c[2];
+      all_scores(buf, kr, s0);
+      c[0] = scales(buf, kr, 0);
+      if (NB == 2) request(buf, kr + 32, 0, kf[0]);
+      fence();
+#pragma unroll
+      for (int aa = 0; aa < 4; ++aa) {
+        if (aa < 3) c[(aa + 1) % 2] = scales(buf, kr, aa + 1);
+        else columns(kr, 0);
+        if (NB == 2) {
+          if (aa < 3) request(buf, kr + 32, aa + 1, kf[(aa + 1) % 2]);
+          scores(s1, aa, kf[aa % 2]);
+        }
+        scale(c[aa % 2], kr, key0, okb, masked, s0, aa);
+        probs(c[aa % 2], s0, r0, aa);
+        fence();
       }
+      if (NB == 2) c[0] = scales(buf, kr + 32, 0);
+      check(buf, kr, s0, r0);
+      fence();
+      if (NB == 2) {
+        products(r0, kr, [&](int aa) __attribute__((always_inline)) {
+          if (aa < 3) c[(aa + 1) % 2] = scales(buf, kr + 32, aa + 1);
+          scale(c[aa % 2], kr + 32, key0, okb, masked, s1, aa);
+          probs(c[aa % 2], s1, r1, aa);
+        });
+        columns(kr + 32, 0);
+        check(buf, kr + 32, s1, r1);
+        fence();
+      }
+      const int l = opaque(lane), lds = skv_tile_off<SLAB>(chunk_row(l), chunk_col(l), 0);
+      products(NB == 2 ? r1 : r0, NB == 2 ? kr + 32 : kr, [&](int j) __attribute__((always_inline)) {
+        // (past the last tile: once more what is there)
+        constexpr int N2 = 2 * Chunks::N;
+#pragma unroll
+        for (int i = j * N2 / 4; i < (j + 1) * N2 / 4; ++i) commit_chunk(nbuf, lds, i);
+        if (j == 0) commit_scales(nbuf, l);
+      });
     };
 
+    // the first reference, of the piece's first keys
+    if (active) {
+      f32x16 s;
+      all_scores(smem, 32 * NB * kw, s);
+#pragma unroll
+      for (int aa = 0; aa < 4; ++aa) scale(scales(smem, 32 * NB * kw, aa), 32 * NB * kw, t0 * TK, ok, true, s, aa);
+      move(smem, 32 * NB * kw, s);
+    }
     int cur = 0;
     for (int t = 0; t < nt; ++t) {
       const unsigned char *buf = smem + cur * GM::BUF;
       const int key0 = (t0 + t) * TK;
-      if (active) {
-        const bool masked = key0 + TK - 1 > first_lim || key0 < lo || ok != 15u;
-#pragma unroll 1
-        for (int nb = 0; nb < NB; ++nb) {
-          const int kr = 32 * (NB * kw + nb);
-          f32x16 s;
-          scores(buf, kr, s);
-          __builtin_amdgcn_sched_barrier(0);
-          if (masked) block(buf, kr, key0, ok, s, std::true_type{});
-          else block(buf, kr, key0, ok, s, std::false_type{});
-        }
-      }
       cur ^= 1;
+      unsigned char *nbuf = smem + cur * GM::BUF;
+      if (active) tile(buf, nbuf, key0, ok, key0 + TK - 1 > first_lim || key0 < lo || ok != 15u);
+      else commit(nbuf);
       if (t + 1 < nt) {
-        commit(smem + cur * GM::BUF);
         ok = ok_next;
         if (t + 2 < nt) issue(t + 2);
       }
