@@ -222,34 +222,39 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
 #pragma unroll
       for (int i = 0; i < 4; ++i) scores(s, i, kf[i]);
     };
-    // Scales of keys 8 aa + 4 g + {0..3} of rows kr .. and of their values
-    struct Scales { f32x4 k, v; };
-    auto scales = [&](const unsigned char *buf, int kr, int aa) __attribute__((always_inline)) -> Scales {
-      const unsigned char *at = buf + 16 * g + kr * 4 + 32 * aa;
-      return {*reinterpret_cast<const f32x4 *>(at + GM::CONST_K), *reinterpret_cast<const f32x4 *>(at + GM::CONST_V)};
+    // What keys 8 aa + 4 g + {0..3} of rows kr .. have at `at`: their scales, their values' scales or those's log2
+    auto constants = [&](const unsigned char *buf, int at, int kr, int aa) __attribute__((always_inline)) -> f32x4 {
+      return *reinterpret_cast<const f32x4 *>(buf + at + 16 * g + kr * 4 + 32 * aa);
     };
-    // Those keys' scores times their scales; hidden keys become -inf.  (A branch of its own around the mask and nothing else: with a
-    // masked and an unmasked copy of the whole tile the compiler keeps the accumulators twice.)
-    auto scale = [&](const Scales &c, int kr, int key0, unsigned okb, bool masked, f32x16 &s, int aa) __attribute__((always_inline)) {
+    // The scores times the keys' scales; hidden keys become -inf.  (A branch of its own around the mask and nothing else: with a masked
+    // and an unmasked copy of the whole tile the compiler keeps the accumulators twice; and one for the whole block: it moves what stands
+    // between several of them behind the last one.)
+    auto scale = [&](const unsigned char *buf, int kr, int key0, unsigned okb, bool masked, f32x16 &s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) s[4 * aa + v] *= c.k[v];
+      for (int aa = 0; aa < 4; ++aa) {
+        const f32x4 c = constants(buf, GM::CONST_K, kr, aa);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s[4 * aa + v] *= c[v];
+      }
       if (masked) {
-        const int at0 = key0 + kr + 8 * aa + opaque(4 * g), last = lim - at0, first = lo - at0;
-        const bool page = okb >> (kr / 16 + aa / 2) & 1;
+        const int at0 = key0 + kr + opaque(4 * g), last = lim - at0, first = lo - at0;
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
-          if (v > last || v < first || !page) s[4 * aa + v] = -INFINITY;
+        for (int aa = 0; aa < 4; ++aa) {
+          const bool page = okb >> (kr / 16 + aa / 2) & 1;
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (8 * aa + v > last || 8 * aa + v < first || !page) s[4 * aa + v] = -INFINITY;
+        }
       }
     };
     // p' = p * scale as binary16, the sum of p, the largest p' as bits (of a negative scale: larger than any limit)
     typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     struct Probs { u32x4 f[2]; float sum; u16x2 top; };
-    auto probs = [&](const Scales &c, const f32x16 &s, Probs &r, int aa) __attribute__((always_inline)) {
+    auto probs = [&](const f32x4 &sv, const f32x16 &s, Probs &r, int aa) __attribute__((always_inline)) {
       if (aa == 0) {
         r.sum = 0.f;
         r.top = u16x2{0, 0};
       }
-      const f32x4 sv = c.v;
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, s[4 * aa + 2 * y], -ref)),
@@ -266,7 +271,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
       float t = -INFINITY, u = -INFINITY;
 #pragma unroll
       for (int aa = 0; aa < 4; ++aa) {
-        const f32x4 ls = *reinterpret_cast<const f32x4 *>(buf + GM::CONST_L + (kr + 8 * aa + 4 * g) * 4);
+        const f32x4 ls = constants(buf, GM::CONST_L, kr, aa);
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const float y = s[4 * aa + v];
@@ -289,7 +294,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
 #pragma unroll
           for (int v = 0; v < 16; ++v) acc[db][v] *= alpha;
 #pragma unroll
-        for (int aa = 0; aa < 4; ++aa) probs(scales(buf, kr, aa), s, r, aa);
+        for (int aa = 0; aa < 4; ++aa) probs(constants(buf, GM::CONST_V, kr, aa), s, r, aa);
       }
       l_run += r.sum;
     };
@@ -301,67 +306,73 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
       const int kr = 32 * NB * kw;
       f32x16 s0, s1;
       Probs r0, r1;
-      u32x4 kf[2][KS], vf[2][2];
-      // columns 32 db .. of the values of rows kr ..
+      // fragments on their way: rows of the keys four steps ahead of their products, columns of the values two
+      u32x4 kf[4][KS], vf[DB][2];
       auto columns = [&](int row, int db) __attribute__((always_inline)) {
-        if (db < DB) {
-          const unsigned char *p = buf + GM::SIDE + row * 32;
-          vf[db % 2][0] = rd.cols(p, db, 0);
-          vf[db % 2][1] = rd.cols(p, db, 1);
-        }
+        const unsigned char *p = buf + GM::SIDE + row * 32;
+        vf[db][0] = rd.cols(p, db, 0);
+        vf[db][1] = rd.cols(p, db, 1);
       };
       auto product = [&](const Probs &r, int db) __attribute__((always_inline)) {
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) acc[db] = mfma_h(vf[db % 2][hh], r.f[hh], acc[db]);
+        for (int hh = 0; hh < 2; ++hh) acc[db] = mfma_h(vf[db][hh], r.f[hh], acc[db]);
       };
-      // all products with r, and `step` in four parts beside them
-      auto products = [&](const Probs &r, int row, auto step) __attribute__((always_inline)) {
-        constexpr int PER = DB > 4 ? DB / 4 : 1, EVERY = DB < 4 ? 4 / DB : 1;
+      constexpr int PER = DB > 4 ? DB / 4 : 1, EVERY = DB < 4 ? 4 / DB : 1;   // column blocks of a step, steps of a column block
+      auto step_columns = [&](int row, int j) __attribute__((always_inline)) {
+        if (j % EVERY == 0)
+#pragma unroll
+          for (int x = 0; x < PER; ++x) columns(row, j / EVERY * PER + x);
+      };
+      // all products with r, `step` in four parts beside them; next_row: whose columns come after these (-1: none)
+      auto products = [&](const Probs &r, int row, int next_row, auto step) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          if (j % EVERY == 0) {
 #pragma unroll
-          for (int x = 0; x < PER; ++x) {
-            if (j % EVERY != 0) continue;
-            const int db = j / EVERY * PER + x;
-            columns(row, db + 1);
-            product(r, db);
+            for (int x = 0; x < PER; ++x) product(r, j / EVERY * PER + x);
           }
+          if (j < 2) step_columns(row, j + 2);
+          else if (next_row >= 0) step_columns(next_row, j - 2);
           step(j);
           fence();
         }
       };
-      Scales c[2];
-      all_scores(buf, kr, s0);
-      c[0] = scales(buf, kr, 0);
-      if (NB == 2) request(buf, kr + 32, 0, kf[0]);
+      f32x4 c[2];   // the values' scales
+#pragma unroll
+      for (int i = 0; i < 4; ++i) request(buf, kr, i, kf[i]);
+      fence();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        scores(s0, i, kf[i]);
+        if (NB == 2) request(buf, kr + 32, i, kf[i]);
+      }
+      scale(buf, kr, key0, okb, masked, s0);
+      c[0] = constants(buf, GM::CONST_V, kr, 0);
       fence();
 #pragma unroll
       for (int aa = 0; aa < 4; ++aa) {
-        if (aa < 3) c[(aa + 1) % 2] = scales(buf, kr, aa + 1);
-        else columns(kr, 0);
-        if (NB == 2) {
-          if (aa < 3) request(buf, kr + 32, aa + 1, kf[(aa + 1) % 2]);
-          scores(s1, aa, kf[aa % 2]);
-        }
-        scale(c[aa % 2], kr, key0, okb, masked, s0, aa);
+        if (aa < 3) c[(aa + 1) % 2] = constants(buf, GM::CONST_V, kr, aa + 1);
+        if (NB == 2) scores(s1, aa, kf[aa]);
+        if (aa >= 2) step_columns(kr, aa - 2);
         probs(c[aa % 2], s0, r0, aa);
         fence();
       }
-      if (NB == 2) c[0] = scales(buf, kr + 32, 0);
       check(buf, kr, s0, r0);
+      if (NB == 2) {
+        scale(buf, kr + 32, key0, okb, masked, s1);
+        c[0] = constants(buf, GM::CONST_V, kr + 32, 0);
+      }
       fence();
       if (NB == 2) {
-        products(r0, kr, [&](int aa) __attribute__((always_inline)) {
-          if (aa < 3) c[(aa + 1) % 2] = scales(buf, kr + 32, aa + 1);
-          scale(c[aa % 2], kr + 32, key0, okb, masked, s1, aa);
+        products(r0, kr, kr + 32, [&](int aa) __attribute__((always_inline)) {
+          if (aa < 3) c[(aa + 1) % 2] = constants(buf, GM::CONST_V, kr + 32, aa + 1);
           probs(c[aa % 2], s1, r1, aa);
         });
-        columns(kr + 32, 0);
         check(buf, kr + 32, s1, r1);
         fence();
       }
       const int l = opaque(lane), lds = skv_tile_off<SLAB>(chunk_row(l), chunk_col(l), 0);
-      products(NB == 2 ? r1 : r0, NB == 2 ? kr + 32 : kr, [&](int j) __attribute__((always_inline)) {
+      products(NB == 2 ? r1 : r0, NB == 2 ? kr + 32 : kr, -1, [&](int j) __attribute__((always_inline)) {
         // (past the last tile: once more what is there)
         constexpr int N2 = 2 * Chunks::N;
 #pragma unroll
@@ -374,8 +385,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
     if (active) {
       f32x16 s;
       all_scores(smem, 32 * NB * kw, s);
-#pragma unroll
-      for (int aa = 0; aa < 4; ++aa) scale(scales(smem, 32 * NB * kw, aa), 32 * NB * kw, t0 * TK, ok, true, s, aa);
+      scale(smem, 32 * NB * kw, t0 * TK, ok, true, s);
       move(smem, 32 * NB * kw, s);
     }
     int cur = 0;
