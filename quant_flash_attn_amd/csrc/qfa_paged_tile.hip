@@ -56,7 +56,6 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
   const int page_quarters_log2 = a.page_log2 - 4;   // 16 keys each
 
   // a thread's chunks: 4 columns of chunks by 4 rows per 16 lanes, as SkvTileStage has them
-  // (made again where it is needed, from a lane that is opaque there: kept over the tiles it would cost registers that are not there)
   constexpr int CH = GM::CPR / 4;
   const unsigned quarter_mask = (1u << page_quarters_log2) - 1;
   auto opaque = [](int y) __attribute__((always_inline)) -> int {
@@ -100,7 +99,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
       ok_next = (unsigned)(pages_ok >> (4 * (t % 16))) & 15u;
       const int l = opaque(lane);
       const unsigned scale_row = (unsigned)__shfl((int)first_row, 4 * (t % 16) + l / 16, 64) + l % 16;
-      const unsigned in = (unsigned)chunk_row(l) % 16, off = in * D + 16 * (unsigned)chunk_col(l);
+      const unsigned in = (unsigned)chunk_row(lane) % 16, off = in * D + 16 * (unsigned)chunk_col(lane);
 #pragma unroll
       for (int i = 0; i < Chunks::N; ++i) {
         // (chunk i lies STEP rows further: the same row of its 16, another quarter)
@@ -137,17 +136,18 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
         *reinterpret_cast<u32x4 *>(side + (k == 0 ? lds : lds ^ 16)) = e;
       }
     };
-    auto commit_scales = [&](unsigned char *buf, int l) __attribute__((always_inline)) {
+    auto commit_scales = [&](unsigned char *buf) __attribute__((always_inline)) {
+      const int l = opaque(lane);
       const float f = scale_dtype == QFA_F32 ? __builtin_bit_cast(float, sc) : scale_dtype == QFA_F16 ? lo_to_f32<_Float16>(sc) : lo_to_f32<__bf16>(sc);
       *reinterpret_cast<float *>(buf + (wave % 2 == 0 ? GM::CONST_K : GM::CONST_V) + l * 4) = f;
       // (log2 of the keys' scales goes where nobody reads it)
       *reinterpret_cast<float *>(buf + (wave % 2 == 0 ? GM::CONST_X : GM::CONST_L) + l * 4) = __builtin_floorf(__builtin_amdgcn_logf(fabsf(f)));
     };
     auto commit = [&](unsigned char *buf) __attribute__((always_inline)) {
-      const int l = opaque(lane), lds = skv_tile_off<SLAB>(chunk_row(l), chunk_col(l), 0);
+      const int lds = skv_tile_off<SLAB>(chunk_row(lane), chunk_col(lane), 0);
 #pragma unroll
       for (int i = 0; i < 2 * Chunks::N; ++i) commit_chunk(buf, lds, i);
-      commit_scales(buf, l);
+      commit_scales(buf);
     };
 
     // ---- this lane's row: half of its codes, as binary16 integers code - zero point (k-step m, k-group g holds columns
@@ -308,6 +308,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
       Probs r0, r1;
       // fragments on their way: rows of the keys four steps ahead of their products, columns of the values two
       u32x4 kf[4][KS], vf[DB][2];
+      __builtin_amdgcn_s_setprio(1);   // (the other wave of the SIMD may be making a tile out of codes: 2%)
       auto columns = [&](int row, int db) __attribute__((always_inline)) {
         const unsigned char *p = buf + GM::SIDE + row * 32;
         vf[db][0] = rd.cols(p, db, 0);
@@ -371,13 +372,14 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
         check(buf, kr + 32, s1, r1);
         fence();
       }
-      const int l = opaque(lane), lds = skv_tile_off<SLAB>(chunk_row(l), chunk_col(l), 0);
+      __builtin_amdgcn_s_setprio(0);
+      const int lds = skv_tile_off<SLAB>(chunk_row(lane), chunk_col(lane), 0);
       products(NB == 2 ? r1 : r0, NB == 2 ? kr + 32 : kr, -1, [&](int j) __attribute__((always_inline)) {
         // (past the last tile: once more what is there)
         constexpr int N2 = 2 * Chunks::N;
 #pragma unroll
         for (int i = j * N2 / 4; i < (j + 1) * N2 / 4; ++i) commit_chunk(nbuf, lds, i);
-        if (j == 0) commit_scales(nbuf, l);
+        if (j == 0) commit_scales(nbuf);
       });
     };
 
