@@ -24,7 +24,7 @@ constexpr int paged_wgs_per_cu(int D) { return D == 256 ? 1 : 2; }
 
 __device__ __forceinline__ i32x4 paged_mfma_i8(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
-template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, paged_wgs_per_cu(D)) void paged_rows_kernel(PagedAttnKernelArgs a) {
+template <typename S, int D, bool SHARED, bool ONE> __global__ __launch_bounds__(256, paged_wgs_per_cu(D)) void paged_rows_kernel(PagedAttnKernelArgs a) {
   constexpr int KM = D / 64;    // 64-wide k-steps of the score product
   constexpr int DB = D / 16;    // 16-row blocks of O^T
   constexpr int VB = D / 16;    // bytes of a V row per lane
@@ -36,7 +36,7 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
   constexpr int TOTAL = MERGE > OFF_TC + 4 * TC ? MERGE : OFF_TC + 4 * TC;
   __shared__ __attribute__((aligned(16))) unsigned char smem[TOTAL];
 
-  typedef PagedDeal<SHARED, true> Deal;
+  typedef PagedDeal<SHARED, ONE> Deal;
   Deal deal(a.work, PAGED_ROWS, SKV_TILE);
   unsigned x;
   typename Deal::Item item;
@@ -128,12 +128,15 @@ template <typename S, int D, bool SHARED> __global__ __launch_bounds__(256, page
       else Load8<_Float16>::run(static_cast<const _Float16 *>(a.q) + off, qv[p]);
     }
     // last key of this lane's row; a row that is not there, or brings no token, goes along with the others and is not looked at
+    // (Without a branch that some lanes take, see qfa_paged_work.h.)
     const int block_end = deal.end(item.s, item.rb) - 1, lo = deal.begin();
-    int lim = block_end;
-    if (q16 < nrows) {
-      const auto r = deal.row(item.p, item.h, PAGED_ROWS * item.rb + q16);
+    int lim;
+    {
+      const auto r = deal.row(item.p, item.h, PAGED_ROWS * item.rb + min(q16, nrows - 1));
       const PagedSeq s = SHARED ? deal.load(r.b) : item.s;
-      if (r.i < s.tokens) lim = deal.last_key(r, s);
+      const int key = deal.last_key(r, s);
+      const bool seen = (q16 < nrows) & (r.i < s.tokens);
+      lim = seen ? key : block_end;
     }
 
     Tile ta, tb;
@@ -450,25 +453,37 @@ template <int D> __global__ __launch_bounds__(256) void paged_merge_kernel(Paged
   }
 }
 
-// Rows of a block in a launch over problems of that many rows: one block of 16, the tiles' 64 or 128 beyond
-static int block_rows(int64_t rows) { return rows <= PAGED_ROWS ? PAGED_ROWS : rows <= 64 ? 64 : 128; }
+// Rows of a block, in a launch over `problems` (sequences times key heads) of that many rows: 16, or the tiles' 64 or 128 beyond.
+// Two blocks of 16 read the keys twice but need no other launch and leave no wave without rows; 20 rows of 256 elements, 3000 keys
+// of 8 sequences: 39 us against 47 on tiles; 32 rows, 8192 keys of one sequence, 128 elements: 23 against 29, of 64 sequences with
+// 64 elements 167 against 193, but with 128 elements, where the keys no longer stay in the last cache, 313 against 250.
+// (48 rows on three blocks: 68 us against 59.)
+static int block_rows(int64_t rows, int D, int64_t problems) {
+  if (rows <= PAGED_ROWS || (rows <= 2 * PAGED_ROWS && (D != 128 || problems <= 128))) return PAGED_ROWS;
+  return rows <= 64 ? 64 : 128;
+}
 static int work_grid(int br, int D) { return br == PAGED_ROWS ? 256 * paged_wgs_per_cu(D) : paged_tile_grid(D); }
 // bytes of a launch's slots, and of its whole items
 static int64_t slots_bytes(int br, int D) { return 2LL * work_grid(br, D) * br * (D + 2) * 4; }
 static int64_t whole_bytes(int64_t rows, int D) { return (rows * (D + 2) * 4 + 15) / 16 * 16; }
-static int64_t first_bytes(int64_t B, int64_t Hk, int64_t rows) { return (8 * B * Hk * ((rows + block_rows(rows) - 1) / block_rows(rows)) + 15) / 16 * 16; }
+static int64_t first_bytes(int64_t problems, int64_t rows, int br) { return (8 * problems * ((rows + br - 1) / br) + 15) / 16 * 16; }
 static int64_t quantized_bytes(int64_t rows, int D) { return (rows * D + 4 * rows + rows + 15) / 16 * 16; }
 int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix) {
-  const int64_t rows = N * (H / Hk), own = slots_bytes(block_rows(rows), D) + first_bytes(B, Hk, rows);
-  // (16 rows or fewer are quantized by those who use them)
-  const int64_t q = rows > PAGED_ROWS || (prefix > 0 && B * rows > PAGED_ROWS) ? quantized_bytes(B * H * N, D) : 0;
-  return prefix > 0 ? own + q + slots_bytes(block_rows(B * rows), D) + 2 * whole_bytes(B * H * N, D) : own + q;
+  const int64_t rows = N * (H / Hk);
+  const int own = block_rows(rows, D, B * Hk), shared = prefix > 0 ? block_rows(B * rows, D, Hk) : 0;
+  int64_t bytes = slots_bytes(own, D) + first_bytes(B * Hk, rows, own);
+  if (prefix > 0) bytes += slots_bytes(shared, D) + 2 * whole_bytes(B * H * N, D);
+  if (own > PAGED_ROWS || shared > PAGED_ROWS) bytes += quantized_bytes(B * H * N, D);   // (blocks of 16 quantize their own)
+  return bytes;
 }
 
-template <typename S, int D> static int launch_rows(const PagedAttnKernelArgs &a, bool shared, hipStream_t st) {
-  if (shared) paged_rows_kernel<S, D, true><<<dim3((unsigned)a.work.grid), dim3(256), 0, st>>>(a);
-  else paged_rows_kernel<S, D, false><<<dim3((unsigned)a.work.grid), dim3(256), 0, st>>>(a);
-  return check_launch(shared ? "qfa_attn_paged (prefix)" : "qfa_attn_paged");
+template <typename S, int D, bool SHARED> static int launch_rows(const PagedAttnKernelArgs &a, bool one, hipStream_t st) {
+  if (one) paged_rows_kernel<S, D, SHARED, true><<<dim3((unsigned)a.work.grid), dim3(256), 0, st>>>(a);
+  else paged_rows_kernel<S, D, SHARED, false><<<dim3((unsigned)a.work.grid), dim3(256), 0, st>>>(a);
+  return check_launch(SHARED ? "qfa_attn_paged (prefix)" : "qfa_attn_paged");
+}
+template <typename S, int D> static int launch_rows(const PagedAttnKernelArgs &a, bool shared, int64_t rows, hipStream_t st) {
+  return shared ? launch_rows<S, D, true>(a, rows <= PAGED_ROWS, st) : launch_rows<S, D, false>(a, rows <= PAGED_ROWS, st);
 }
 template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
   PagedAttnKernelArgs a = {};
@@ -482,13 +497,13 @@ template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
   PagedWork w[2];
   float *mem = static_cast<float *>(x.workspace);
   for (int i = 0; i < 2; ++i) {
-    const int br = block_rows(problem[i]), grid = x.prefix > 0 || i == 0 ? work_grid(br, D) : 0;
+    const int br = block_rows(problem[i], D, (i == 0 ? x.B : 1) * x.Hk), grid = x.prefix > 0 || i == 0 ? work_grid(br, D) : 0;
     w[i] = {x.starts, x.counts, (int)x.B, (int)x.Hk, G, (int)x.N, x.causal, (int)x.prefix, (int)(x.width << x.page_log2), grid, br,
             br == PAGED_ROWS ? SKV_TILE : PAGED_TILE, br == PAGED_ROWS ? 8 : 4, nullptr, nullptr, nullptr, nullptr, nullptr};
     if (grid == 0) continue;
     if (i == 0) {
       w[i].first = reinterpret_cast<unsigned *>(mem);
-      mem += first_bytes(x.B, x.Hk, problem[0]) / 4;
+      mem += first_bytes(x.B * x.Hk, problem[0], br) / 4;
     }
     w[i].slots = mem;
     w[i].slots_ml = mem + 2LL * grid * br * D;
@@ -514,9 +529,9 @@ template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
     a.work = w[i];
     int e;
     if (w[i].br > PAGED_ROWS) e = launch_paged_tile(a, i == 1, D, x.scale_dtype, w[i].br / 32, st);
-    else if (x.scale_dtype == QFA_F32) e = launch_rows<float, D>(a, i == 1, st);
-    else if (x.scale_dtype == QFA_F16) e = launch_rows<_Float16, D>(a, i == 1, st);
-    else e = launch_rows<__bf16, D>(a, i == 1, st);
+    else if (x.scale_dtype == QFA_F32) e = launch_rows<float, D>(a, i == 1, problem[i], st);
+    else if (x.scale_dtype == QFA_F16) e = launch_rows<_Float16, D>(a, i == 1, problem[i], st);
+    else e = launch_rows<__bf16, D>(a, i == 1, problem[i], st);
     if (e) return e;
   }
   // rows per workgroup: few, whose pieces many lanes share, while that leaves no more than 4096 workgroups

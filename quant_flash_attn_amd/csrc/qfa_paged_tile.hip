@@ -35,6 +35,9 @@ template <int D> struct PagedChunks {
   unsigned z[N];
 };
 
+typedef const __attribute__((address_space(1))) unsigned char *GlobalBytes;
+typedef const __attribute__((address_space(1))) u32x4 *GlobalWords;
+
 template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(PagedAttnKernelArgs a_, int scale_dtype) {
   typedef PagedTileGeom<D, QW> GM;
   typedef PagedChunks<D> Chunks;
@@ -83,7 +86,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
     };
     auto take_pages = [&](int t) __attribute__((always_inline)) {
       const int l = opaque(lane), quarter = 4 * (t0 + t) + l;
-      const bool ok = 4 * t + l < 4 * nt && quarter >> page_quarters_log2 < a.width && pg >= 0 && pg < a.pages;
+      const bool ok = (4 * t + l < 4 * nt) & (quarter >> page_quarters_log2 < a.width) & (pg >= 0) & (pg < a.pages);
       pages_ok = __builtin_amdgcn_ballot_w64(ok);
       first_row = (((unsigned)(ok ? pg : 0) * (unsigned)a.work.Hk + (unsigned)item.h) << a.page_log2) + (((unsigned)quarter & quarter_mask) << 4);
     };
@@ -106,12 +109,13 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
         static_assert(Chunks::STEP % 16 == 0, "a thread's chunks differ in the quarter");
         const int quarter = (wave * Chunks::RPW + Chunks::STEP * i) / 16;
         const unsigned at = (unsigned)__builtin_amdgcn_readlane((int)first_row, 4 * (t % 16) + quarter);
-        const int8_t *k = a.kc + (uint64_t)at * D, *v = a.vc + (uint64_t)at * D, *zk = a.kz + at, *zv = a.vz + at;
+        GlobalBytes k = (GlobalBytes)(a.kc + (uint64_t)at * D), v = (GlobalBytes)(a.vc + (uint64_t)at * D), zk = (GlobalBytes)(a.kz + at),
+                    zv = (GlobalBytes)(a.vz + at);
         asm("" : "+s"(k), "+s"(v), "+s"(zk), "+s"(zv));   // (scalar bases: else the lanes' 64-bit addresses are kept)
-        ck.w[i] = *reinterpret_cast<const u32x4 *>(k + off);
-        cv.w[i] = *reinterpret_cast<const u32x4 *>(v + off);
-        ck.z[i] = (unsigned char)zk[in];
-        cv.z[i] = (unsigned char)zv[in];
+        ck.w[i] = *(GlobalWords)(k + off);
+        cv.w[i] = *(GlobalWords)(v + off);
+        ck.z[i] = zk[in];
+        cv.z[i] = zv[in];
       }
       const void *p = wave % 2 == 0 ? a.ks : a.vs;
       sc = scale_dtype == QFA_F32 ? static_cast<const unsigned *>(p)[scale_row] : static_cast<const unsigned short *>(p)[scale_row];
@@ -153,9 +157,9 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
     // ---- this lane's row: half of its codes, as binary16 integers code - zero point (k-step m, k-group g holds columns
     // 16m + 8g + {0..7}), and a = scale * sm_scale * log2(e).  Rows past the last are zeros.
     const int row_q = 32 * slot + opaque(lr), block_end = deal.end(item.s, item.rb) - 1, lo = deal.begin();
-    int lim = block_end;   // last key of the row; one that is not there, or brings no token, goes along with the others and is not looked at
+    int lim;   // last key of the row; one that is not there, or brings no token, goes along with the others and is not looked at
     u32x2 qc[KD];
-    float a_i = 0x1p-126f, zq = 0.f;
+    float a_i, zq;
     const bool have = row_q < nrows;
     {
       const auto r = deal.row(item.p, item.h, BR * item.rb + min(row_q, nrows - 1));
@@ -166,8 +170,10 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
       for (int m = 0; m < KD; ++m) qc[m] = *reinterpret_cast<const u32x2 *>(codes + 16 * m);
       const float f = a.q_scale[at] * a.sm_scale_log2;
       zq = (float)a.q_zero[at];
-      if (have) a_i = f < 0x1p-126f ? 0x1p-126f : f;   // (not zero: the mask's -inf is multiplied by it)
-      if (have && r.i < s.tokens) lim = deal.last_key(r, s);
+      const int key = deal.last_key(r, s);   // (no branches: see qfa_paged_work.h)
+      const bool seen = have & (r.i < s.tokens), small = !have | (f < 0x1p-126f);
+      a_i = small ? 0x1p-126f : f;   // (not zero: the mask's -inf is multiplied by it)
+      lim = seen ? key : block_end;
     }
     issue(0);
     u32x4 qf[KD];

@@ -12,6 +12,10 @@
 // that no cache holds yet: the lengths of 64 sequences are loaded once, a sequence in each lane, and read out of the lanes from
 // there on; where an item begins is left in memory for the kernel that joins the pieces.
 //
+// Nothing here branches on what differs between lanes (& in place of &&, values before their selection): where the branches of some
+// lanes join again the compiler has saved registers of all lanes before it turned the others back on, a thread's own index among
+// them, in kernels that have none to spare.
+//
 // Rows of a sequence are its queries times the query heads that share a key head: row = query * G + head % G.
 #pragma once
 #include "qfa_device.h"
@@ -71,18 +75,17 @@ template <bool SHARED, bool ONE> struct PagedDeal {
   // the keys of a block of rows end here
   __device__ __forceinline__ int end(const PagedSeq &s, int rb) const {
     if (SHARED) return min(a.prefix, a.capacity);
-    if (s.tokens == 0) return 0;
     int last = s.tokens - 1;
-    if (!ONE) {
-      if (rb * BR / a.G > last) return 0;
-      if (a.causal) last = min(((rb + 1) * BR - 1) / a.G, last);
-    }
-    return (int)max((int64_t)0, min((int64_t)s.start + last + 1, (int64_t)a.capacity));
+    const bool none = last < (ONE ? 0 : rb * BR / a.G);
+    if (!ONE && a.causal) last = min(((rb + 1) * BR - 1) / a.G, last);
+    const int e = (int)max((int64_t)0, min((int64_t)s.start + last + 1, (int64_t)a.capacity));
+    return none ? 0 : e;
   }
   __device__ __forceinline__ int begin() const { return SHARED ? 0 : a.prefix; }
   __device__ __forceinline__ unsigned tiles(const PagedSeq &s, int rb) const {
     const int e = end(s, rb), b = begin();
-    return e > b ? (unsigned)((e + TK - 1) / TK - b / TK) : 0u;
+    const unsigned n = (unsigned)((int)(((unsigned)e + TK - 1) / TK) - b / TK);
+    return e > b ? n : 0u;
   }
   __device__ __forceinline__ unsigned units(const PagedSeq &s, int rb) const {
     const unsigned n = tiles(s, rb);
@@ -121,10 +124,15 @@ template <bool SHARED, bool ONE> struct PagedDeal {
     } else {
       const int lane = threadIdx.x % 64;
       lanes = load(lane);
-      unsigned mine = lane < problems ? units_of_head(lanes) * (unsigned)a.Hk : 0u, sum = wave_scan(mine);
+      // (of a sequence that there is)
+      const auto units_of = [&](const PagedSeq &s, int p) __attribute__((always_inline)) -> unsigned {
+        const unsigned u = units_of_head(s) * (unsigned)a.Hk;
+        return p < problems ? u : 0u;
+      };
+      unsigned mine = units_of(lanes, lane), sum = wave_scan(mine);
       total = (unsigned)__builtin_amdgcn_readlane((int)sum, 63);
       for (int base = 64; base < problems; base += 64) {
-        const unsigned u = base + lane < problems ? units_of_head(load(base + lane)) * (unsigned)a.Hk : 0u;
+        const unsigned u = units_of(load(base + lane), base + lane);
         total += (unsigned)__builtin_amdgcn_readlane((int)wave_scan(u), 63);
       }
       divide();
@@ -142,7 +150,7 @@ template <bool SHARED, bool ONE> struct PagedDeal {
         before += (unsigned)__builtin_amdgcn_readlane((int)sum, 63);   // (x < total: a later sequence has it)
         held += 64;
         lanes = load(held + lane);
-        mine = held + lane < problems ? units_of_head(lanes) * (unsigned)a.Hk : 0u;
+        mine = units_of(lanes, held + lane);
         sum = wave_scan(mine);
       }
       it.s = seq(it.p);

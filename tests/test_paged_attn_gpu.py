@@ -82,6 +82,15 @@ def test_dealing(qfa, B, H, Hk, N, D, keys):
     _check(qfa, B, H, Hk, N, D, 16, [max(k, N) for k in keys], seed=B)
 
 
+# every size of a block of rows, for every row size: 16 (one and two blocks), 64, 128 and more
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("B,H,Hk,N", [(2, 8, 1, 2), (3, 8, 2, 5), (65, 4, 2, 9), (2, 4, 1, 10), (2, 3, 1, 41), (1, 2, 1, 161)])
+def test_blocks_of_rows(qfa, D, B, H, Hk, N):
+    _check(qfa, B, H, Hk, N, D, 32, [N + (211 * i) % 600 for i in range(B)], seed=D + N)
+    _check(qfa, B, H, Hk, N, D, 16, [161 + N + (97 * i) % 300 for i in range(B)], prefix=161, seed=D + N)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("scale_dtype", [torch.float16, torch.bfloat16, torch.float32])
