@@ -24,11 +24,12 @@ constexpr int paged_wgs_per_cu(int D) { return D == 256 ? 1 : 2; }
 
 __device__ __forceinline__ i32x4 paged_mfma_i8(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
-template <typename S, int D, bool SHARED, bool ONE> __global__ __launch_bounds__(256, paged_wgs_per_cu(D)) void paged_rows_kernel(PagedAttnKernelArgs a) {
+template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __launch_bounds__(256, paged_wgs_per_cu(D)) void paged_rows_kernel(PagedAttnKernelArgs a) {
   constexpr int KM = D / 64;    // 64-wide k-steps of the score product
   constexpr int DB = D / 16;    // 16-row blocks of O^T
   constexpr int VB = D / 16;    // bytes of a V row per lane
   constexpr int VD = VB / 4;    // ... in dwords
+  constexpr int HINT = STREAM ? LOAD_ONCE : 0;
   constexpr int LPT = D / 8, TPP = 256 / LPT;   // quantizer: lanes per token, tokens per pass
   // LDS: query codes and constants, per-wave token constants; the merge of the four waves overlays them
   constexpr int OFF_ST = 16 * D, OFF_TC = OFF_ST + 3 * 16 * 4, MERGE = 4 * 16 * (D + 2) * 4;
@@ -92,20 +93,20 @@ template <typename S, int D, bool SHARED, bool ONE> __global__ __launch_bounds__
         const rsrc_t rk = make_rsrc(a.kc + first[rb] * D, ok ? 16 * D : 0), rv = make_rsrc(a.vc + first[rb] * D, ok ? 16 * D : 0);
 #pragma unroll
         for (int m = 0; m < KM; ++m)
-          t.k[rb][m] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off, 64 * m, 0));
+          t.k[rb][m] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off, 64 * m, HINT));
 #pragma unroll
         for (int e = 4 * rb; e < 4 * rb + 4; ++e) {
           const int soff = (e % 4) * D;
           if constexpr (VD == 4) {
-            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off, soff, 0));
+            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off, soff, HINT));
 #pragma unroll
             for (int y = 0; y < 4; ++y) t.v[e][y] = w[y];
           } else if constexpr (VD == 2) {
-            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_off, soff, 0));
+            const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_off, soff, HINT));
             t.v[e][0] = w[0];
             t.v[e][1] = w[1];
           } else {
-            t.v[e][0] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rv, v_off, soff, 0);
+            t.v[e][0] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rv, v_off, soff, HINT);
           }
         }
       }
@@ -477,13 +478,15 @@ int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, 
   return bytes;
 }
 
-template <typename S, int D, bool SHARED> static int launch_rows(const PagedAttnKernelArgs &a, bool one, hipStream_t st) {
-  if (one) paged_rows_kernel<S, D, SHARED, true><<<dim3((unsigned)a.work.grid), dim3(256), 0, st>>>(a);
-  else paged_rows_kernel<S, D, SHARED, false><<<dim3((unsigned)a.work.grid), dim3(256), 0, st>>>(a);
+template <typename S, int D, bool SHARED> static int launch_rows(const PagedAttnKernelArgs &a, bool one, bool stream, hipStream_t st) {
+  const dim3 grid((unsigned)a.work.grid), block(256);
+  if (!one) paged_rows_kernel<S, D, SHARED, false, false><<<grid, block, 0, st>>>(a);
+  else if (!SHARED && stream) paged_rows_kernel<S, D, false, true, true><<<grid, block, 0, st>>>(a);
+  else paged_rows_kernel<S, D, SHARED, true, false><<<grid, block, 0, st>>>(a);
   return check_launch(SHARED ? "qfa_attn_paged (prefix)" : "qfa_attn_paged");
 }
-template <typename S, int D> static int launch_rows(const PagedAttnKernelArgs &a, bool shared, int64_t rows, hipStream_t st) {
-  return shared ? launch_rows<S, D, true>(a, rows <= PAGED_ROWS, st) : launch_rows<S, D, false>(a, rows <= PAGED_ROWS, st);
+template <typename S, int D> static int launch_rows(const PagedAttnKernelArgs &a, bool shared, bool one, bool stream, hipStream_t st) {
+  return shared ? launch_rows<S, D, true>(a, one, stream, st) : launch_rows<S, D, false>(a, one, stream, st);
 }
 template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
   PagedAttnKernelArgs a = {};
@@ -524,19 +527,23 @@ template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
       return e;
     a.q_codes = codes; a.q_scale = scale; a.q_zero = zero;
   }
+  // Non-temporal loads (LOAD_ONCE) where the keys and values that a call may reach outgrow the last-level cache (550 MB, 64 sequences:
+  // 104.9 us with plain loads, 98.5 with these; 67 MB: 17.7 and 18.0, 34 MB behind a prefix 16.2 and 17.8)
+  const bool stream = (double)(x.pages < x.B * x.width ? x.pages : x.B * x.width) * (double)(x.Hk << x.page_log2) * 2 * D >= 320.0 * (1 << 20);
   for (int i = 1; i >= 0; --i) {
     if (w[i].grid == 0) continue;
     a.work = w[i];
     int e;
     if (w[i].br > PAGED_ROWS) e = launch_paged_tile(a, i == 1, D, x.scale_dtype, w[i].br / 32, st);
-    else if (x.scale_dtype == QFA_F32) e = launch_rows<float, D>(a, i == 1, problem[i], st);
-    else if (x.scale_dtype == QFA_F16) e = launch_rows<_Float16, D>(a, i == 1, problem[i], st);
-    else e = launch_rows<__bf16, D>(a, i == 1, problem[i], st);
+    else if (x.scale_dtype == QFA_F32) e = launch_rows<float, D>(a, i == 1, problem[i] <= PAGED_ROWS, stream, st);
+    else if (x.scale_dtype == QFA_F16) e = launch_rows<_Float16, D>(a, i == 1, problem[i] <= PAGED_ROWS, stream, st);
+    else e = launch_rows<__bf16, D>(a, i == 1, problem[i] <= PAGED_ROWS, stream, st);
     if (e) return e;
   }
-  // rows per workgroup: few, whose pieces many lanes share, while that leaves no more than 4096 workgroups
+  // rows per workgroup: few, whose pieces many lanes share, while that leaves no more than 1024 workgroups (2048 rows one by one: 9.4 us
+  // against 6.4 two by two, with a prefix 12.9 against 10.5; in 512 workgroups 5.7 and 11.4)
   int chunk_rows = 1;
-  while (chunk_rows < 16 && x.B * x.Hk * ((problem[0] + chunk_rows - 1) / chunk_rows) > 4096) chunk_rows *= 2;
+  while (chunk_rows < 16 && x.B * x.Hk * ((problem[0] + chunk_rows - 1) / chunk_rows) > 1024) chunk_rows *= 2;
   const int chunks = (int)((problem[0] + chunk_rows - 1) / chunk_rows);
   const PagedMergeArgs m = {w[0], w[1], x.o, x.q_dtype, chunks, chunk_rows};
   paged_merge_kernel<D><<<dim3((unsigned)(x.B * x.Hk * chunks)), dim3(256), 0, st>>>(m);
