@@ -60,7 +60,7 @@ template <typename T, int D, bool INTERLEAVED> __global__ __launch_bounds__(256)
   const int64_t b = index_div(t, x.N), n = t - b * x.N, pos = (int64_t)x.starts[b] + n;
   const Place place(x, b, n, pos);
   const bool turn = !values && x.half != 0, norm = !values && x.w != nullptr;
-  const bool live = t_raw < tokens && place.page >= 0 && (!turn || pos < x.rope_rows);
+  const bool live = t_raw < tokens && place.page >= 0 && (x.half == 0 || pos < x.rope_rows);   // (the same tokens of both)
   RopeLane<D, INTERLEAVED> lane(sub, turn ? x.half : 0);
   if (turn) lane.angles(x.cos, x.sin, live ? pos : 0, x.rope_rows, x.half);
   const void *src = values ? x.v : x.k;

@@ -48,9 +48,10 @@ def paged_cache_append(cache, k: torch.Tensor, v: torch.Tensor, page_table: torc
     position starts[b] + n of its sequence.
 
     The keys are normed (k_weight, eps) and rotated by their position (cos, sin, interleaved) on the way, as norm_rope does it, without
-    a rounding in between.  A token has no place, and is not written, where its position is negative, past the page table or past the
-    table of angles, or its page is none of the cache's (so a -1 in the page table skips).  A page that is written may stand only once in the call's page table (pages that sequences share may be
-    read by all of them).  No gradient flows through a cache.
+    a rounding in between.  A token has no place, and neither its keys nor its values are written, where its position is negative, past
+    the page table or past the table of angles, or its page is none of the cache's (so a -1 in the page table skips).  A page that is
+    written may stand only once in the call's page table (pages that sequences share may be read by all of them).  No gradient flows
+    through a cache.
     """
     _lib.host().paged_append(tuple(cache), k, v, page_table, starts, counts, k_weight, cos, sin, float(eps), bool(interleaved))
 

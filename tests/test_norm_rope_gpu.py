@@ -205,6 +205,14 @@ def test_traced(qfa):
             qfa.norm_rope(dual, v0, c, s)
 
 
+@pytest.mark.gpu
+def test_no_second_derivative(qfa):
+    x, w = torch.randn(1, 2, 8, 64, device=DEV, requires_grad=True), torch.ones(64, device=DEV, requires_grad=True)
+    y = qfa.norm_rope(x, w, None, None)
+    with pytest.raises(NotImplementedError, match="second derivative"):
+        torch.autograd.grad(y, (x, w), torch.ones_like(y), create_graph=True)
+
+
 def test_refusals(qfa):
     x, w, (cos, sin) = torch.randn(1, 2, 8, 64), torch.ones(64), m.table(16, 64)
     with pytest.raises(RuntimeError, match="GPU only"):

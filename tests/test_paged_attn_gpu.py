@@ -257,6 +257,40 @@ def test_repeats_and_graphs(qfa, prefix):
 
 
 @pytest.mark.gpu
+def test_two_calls_at_once(qfa):
+    """Calls on two streams that overlap, and two captured ones whose replays do, give what each gives alone."""
+    made = []
+    for B, H, Hk, N, D, keys, prefix in ((40, 8, 2, 1, 128, 700, 300), (2, 4, 4, 150, 64, 1200, 0)):
+        q, cache, table, starts, *_ = _problem(B, H, Hk, N, D, 32, [keys - i for i in range(B)], prefix=prefix, seed=B)
+        args = (q.to(DEV), [t.to(DEV) for t in cache], table.to(DEV), starts.to(DEV))
+        made.append(lambda args=args, prefix=prefix: qfa.quant_flash_attn_paged(*args, prefix_len=prefix))
+    want = [f().clone() for f in made]
+    streams = [torch.cuda.Stream() for _ in made]
+    graphs = [torch.cuda.CUDAGraph() for _ in made]
+    torch.cuda.synchronize()
+    for i in range(3):
+        got = []
+        for f, st in zip(made, streams):
+            with torch.cuda.stream(st):
+                got.append([f() for _ in range(5)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for os, w in zip(got, want) for o in os), i
+    outs = []
+    for f, g in zip(made, graphs):
+        with torch.cuda.graph(g):
+            outs.append(f())
+    for i in range(3):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)), f"replay {i}"
+
+
+@pytest.mark.gpu
 def test_pages_past_32_bits(qfa):
     H, page, D = 8, 64, 128
     pages = (1 << 32) // (H * page * D) + 64
