@@ -493,11 +493,14 @@ int qfa_paged_read(const qfa_paged_cache *cache, const int32_t *page_table, int6
  * [0, pages) are hidden.  What hidden rows of the cache hold is irrelevant.
  *   q [B,H,N,D] of q_dtype with strides as in qfa_attn_fwd; H a multiple of the cache's heads: query head h reads key head
  *     h / (H / cache->H).  o [B,H,N,D] of q_dtype, dense.
- *   prefix  the first `prefix` keys are the same for all sequences: they are read once, from sequence 0's pages.
+ *   prefix  the first `prefix` keys are the same for all sequences: they are read once, from sequence 0's pages.  That pays where they
+ *     are many for the sequences and rows: qfa_attn_paged_shared_prefix says whether (prefix, or 0: every sequence's own pages then,
+ *     which have to hold them too).
  *   workspace  qfa_attn_paged_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant; one for each call under way.
  * The lengths are read on the device: a captured call follows them.  Keys are dealt to workgroups evenly over the whole batch, so
  * the last bits of a sequence's O depend on the lengths of the others; a call repeated gives the same bits.
  */
+int64_t qfa_attn_paged_shared_prefix(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
 int64_t qfa_attn_paged_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
 
 int qfa_attn_paged(const qfa_paged_cache *cache, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn, const int32_t *page_table,

@@ -79,6 +79,7 @@ _SIGNATURES = {
     "qfa_norm_rope_bwd": (c_int, [_P] * 4 + [_L, _I, _I, _P, _L, _L, _I, _F, _I, _I, _L, _L, _I, _P, _L, _P]),
     "qfa_paged_append": (c_int, [_P, _P, _P, _I] + [_L] * 6 + [_P, _L, _L, _L, _P, _P, _P, _I, _I, _F, _P, _P, _L, _I, _I, _L, _L, _P]),
     "qfa_paged_read": (c_int, [_P, _P, _L, _L, _L, _P, _P, _P, _P, _I, _L, _L, _P]),
+    "qfa_attn_paged_shared_prefix": (c_int64, [_L, _L, _L, _L, _I, _L]),
     "qfa_attn_paged_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _L]),
     "qfa_attn_paged": (c_int, [_P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _L, _L, _L, _L, _F, _I, _P, _L, _P]),
     "qfa_attn_bwd": (c_int, [_P] * 13 + [_L] + [_P] * 3 + [_I, _L, _L, _L, _L, _I] + [_L] * 24 + [_F, _I, _P]),

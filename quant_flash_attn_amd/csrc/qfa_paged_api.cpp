@@ -168,6 +168,11 @@ int64_t qfa_attn_paged_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t
   return paged_attn_workspace_bytes(B, H, Hk, N, D, prefix);
 }
 
+int64_t qfa_attn_paged_shared_prefix(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix) {
+  if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || N <= 0 || !head_dim_ok(D) || prefix <= 0) return 0;
+  return paged_attn_shared_prefix(B, H, Hk, N, D, prefix);
+}
+
 int qfa_attn_paged(const qfa_paged_cache *cache, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn, const int32_t *page_table,
                    int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, void *o, int64_t B, int64_t H, int64_t N,
                    int64_t prefix, float sm_scale, int causal, void *workspace, int64_t workspace_bytes, void *stream) {

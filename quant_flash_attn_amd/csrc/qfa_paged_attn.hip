@@ -478,6 +478,24 @@ int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, 
   return bytes;
 }
 
+// How long a pass over `keys` keys takes for problems * rows rows beside its start, in us: every block of rows reads them again, at the
+// rate (TB/s, of a chip that is full) that its kernel has in its caches
+static double pass_us(int64_t problems, int64_t rows, int64_t keys, int D) {
+  const int br = block_rows(rows, D, problems);
+  const double rate = br == PAGED_ROWS ? 11.0 : br == 64 ? (D == 128 ? 5.5 : 3.75) : (D == 128 ? 3.4 : 2.5);
+  return (double)problems * (double)((rows + br - 1) / br) * (double)keys * 2 * D / (rate * 1e6);
+}
+// Whether a prefix gets a pass of its own.  That one has its start, its queries quantized and results of all rows written and joined
+// again against it: where it saves less, every sequence reads the prefix from its own pages.  Of 240 calls timed both ways (4 to 64
+// sequences, 1 to 300 rows, prefixes of 400, 2000 and 8000 keys, D 64, 128 and 256) 34 get one, which take 0.29 to 0.98 of the time
+// without; of the others 200 take 0.41 to 1.0 of the time with it, six 1.02 to 1.25.
+int64_t paged_attn_shared_prefix(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix) {
+  const int64_t rows = N * (H / Hk);
+  const double start = block_rows(B * rows, D, Hk) == PAGED_ROWS ? 6.0 + D / 64 : 13.0 + 3.5 * (D / 64);
+  const double joined = (double)(B * H * N) * (D + 2) * 16 / 4.5e6;   // written twice, read twice
+  return B > 1 && pass_us(B * Hk, rows, prefix, D) > pass_us(Hk, B * rows, prefix, D) + start + joined ? prefix : 0;
+}
+
 template <typename S, int D, bool SHARED> static int launch_rows(const PagedAttnKernelArgs &a, bool one, bool stream, hipStream_t st) {
   const dim3 grid((unsigned)a.work.grid), block(256);
   if (!one) paged_rows_kernel<S, D, SHARED, false, false><<<grid, block, 0, st>>>(a);

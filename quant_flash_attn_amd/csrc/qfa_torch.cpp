@@ -61,6 +61,7 @@ struct Api {
   QFA_ENTRY(qfa_norm_rope_bwd);
   QFA_ENTRY(qfa_paged_append);
   QFA_ENTRY(qfa_paged_read);
+  QFA_ENTRY(qfa_attn_paged_shared_prefix);
   QFA_ENTRY(qfa_attn_paged_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged);
 #undef QFA_ENTRY
@@ -104,6 +105,7 @@ void init(const py::dict &address) {
   QFA_ENTRY(qfa_norm_rope_bwd);
   QFA_ENTRY(qfa_paged_append);
   QFA_ENTRY(qfa_paged_read);
+  QFA_ENTRY(qfa_attn_paged_shared_prefix);
   QFA_ENTRY(qfa_attn_paged_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged);
 #undef QFA_ENTRY

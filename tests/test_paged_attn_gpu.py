@@ -45,14 +45,33 @@ def _check(qfa, *args, causal=True, **kw):
     q, cache, table, starts, counts, ks, vs, v_scale = _problem(*args, **kw)
     D, sm = q.shape[-1], m.sm_of(q.shape[-1])
     dev = lambda t: None if t is None else t.to(DEV)   # noqa: E731
-    o = qfa.quant_flash_attn_paged(dev(q), [dev(t) for t in cache], dev(table), dev(starts), dev(counts), causal=causal, sm_scale=sm, prefix_len=prefix)
-    assert o.dtype == q.dtype and o.shape == q.shape
+    call = (dev(q), [dev(t) for t in cache], dev(table), dev(starts), dev(counts))
+    out = [qfa.quant_flash_attn_paged(*call, causal=causal, sm_scale=sm, prefix_len=prefix)]
+    if prefix:
+        out.append(_with_prefix_pass(*call, causal, sm, prefix))
+    assert out[0].dtype == q.dtype and out[0].shape == q.shape
     qh = m.values(*m.quantized(q.float()))
     want, size = m.attention(qh, ks, vs, starts, counts, causal, sm)
     keys = max([t.shape[1] for t in ks] + [1])
-    excess = (o.cpu().double() - want).abs() - m.attention_bound(want, size, q.dtype, keys, v_scale)
-    assert torch.isfinite(o).all()
-    assert excess.max() <= 0, f"over the bound by {excess.max().item():.3e} at {want.flatten()[excess.argmax()].item():.3e}"
+    bound = m.attention_bound(want, size, q.dtype, keys, v_scale)
+    for o in out:
+        excess = (o.cpu().double() - want).abs() - bound
+        assert torch.isfinite(o).all()
+        assert excess.max() <= 0, f"over the bound by {excess.max().item():.3e} at {want.flatten()[excess.argmax()].item():.3e}"
+    return out[0]
+
+
+def _with_prefix_pass(q, cache, table, starts, counts, causal, sm, prefix):
+    """The C entry, which gives a prefix a pass of its own whether it pays or not."""
+    from quant_flash_attn_amd import _lib
+    L, (B, H, N, D), (pages, Hk, page, _) = _lib.lib(), q.shape, cache[0].shape
+    c = _lib.PagedCacheStruct(*[t.data_ptr() for t in cache], pages, Hk, page, D, _lib.DTYPE_CODE[cache[1].dtype])
+    need = L.qfa_attn_paged_workspace_bytes(B, H, Hk, N, D, prefix)
+    ws, o = torch.empty(need, dtype=torch.uint8, device=q.device), torch.full((B, H, N, D), float("nan"), dtype=q.dtype, device=q.device)
+    rc = L.qfa_attn_paged(ctypes.byref(c), q.data_ptr(), _lib.DTYPE_CODE[q.dtype], *q.stride()[:3], table.data_ptr(), table.shape[1], *table.stride(),
+                          starts.data_ptr(), None if counts is None else counts.data_ptr(), o.data_ptr(), B, H, N, prefix, sm, int(causal), ws.data_ptr(), need,
+                          _lib.stream_of(q))
+    assert rc == 0, L.qfa_last_error()
     return o
 
 
@@ -159,7 +178,7 @@ def test_prefix_with_padding_and_short_sequences(qfa):
     starts = torch.tensor([96, 128, 120, 50, 299], dtype=torch.int32)
     for causal in (True, False):
         dev = lambda t: t.to(DEV)   # noqa: E731
-        o = qfa.quant_flash_attn_paged(dev(q), [dev(t) for t in cache], dev(table), dev(starts), dev(counts), causal=causal, prefix_len=prefix).cpu()
+        o = _with_prefix_pass(dev(q), [dev(t) for t in cache], dev(table), dev(starts), dev(counts), causal, m.sm_of(128), prefix).cpu()
         want, size = m.attention(m.values(*m.quantized(q.float())), ks, vs, starts, counts, causal, m.sm_of(128))
         # (not causal, a sequence that ends inside the prefix sees starts + counts keys all the same)
         assert ((o.double() - want).abs() <= m.attention_bound(want, size, q.dtype, 300, v_scale)).all(), causal
@@ -225,7 +244,8 @@ def test_repeats_and_graphs(qfa, prefix):
     B, H, Hk, N, D, page = 5, 8, 2, 2, 128, 16
     q, cache, table, starts, _, ks, vs, _ = _problem(B, H, Hk, N, D, page, [500, 80, 300, 66, 120], prefix=prefix, seed=6)
     q, table, starts, cache = q.to(DEV), table.to(DEV), starts.to(DEV), [t.to(DEV) for t in cache]
-    call = lambda: qfa.quant_flash_attn_paged(q, cache, table, starts, prefix_len=prefix)   # noqa: E731
+    call = lambda: (_with_prefix_pass(q, cache, table, starts, None, True, m.sm_of(D), prefix) if prefix else   # noqa: E731
+                    qfa.quant_flash_attn_paged(q, cache, table, starts))
     want = call()
     assert torch.equal(want, call())
     side = torch.cuda.Stream()
@@ -263,7 +283,7 @@ def test_two_calls_at_once(qfa):
     for B, H, Hk, N, D, keys, prefix in ((40, 8, 2, 1, 128, 700, 300), (2, 4, 4, 150, 64, 1200, 0)):
         q, cache, table, starts, *_ = _problem(B, H, Hk, N, D, 32, [keys - i for i in range(B)], prefix=prefix, seed=B)
         args = (q.to(DEV), [t.to(DEV) for t in cache], table.to(DEV), starts.to(DEV))
-        made.append(lambda args=args, prefix=prefix: qfa.quant_flash_attn_paged(*args, prefix_len=prefix))
+        made.append(lambda args=args, prefix=prefix: _with_prefix_pass(*args, None, True, 0.1, prefix))
     want = [f().clone() for f in made]
     streams = [torch.cuda.Stream() for _ in made]
     graphs = [torch.cuda.CUDAGraph() for _ in made]
@@ -342,6 +362,9 @@ def test_argument_errors_need_no_gpu(qfa):
         assert rc == code, (rc, code, what)
     assert call(q=None) == -1 and b"null" in L.qfa_last_error()
     ws = L.qfa_attn_paged_workspace_bytes
+    share = L.qfa_attn_paged_shared_prefix
+    assert share(64, 32, 8, 1, 128, 16384) == 16384 and share(64, 32, 8, 1, 128, 100) == 0 and share(1, 32, 8, 1, 128, 16384) == 0
+    assert share(64, 32, 8, 1, 96, 16384) == 0 and share(64, 32, 7, 1, 128, 16384) == 0 and share(64, 32, 8, 300, 128, 400) == 0
     assert ws(1, 4, 2, 1, 128, 0) > 0 and ws(1, 4, 2, 1, 96, 0) == 0 and ws(1, 4, 3, 1, 128, 0) == 0 and ws(8, 4, 2, 1, 128, 5) > 2 * ws(8, 4, 2, 1, 128, 0)
 
 
