@@ -381,19 +381,40 @@ struct PagedPieces {
   }
 };
 struct PagedSum { float m, l; f32x4 acc; };
+// Pieces are loaded four at a time (past the last one: once more that one, which then counts for nothing); one by one, each would wait
+// for its own loads
 template <int D> __device__ __forceinline__ void paged_add(const PagedWork &work, const PagedPieces &at, int d, int group, int groups, PagedSum &x) {
+  constexpr int AT_ONCE = 4;
   const float *po = at.whole >= 0 ? work.whole : work.slots, *pml = at.whole >= 0 ? work.whole_ml : work.slots_ml;
-#pragma unroll 4
-  for (unsigned w = at.w0 + group; w <= at.w1; w += groups) {
-    const int64_t i = at.whole >= 0 ? at.whole : ((int64_t)w * 2 + (w == at.w0 ? 1 : 0)) * work.br + at.in_block;
-    const f32x2 ml = *reinterpret_cast<const f32x2 *>(pml + 2 * i);
-    const f32x4 y = *reinterpret_cast<const f32x4 *>(po + i * D + d);
-    const float m_new = ml[1] == 0.f ? x.m : fmaxf(x.m, ml[0]);   // (a piece that saw no key: its sums are zero)
-    const float s0 = __builtin_amdgcn_exp2f(x.m - m_new), s1 = ml[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m_new);
-    x.m = m_new;
-    x.l = x.l * s0 + ml[1] * s1;
+  for (unsigned w = at.w0 + group; w <= at.w1; w += AT_ONCE * groups) {
+    f32x2 ml[AT_ONCE];
+    f32x4 y[AT_ONCE];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x.acc[e] = x.acc[e] * s0 + mul_zero_wins(s1, y[e]);
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const unsigned wj = min(w + j * groups, at.w1);
+      const int64_t i = at.whole >= 0 ? at.whole : ((int64_t)wj * 2 + (wj == at.w0 ? 1 : 0)) * work.br + at.in_block;
+      ml[j] = *reinterpret_cast<const f32x2 *>(pml + 2 * i);
+      y[j] = *reinterpret_cast<const f32x4 *>(po + i * D + d);
+    }
+    float m_new = x.m;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const float l = ml[j][1];
+      if ((w + j * groups > at.w1) | (l == 0.f)) ml[j] = f32x2{NO_KEY, 0.f};   // (a piece that saw no key: its sums are zero)
+      m_new = fmaxf(m_new, ml[j][0]);
+    }
+    const float s0 = __builtin_amdgcn_exp2f(x.m - m_new);
+    x.m = m_new;
+    x.l *= s0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x.acc[e] *= s0;
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const float l = ml[j][1], s1 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[j][0] - m_new);
+      x.l += l * s1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x.acc[e] += mul_zero_wins(s1, y[j][e]);
+    }
   }
 }
 
