@@ -2,14 +2,15 @@
 //     y = rot(x * r * w),   r = 1 / sqrt(mean(x^2) + eps)
 //     g = rot^T(dy),  dw = sum over rows of g x r,  dx = r (g w) - x r^3 mean((g w) x)
 // Bound by memory: the forward reads and writes each row once, the backward reads x and dy and writes dx; r is computed again
-// from x, which it reads anyway, so the forward keeps nothing.
+// from x, which it reads anyway, so the forward keeps nothing.  4 x 64 heads x 4096 x 128 bf16: forward 100 us (5.4 TB/s), gradient
+// 162 us (5.0 TB/s); a copy of that size 5.0.
 //
 // A row is held by D/16 lanes (RopeLane), a workgroup of 256 threads holds 4096/D tokens of one head at a time and walks over
 // `heads_each` heads of these tokens, so that the angles (4 D bytes of fp32 per token against 2 D of a 16-bit row) are read once
 // for all of them.  Queries and keys go out in one launch.  Everything in between is fp32, one rounding at the end.
 //
 // dw: a thread adds up what it sees in registers; the workgroup's threads meet in LDS and leave one row of partial sums, which
-// a second small kernel adds up in a fixed order (no atomics: the same call gives the same bits).
+// a second small kernel adds up in a fixed order (no atomics: the same call gives the same bits): 8 us for 2 x 2048 rows of 128.
 #include "qfa_rope_row.h"
 
 namespace qfa {
@@ -154,7 +155,8 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_rope_dw_kerne
   else static_cast<T *>(a.dw)[o + col] = (T)s;
 }
 
-// Heads that a workgroup walks over: as many as leave the chip 2048 workgroups, eight at most
+// Heads that a workgroup walks over: as many as leave the chip 2048 workgroups, eight at most.  (64 heads of 128, 4 x 4096 tokens: eight
+// 100 us forward and 162 backward, sixteen 115 and 178; the fewer partial sums of dw take 5.6 us in place of 8.)
 static int heads_each(int64_t tokens, int64_t H, int D) {
   const int64_t blocks = (tokens + 4096 / D - 1) / (4096 / D) * H;
   int e = 1;

@@ -3,7 +3,9 @@
 // with the arithmetic of the kernel for a cache in one piece (qfa_cache.hip): queries quantized per token here, Q K^T on INT8
 // MFMA with the exact zero-point term, V as its exact codes in binary16, softmax statistics and sums in fp32.
 //
-// Bound by reading the cache once (2 D + 6 bytes per key and key head).  A workgroup = 4 waves = 16 rows (queries times the
+// Bound by reading the cache once (2 D + 6 bytes per key and key head): 64 sequences of 65 to 8192 keys, 8 key heads of 128, 550 MB in
+// 99 us (5.6 TB/s); of short work the start, where lengths, page numbers and keys are three loads that wait for each other (4 us), and
+// the kernel that joins the pieces (5 us): 16 heads of 16384 keys 22 us.  A workgroup = 4 waves = 16 rows (queries times the
 // query heads that share a key head) of one sequence and key head, and a piece of its keys (qfa_paged_work.h); 32-key tiles are
 // dealt to the waves, each with its own online softmax.  A tile lives in registers, double-buffered, as there.  A page holds 16
 // keys or a multiple, so the two halves of a tile lie in one page each: their pages' numbers are fetched 32 tiles ahead, one
