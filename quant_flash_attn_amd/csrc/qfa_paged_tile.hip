@@ -161,26 +161,31 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
     const int row_q = 32 * slot + opaque(lr), block_end = deal.end(item.s, item.rb) - 1, lo = deal.begin();
     int lim;   // last key of the row; one that is not there, or brings no token, goes along with the others and is not looked at
     u32x2 qc[KD];
-    float a_i, zq;
     const bool have = row_q < nrows;
-    {
-      const auto r = deal.row(item.p, item.h, BR * item.rb + min(row_q, nrows - 1));
-      const PagedSeq s = SHARED ? deal.load(r.b) : item.s;
-      const int64_t at = ((int64_t)r.b * a.work.Hk * a.work.G + r.qh) * a.work.N + r.i;
-      const int8_t *codes = a.q_codes + at * D + 8 * g;
+    const auto r_q = deal.row(item.p, item.h, BR * item.rb + min(row_q, nrows - 1));
+    const int64_t at_q = ((int64_t)r_q.b * a.work.Hk * a.work.G + r_q.qh) * a.work.N + r_q.i;
+    const int8_t *codes = a.q_codes + at_q * D + 8 * g;
 #pragma unroll
-      for (int m = 0; m < KD; ++m) qc[m] = *reinterpret_cast<const u32x2 *>(codes + 16 * m);
-      const float f = a.q_scale[at] * a.sm_scale_log2;
-      zq = (float)a.q_zero[at];
-      const int key = deal.last_key(r, s);   // (no branches: see qfa_paged_work.h)
-      const bool seen = have & (r.i < s.tokens), small = !have | (f < 0x1p-126f);
+    for (int m = 0; m < KD; ++m) qc[m] = *reinterpret_cast<const u32x2 *>(codes + 16 * m);
+    const float scale_q = a.q_scale[at_q];
+    const int8_t zero_q = a.q_zero[at_q];
+    PagedSeq seq_q = item.s;
+    if (SHARED) seq_q = {a.work.starts[r_q.b], a.work.counts ? a.work.counts[r_q.b] : a.work.N};
+    __builtin_amdgcn_sched_barrier(0);
+    issue(0);   // (waits for the pages alone, which were requested first)
+    __builtin_amdgcn_sched_barrier(0);
+    float a_i;
+    {
+      const float f = scale_q * a.sm_scale_log2;
+      if (SHARED) seq_q.tokens = max(0, min(seq_q.tokens, a.work.N));
+      const int key = deal.last_key(r_q, seq_q);   // (no branches: see qfa_paged_work.h)
+      const bool seen = have & (r_q.i < seq_q.tokens), small = !have | (f < 0x1p-126f);
       a_i = small ? 0x1p-126f : f;   // (not zero: the mask's -inf is multiplied by it)
       lim = seen ? key : block_end;
     }
-    issue(0);
     u32x4 qf[KD];
     {
-      const _Float16 neg = (_Float16)(-1152.0f - zq);
+      const _Float16 neg = (_Float16)(-1152.0f - (float)zero_q);
       const f16x2 neg2 = {neg, neg};
 #pragma unroll
       for (int m = 0; m < KD; ++m) {
@@ -221,14 +226,6 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
       }
 #pragma unroll
       for (int m = 0; m < KS; ++m) s = mfma_h(kf[m], qf[step * KS + m], s);
-    };
-    auto all_scores = [&](const unsigned char *buf, int kr, f32x16 &s) __attribute__((always_inline)) {
-      u32x4 kf[4][KS];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) request(buf, kr, i, kf[i]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) scores(s, i, kf[i]);
     };
     // What keys 8 aa + 4 g + {0..3} of rows kr .. have at `at`: their scales, their values' scales or those's log2
     auto constants = [&](const unsigned char *buf, int at, int kr, int aa) __attribute__((always_inline)) -> f32x4 {
@@ -292,7 +289,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
       ref = t;
       return alpha;
     };
-    // The reference moves where some p' (or the sum) has become too large; what was made of it is made again
+    // The reference moves where some p' (or the sum) has become too large, and at the first keys; what was made of it is made again
     auto check = [&](const unsigned char *buf, int kr, const f32x16 &s, Probs &r) __attribute__((always_inline)) {
       if (__builtin_amdgcn_ballot_w64(max((unsigned)r.top[0], (unsigned)r.top[1]) > PAGED_P_MAX_BITS || !(l_run + r.sum <= 0x1p100f)) != 0) {
         const float alpha = move(buf, kr, s);
@@ -391,13 +388,6 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
       });
     };
 
-    // the first reference, of the piece's first keys
-    if (active) {
-      f32x16 s;
-      all_scores(smem, 32 * NB * kw, s);
-      scale(smem, 32 * NB * kw, t0 * TK, ok, true, s);
-      move(smem, 32 * NB * kw, s);
-    }
     int cur = 0;
     for (int t = 0; t < nt; ++t) {
       const unsigned char *buf = smem + cur * GM::BUF;
