@@ -38,7 +38,7 @@ template <typename T> __device__ __forceinline__ void load_weight(const void *w,
   else load8<T>(static_cast<const T *>(w) + at, v);
 }
 
-template <typename T, int D, bool INTERLEAVED, bool BACK>
+template <typename T, int D, bool INTERLEAVED, bool BACK, bool ONCE>
 __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeKernelArgs p) {
   constexpr int LPR = D / 16, TOK = 256 / LPR;
   const bool second = blockIdx.x >= p.blocks0;
@@ -125,8 +125,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeKernelArgs p) {
     }
     if (live) {
       T *y = static_cast<T *>(a.y) + b * a.syb + h * a.syh + n * a.syn;
-      store8<T>(y + lane.a, v);
-      store8<T>(y + lane.b, v + 8);
+      store8<T, ONCE>(y + lane.a, v);
+      store8<T, ONCE>(y + lane.b, v + 8);
     }
     if (BACK && a.dw_parts && a.sw != 0) leave((int64_t)h * p.token_blocks + tb);
   }
@@ -200,11 +200,20 @@ template <typename T, int D, bool INTERLEAVED> static int launch_typed(const Nor
   a.blocks0 = (unsigned)blocks[0];
   a.token_blocks = (unsigned)tb;
   const dim3 grid((unsigned)(blocks[0] + blocks[1])), block(256);
+  // Stores are non-temporal where what a launch touches outgrows the last-level cache, of the forward up to three times its size.  4 x 64
+  // heads of 128 in bf16, forward + gradient, us with plain stores and with these: 512 tokens 15 + 24 and 14 + 23; 1024 (134 and 201 MB) 24
+  // + 36 and 22 + 35; 2048 51 + 76 and 44 + 64; 4096 106 + 163 and 106 + 142; 8192 204 + 329 and 220 + 320; in fp32 512 tokens 22 + 33 and
+  // 23 + 36, 1024 52 + 72 and 46 + 68, 2048 101 + 156 and 109 + 141, 4096 212 + 350 and 244 + 349.
+  const double bytes = (back ? 3.0 : 2.0) * (double)(tokens * (x.t[0].H + (x.t[1].H > 0 ? x.t[1].H : 0))) * D * sizeof(T);
+  const double last = (double)LAST_LEVEL_BYTES;
+  const bool once = bytes >= last && (back || bytes < 3 * last);
   if (!back) {
-    norm_rope_kernel<T, D, INTERLEAVED, false><<<grid, block, 0, st>>>(a);
+    if (once) norm_rope_kernel<T, D, INTERLEAVED, false, true><<<grid, block, 0, st>>>(a);
+    else norm_rope_kernel<T, D, INTERLEAVED, false, false><<<grid, block, 0, st>>>(a);
     return check_launch("qfa_norm_rope");
   }
-  norm_rope_kernel<T, D, INTERLEAVED, true><<<grid, block, 0, st>>>(a);
+  if (once) norm_rope_kernel<T, D, INTERLEAVED, true, true><<<grid, block, 0, st>>>(a);
+  else norm_rope_kernel<T, D, INTERLEAVED, true, false><<<grid, block, 0, st>>>(a);
   if (int e = check_launch("qfa_norm_rope_bwd")) return e;
   SumPartsTensor s[2] = {};
   for (int i = 0; i < 2; ++i)

@@ -51,7 +51,7 @@ __device__ __forceinline__ float load_scale(const void *p, int dtype, int64_t at
   return (float)static_cast<const __bf16 *>(p)[at];
 }
 
-template <typename T, int D, bool INTERLEAVED> __global__ __launch_bounds__(256) void paged_append_kernel(PagedRowsKernelArgs p) {
+template <typename T, int D, bool INTERLEAVED, bool ONCE> __global__ __launch_bounds__(256) void paged_append_kernel(PagedRowsKernelArgs p) {
   constexpr int LPR = D / 16, TOK = 256 / LPR;
   const PagedRowsArgs &x = p.x;
   const bool values = blockIdx.x >= p.blocks0;
@@ -72,8 +72,8 @@ template <typename T, int D, bool INTERLEAVED> __global__ __launch_bounds__(256)
   for (int h = h0; h < h1; ++h) {
     const T *row = static_cast<const T *>(src) + b * st[0] + h * st[1] + n * st[2];
     float v[16];
-    load8<T>(row + lane.a, v);
-    load8<T>(row + lane.b, v + 8);
+    load8<T, ONCE>(row + lane.a, v);
+    load8<T, ONCE>(row + lane.b, v + 8);
     if (norm) {
       float ss = 0.f, w[16];
 #pragma unroll
@@ -103,7 +103,7 @@ template <typename T, int D, bool INTERLEAVED> __global__ __launch_bounds__(256)
   }
 }
 
-template <typename T, int D> __global__ __launch_bounds__(256) void paged_read_kernel(PagedRowsKernelArgs p) {
+template <typename T, int D, bool ONCE> __global__ __launch_bounds__(256) void paged_read_kernel(PagedRowsKernelArgs p) {
   constexpr int LPR = D / 16, TOK = 256 / LPR;
   const PagedRowsArgs &x = p.x;
   const bool values = blockIdx.x >= p.blocks0;
@@ -121,7 +121,8 @@ template <typename T, int D> __global__ __launch_bounds__(256) void paged_read_k
     float v[16];
     if (place.page >= 0) {
       const int64_t at = place.of_head(x, h);
-      const u32x4 w = *reinterpret_cast<const u32x4 *>(codes + at * D + 16 * sub);
+      const u32x4 *from = reinterpret_cast<const u32x4 *>(codes + at * D + 16 * sub);
+      const u32x4 w = ONCE ? __builtin_nontemporal_load(from) : *from;
       const float s = load_scale(scale, x.scale_dtype, at);
       const int z = zero[at];
 #pragma unroll
@@ -154,9 +155,18 @@ template <typename T, int D> static int launch_td(const PagedRowsArgs &x, bool r
   a.x = x;
   int64_t grid;
   if (int e = plan(a, &grid)) return e;
-  if (read) paged_read_kernel<T, D><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
-  else if (x.interleaved) paged_append_kernel<T, D, true><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
-  else paged_append_kernel<T, D, false><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
+  // Non-temporal loads where what a launch touches outgrows the last-level cache.  4 x 32 heads of 128 in bf16, append and read in turn, us
+  // with plain loads and with these: 101 MB each 21 + 17 and 24 + 18; 203 MB 45 + 41 and 45 + 37 (alone, again and again 41 and 47, 36
+  // and 47); 405 MB 97 + 89 and 89 + 77; 811 MB 191 + 176 and 176 + 178.  Non-temporal stores of codes: 405 MB 104 + 86, of rows 80 + 85,
+  // 203 MB 38 + 55.
+  const bool once = 2.0 * (double)(x.B * x.N * x.H) * (D * (sizeof(T) + 1) + 3) >= (double)LAST_LEVEL_BYTES;
+  const dim3 g((unsigned)grid), block(256);
+  if (read && once) paged_read_kernel<T, D, true><<<g, block, 0, st>>>(a);
+  else if (read) paged_read_kernel<T, D, false><<<g, block, 0, st>>>(a);
+  else if (x.interleaved && once) paged_append_kernel<T, D, true, true><<<g, block, 0, st>>>(a);
+  else if (x.interleaved) paged_append_kernel<T, D, true, false><<<g, block, 0, st>>>(a);
+  else if (once) paged_append_kernel<T, D, false, true><<<g, block, 0, st>>>(a);
+  else paged_append_kernel<T, D, false, false><<<g, block, 0, st>>>(a);
   return check_launch(read ? "qfa_paged_read" : "qfa_paged_append");
 }
 template <typename T> static int launch_t(const PagedRowsArgs &x, bool read, hipStream_t st) {

@@ -10,24 +10,30 @@
 
 namespace qfa {
 
-// eight consecutive elements of T as floats, and back with one rounding
-template <typename T> __device__ __forceinline__ void load8(const T *p, float *v) {
+// eight consecutive elements of T as floats, and back with one rounding.  ONCE: non-temporal, for what nothing in the caches is to make
+// room for
+template <typename T, bool ONCE = false> __device__ __forceinline__ void load8(const T *p, float *v) {
   if constexpr (sizeof(T) == 4) {
-    const f32x4 a = reinterpret_cast<const f32x4 *>(p)[0], b = reinterpret_cast<const f32x4 *>(p)[1];
+    const f32x4 *w = reinterpret_cast<const f32x4 *>(p);
+    const f32x4 a = ONCE ? __builtin_nontemporal_load(w) : w[0], b = ONCE ? __builtin_nontemporal_load(w + 1) : w[1];
 #pragma unroll
     for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
   } else {
-    const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+    const u32x4 *from = reinterpret_cast<const u32x4 *>(p), w = ONCE ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
     for (int e = 0; e < 4; ++e) { v[2 * e] = lo_to_f32<T>(w[e]); v[2 * e + 1] = hi_to_f32<T>(w[e]); }
   }
 }
-template <typename T> __device__ __forceinline__ void store8(T *p, const float *v) {
+template <typename V, bool ONCE> __device__ __forceinline__ void store_words(void *p, V x) {
+  if constexpr (ONCE) __builtin_nontemporal_store(x, static_cast<V *>(p));
+  else *static_cast<V *>(p) = x;
+}
+template <typename T, bool ONCE = false> __device__ __forceinline__ void store8(T *p, const float *v) {
   if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<f32x4 *>(p)[0] = f32x4{v[0], v[1], v[2], v[3]};
-    reinterpret_cast<f32x4 *>(p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+    store_words<f32x4, ONCE>(p, f32x4{v[0], v[1], v[2], v[3]});
+    store_words<f32x4, ONCE>(p + 4, f32x4{v[4], v[5], v[6], v[7]});
   } else {
-    *reinterpret_cast<u32x4 *>(p) = u32x4{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])};
+    store_words<u32x4, ONCE>(p, u32x4{pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7])});
   }
 }
 

@@ -161,6 +161,25 @@ def test_partial_gradients_and_fixed_bits(qfa):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_one_large_call_is_many_small_ones(qfa, interleaved):
+    """What outgrows the last-level cache is stored with other hints."""
+    B, H, N, D = 4, 32, 2800, 128
+    g = torch.Generator(device=DEV).manual_seed(1)
+    q, k, dq, dk = (torch.randn(B, H, N, D, device=DEV, generator=g).bfloat16() for _ in range(4))
+    w = torch.rand(D, device=DEV, generator=g) + 0.5
+    cos, sin = (t.to(DEV) for t in m.table(N, D))
+
+    def step(at):
+        x = [t[at].detach().requires_grad_(True) for t in (q, k)]
+        y = qfa.norm_rope_pair(*x, w, w, cos, sin, interleaved=interleaved)
+        return tuple(t.detach() for t in y) + torch.autograd.grad(y, x, (dq[at], dk[at]))
+    whole = step(slice(0, B))
+    for b in range(B):
+        assert all(torch.equal(a[b:b + 1], p) for a, p in zip(whole, step(slice(b, b + 1))))
+
+
+@pytest.mark.gpu
 def test_stream_and_graph(qfa):
     q, k, w, cos, sin, pos, dy = (x for x in _make(2, 4, 2, 129, 128, 128, torch.bfloat16, "shared", torch.bfloat16, "starts", 13))
     t = [x.to(DEV) for x in (q, k, *w, cos, sin, pos)]

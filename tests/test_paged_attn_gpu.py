@@ -311,6 +311,22 @@ def test_two_calls_at_once(qfa):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_call_that_may_reach_a_large_cache(qfa, D):
+    """... reads it with other hints: the same bits whatever room the page table has."""
+    B, H, page = 8, 16, 64
+    pages = (400 << 20) // (2 * H * page * D)
+    q, small, table, starts, *_ = _problem(B, H, H, 1, D, page, [700 - 60 * i for i in range(B)], seed=D)
+    cache = [torch.zeros(pages, *t.shape[1:], dtype=t.dtype, device=DEV) for t in small]
+    for c, t in zip(cache, small):
+        c[:t.shape[0]] = t.to(DEV)
+    wide = torch.zeros(B, -(-pages // B), dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table.to(DEV)
+    q, table, starts = q.to(DEV), table.to(DEV), starts.to(DEV)
+    assert torch.equal(qfa.quant_flash_attn_paged(q, cache, wide, starts), qfa.quant_flash_attn_paged(q, [t.to(DEV) for t in small], table, starts))
+
+
+@pytest.mark.gpu
 def test_pages_past_32_bits(qfa):
     H, page, D = 8, 64, 128
     pages = (1 << 32) // (H * page * D) + 64

@@ -151,6 +151,26 @@ def test_rows_past_32_bits(qfa):
 
 
 @pytest.mark.gpu
+def test_one_large_call_is_many_small_ones(qfa):
+    """What outgrows the last-level cache is loaded with other hints."""
+    B, H, N, D, page = 4, 32, 2800, 128, 64
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randn(B, H, N, D, device=DEV, generator=g).bfloat16() for _ in range(2))
+    cos, sin = (t.to(DEV) for t in m.table(N, D))
+    width = -(-N // page)
+    table, zero = torch.arange(B * width, device=DEV, dtype=torch.int32).reshape(B, width), torch.zeros(B, dtype=torch.int32, device=DEV)
+    for interleaved in (False, True):
+        whole, parts = (qfa.make_paged_cache(B * width, H, page, D) for _ in range(2))
+        qfa.paged_cache_append(whole, k, v, table, zero, cos=cos, sin=sin, interleaved=interleaved)
+        for b in range(B):
+            qfa.paged_cache_append(parts, k[b:b + 1], v[b:b + 1], table[b:b + 1], zero[:1], cos=cos, sin=sin, interleaved=interleaved)
+        assert all(torch.equal(a, b) for a, b in zip(whole, parts))
+    rows = qfa.paged_cache_read(whole, table, zero, N)
+    for b in range(B):
+        assert all(torch.equal(r[b:b + 1], x) for r, x in zip(rows, qfa.paged_cache_read(whole, table[b:b + 1], zero[:1], N)))
+
+
+@pytest.mark.gpu
 def test_graph_follows_the_lengths(qfa):
     B, H, N, D, page = 3, 2, 2, 64, 16
     table, pages = m.shared_pages(B, 4, 0, 1)
