@@ -63,7 +63,7 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
   // a thread's chunks: 4 columns of chunks by 4 rows per 16 lanes, as SkvTileStage has them
   constexpr int CH = GM::CPR / 4;
   const unsigned quarter_mask = (1u << page_quarters_log2) - 1;
-  auto opaque = [](int y) __attribute__((always_inline)) -> int {
+  auto opaque = [](auto y) __attribute__((always_inline)) {
     asm volatile("" : "+v"(y));
     return y;
   };
@@ -127,12 +127,15 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
     auto commit_chunk = [&](unsigned char *buf, int lds, int i) __attribute__((always_inline)) {
       const Chunks &c = i < Chunks::N ? ck : cv;
       const int n = i % Chunks::N;
-      const unsigned nz = 0xe400u | (c.z[n] ^ 0x80u), nz2 = nz | nz << 16;   // -(1152 + zero_point), twice
+      // (What was loaded is looked at here and not before: the compiler moves what both callers begin with, and with it the wait for the
+      // loads, in front of the tile.)
+      const unsigned zero = opaque(c.z[n]), nz = 0xe400u | (zero ^ 0x80u), nz2 = nz | nz << 16;   // -(1152 + zero_point), twice
       const f16x2 neg = __builtin_bit_cast(f16x2, nz2);
       unsigned char *side = buf + (i < Chunks::N ? 0 : GM::SIDE) + n * (Chunks::STEP * 32);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const u32x4 m = expand_codes(c.w[n][2 * k], c.w[n][2 * k + 1]);
+        const unsigned w0 = opaque(c.w[n][2 * k]), w1 = opaque(c.w[n][2 * k + 1]);
+        const u32x4 m = expand_codes(w0, w1);
         u32x4 e;
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
@@ -144,7 +147,8 @@ template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256
     };
     auto commit_scales = [&](unsigned char *buf) __attribute__((always_inline)) {
       const int l = opaque(lane);
-      const float f = scale_dtype == QFA_F32 ? __builtin_bit_cast(float, sc) : scale_dtype == QFA_F16 ? lo_to_f32<_Float16>(sc) : lo_to_f32<__bf16>(sc);
+      const unsigned raw = opaque(sc);
+      const float f = scale_dtype == QFA_F32 ? __builtin_bit_cast(float, raw) : scale_dtype == QFA_F16 ? lo_to_f32<_Float16>(raw) : lo_to_f32<__bf16>(raw);
       *reinterpret_cast<float *>(buf + (wave % 2 == 0 ? GM::CONST_K : GM::CONST_V) + l * 4) = f;
       // (log2 of the keys' scales goes where nobody reads it)
       *reinterpret_cast<float *>(buf + (wave % 2 == 0 ? GM::CONST_X : GM::CONST_L) + l * 4) = __builtin_floorf(__builtin_amdgcn_logf(fabsf(f)));
