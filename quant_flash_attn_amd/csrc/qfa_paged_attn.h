@@ -23,7 +23,8 @@ constexpr unsigned PAGED_P_MAX_BITS = 0x6400;   // that limit as a binary16 numb
 
 constexpr int PAGED_TILE = 64;   // keys of a tile there
 // blocks of 64 or 128 rows: qw = 2 or 4 waves side by side; the workgroups of a launch, and the launch
-inline int paged_tile_grid(int D) { return D == 256 ? 256 : 512; }
+// (three workgroups on a CU with 64 elements: 2 to 5 % over two)
+inline int paged_tile_grid(int D) { return D == 256 ? 256 : D == 64 ? 768 : 512; }
 int launch_paged_tile(const PagedAttnKernelArgs &a, bool shared, int D, int scale_dtype, int qw, hipStream_t st);
 
 }  // namespace qfa

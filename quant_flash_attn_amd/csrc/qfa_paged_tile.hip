@@ -40,7 +40,7 @@ template <int D> struct PagedChunks {
 typedef const __attribute__((address_space(1))) unsigned char *GlobalBytes;
 typedef const __attribute__((address_space(1))) u32x4 *GlobalWords;
 
-template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void paged_tile_kernel(PagedAttnKernelArgs a_, int scale_dtype) {
+template <int D, int QW, bool SHARED> __global__ __launch_bounds__(256, D == 256 ? 1 : D == 64 ? 3 : 2) void paged_tile_kernel(PagedAttnKernelArgs a_, int scale_dtype) {
   typedef PagedTileGeom<D, QW> GM;
   typedef PagedChunks<D> Chunks;
   constexpr int TK = GM::TK, NB = GM::NB, KW = GM::KW, BR = GM::BR, DB = D / 32, KD = D / 16, SLAB = GM::SLAB;
