@@ -383,39 +383,46 @@ struct PagedPieces {
   }
 };
 struct PagedSum { float m, l; f32x4 acc; };
-// Pieces are loaded four at a time (past the last one: once more that one, which then counts for nothing); one by one, each would wait
-// for its own loads
-template <int D> __device__ __forceinline__ void paged_add(const PagedWork &work, const PagedPieces &at, int d, int group, int groups, PagedSum &x) {
-  constexpr int AT_ONCE = 4;
+// Adds a row's pieces, or those of R rows that lie `step` apart in their blocks.  Four are loaded at a time (past the last piece: once more
+// that one, which then counts for nothing); one by one, each would wait for its own loads
+template <int D, int R> __device__ __forceinline__ void paged_add(const PagedWork &work, const PagedPieces &at, int d, int group, int groups, PagedSum (&x)[R],
+                                                                  int step) {
+  constexpr int AT_ONCE = 4 / R;
   const float *po = at.whole >= 0 ? work.whole : work.slots, *pml = at.whole >= 0 ? work.whole_ml : work.slots_ml;
   for (unsigned w = at.w0 + group; w <= at.w1; w += AT_ONCE * groups) {
-    f32x2 ml[AT_ONCE];
-    f32x4 y[AT_ONCE];
+    f32x2 ml[R][AT_ONCE];
+    f32x4 y[R][AT_ONCE];
 #pragma unroll
     for (int j = 0; j < AT_ONCE; ++j) {
       const unsigned wj = min(w + j * groups, at.w1);
       const int64_t i = at.whole >= 0 ? at.whole : ((int64_t)wj * 2 + (wj == at.w0 ? 1 : 0)) * work.br + at.in_block;
-      ml[j] = *reinterpret_cast<const f32x2 *>(pml + 2 * i);
-      y[j] = *reinterpret_cast<const f32x4 *>(po + i * D + d);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        ml[r][j] = *reinterpret_cast<const f32x2 *>(pml + 2 * (i + r * step));
+        y[r][j] = *reinterpret_cast<const f32x4 *>(po + (i + r * step) * D + d);
+      }
     }
-    float m_new = x.m;
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) {
-      const float l = ml[j][1];
-      if ((w + j * groups > at.w1) | (l == 0.f)) ml[j] = f32x2{NO_KEY, 0.f};   // (a piece that saw no key: its sums are zero)
-      m_new = fmaxf(m_new, ml[j][0]);
-    }
-    const float s0 = __builtin_amdgcn_exp2f(x.m - m_new);
-    x.m = m_new;
-    x.l *= s0;
+    for (int r = 0; r < R; ++r) {
+      float m_new = x[r].m;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x.acc[e] *= s0;
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const float l = ml[r][j][1];
+        if ((w + j * groups > at.w1) | (l == 0.f)) ml[r][j] = f32x2{NO_KEY, 0.f};   // (a piece that saw no key: its sums are zero)
+        m_new = fmaxf(m_new, ml[r][j][0]);
+      }
+      const float s0 = __builtin_amdgcn_exp2f(x[r].m - m_new);
+      x[r].m = m_new;
+      x[r].l *= s0;
 #pragma unroll
-    for (int j = 0; j < AT_ONCE; ++j) {
-      const float l = ml[j][1], s1 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[j][0] - m_new);
-      x.l += l * s1;
+      for (int e = 0; e < 4; ++e) x[r].acc[e] *= s0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x.acc[e] += mul_zero_wins(s1, y[j][e]);
+      for (int j = 0; j < AT_ONCE; ++j) {
+        const float l = ml[r][j][1], s1 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml[r][j][0] - m_new);
+        x[r].l += l * s1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[r].acc[e] += mul_zero_wins(s1, y[r][j][e]);
+      }
     }
   }
 }
@@ -431,49 +438,64 @@ template <int D> __global__ __launch_bounds__(256) void paged_merge_kernel(Paged
   const PagedSeq seq = own.load(b);
   const PagedPieces mine(first, each, own.tiles(seq, rb), (int64_t)bh * own.rows + r0, r0 % own.BR);
   if (!a.own.whole && mine.whole >= 0) return;   // stored
+  auto store = [&](int r, const PagedSum &x) __attribute__((always_inline)) {
+    const int i = r / a.own.G;
+    const float inv = i >= seq.tokens || x.l == 0.f ? 0.f : 1.0f / x.l;
+    const int64_t off = (((int64_t)b * a.own.Hk * a.own.G + h * a.own.G + r % a.own.G) * a.own.N + i) * D;
+    store4(static_cast<char *>(a.o) + off * (a.o_dtype == QFA_F32 ? 4 : 2), a.o_dtype, d,
+           f32x4{mul_zero_wins(x.acc[0], inv), mul_zero_wins(x.acc[1], inv), mul_zero_wins(x.acc[2], inv), mul_zero_wins(x.acc[3], inv)});
+  };
+  if (n > SLOTS && a.shared.grid == 0) {   // two rows at a time
+    for (int k = slot; k < n; k += 2 * SLOTS) {
+      PagedSum x[2] = {{NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}}, {NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}}};
+      PagedPieces p = mine;
+      p.in_block += k;
+      paged_add<D, 2>(a.own, p, d, 0, 1, x, k + SLOTS < n ? SLOTS : 0);
+      store(r0 + k, x[0]);
+      if (k + SLOTS < n) store(r0 + k + SLOTS, x[1]);
+    }
+    return;
+  }
   const int groups = n >= SLOTS ? 1 : SLOTS / n;   // of pieces
   for (int first = 0; first < n; first += SLOTS) {
     const int k = groups == 1 ? first + slot : slot % n, group = groups == 1 ? 0 : slot / n;   // row of the chunk
     const bool live = k < n && group < groups;
     const int r = r0 + min(k, n - 1), i = r / a.own.G;
-    PagedSum x = {NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+    PagedSum x[1] = {{NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}}};
     if (live && i < seq.tokens) {
       PagedPieces p = mine;
       p.in_block += r - r0;
       if (p.whole >= 0) p.whole += r - r0;
-      paged_add<D>(a.own, p, d, group, groups, x);
+      paged_add<D, 1>(a.own, p, d, group, groups, x, 0);
       if (a.shared.grid > 0) {
         const PagedDeal<true, false> all(a.shared, a.shared.br, a.shared.tk);
         const int rs = b * own.rows + r, item = h * all.blocks + rs / all.BR;
         const unsigned u = all.units({0, 0}, 0);
         const PagedPieces q((unsigned)item * u + (unsigned)a.shared.extra, all.each, all.tiles({0, 0}, 0), (int64_t)h * all.rows + rs, rs % all.BR);
-        paged_add<D>(a.shared, q, d, group, groups, x);
+        paged_add<D, 1>(a.shared, q, d, group, groups, x, 0);
       }
     }
     if (groups > 1) {
-      *reinterpret_cast<f32x4 *>(&red[slot][d]) = x.acc;
+      *reinterpret_cast<f32x4 *>(&red[slot][d]) = x[0].acc;
       if (tid % CL == 0) {
-        red[slot][D] = x.m;
-        red[slot][D + 1] = x.l;
+        red[slot][D] = x[0].m;
+        red[slot][D + 1] = x[0].l;
       }
       __syncthreads();
       if (slot >= n) return;
-      x = {NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
-      for (int g = 0; g < groups; ++g) x.m = fmaxf(x.m, red[g * n + slot][D]);
+      x[0] = {NO_KEY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+      for (int g = 0; g < groups; ++g) x[0].m = fmaxf(x[0].m, red[g * n + slot][D]);
       for (int g = 0; g < groups; ++g) {
-        const float s = __builtin_amdgcn_exp2f(red[g * n + slot][D] - x.m);
-        x.l += red[g * n + slot][D + 1] * s;
+        const float s = __builtin_amdgcn_exp2f(red[g * n + slot][D] - x[0].m);
+        x[0].l += red[g * n + slot][D + 1] * s;
         const f32x4 y = *reinterpret_cast<const f32x4 *>(&red[g * n + slot][d]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x.acc[e] += y[e] * s;
+        for (int e = 0; e < 4; ++e) x[0].acc[e] += y[e] * s;
       }
     } else if (!live) {
       return;
     }
-    const float inv = x.l == 0.f ? 0.f : 1.0f / x.l;
-    const int64_t off = (((int64_t)b * a.own.Hk * a.own.G + h * a.own.G + r % a.own.G) * a.own.N + i) * D;
-    store4(static_cast<char *>(a.o) + off * (a.o_dtype == QFA_F32 ? 4 : 2), a.o_dtype, d,
-           f32x4{x.acc[0] * inv, x.acc[1] * inv, x.acc[2] * inv, x.acc[3] * inv});
+    store(r, x[0]);
   }
 }
 
