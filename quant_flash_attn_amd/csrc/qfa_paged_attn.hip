@@ -565,7 +565,7 @@ template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
   for (int i = 0; i < 2; ++i) {
     const int br = block_rows(problem[i], D, (i == 0 ? x.B : 1) * x.Hk), grid = x.prefix > 0 || i == 0 ? work_grid(br, D) : 0;
     w[i] = {x.starts, x.counts, (int)x.B, (int)x.Hk, G, (int)x.N, x.causal, (int)x.prefix, (int)(x.width << x.page_log2), grid, br,
-            br == PAGED_ROWS ? SKV_TILE : PAGED_TILE, br == PAGED_ROWS ? 8 : 4, nullptr, nullptr, nullptr, nullptr, nullptr};
+            br == PAGED_ROWS ? SKV_TILE : PAGED_TILE, br == PAGED_ROWS ? 12 : 4, nullptr, nullptr, nullptr, nullptr, nullptr};
     if (grid == 0) continue;
     if (i == 0) {
       w[i].first = reinterpret_cast<unsigned *>(mem);
