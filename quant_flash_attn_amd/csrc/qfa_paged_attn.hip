@@ -7,7 +7,7 @@
 // 99 us (5.6 TB/s); of short work the start, where lengths, page numbers and keys are three loads that wait for each other (4 us), and
 // the kernel that joins the pieces (5 us): 16 heads of 16384 keys 22 us.  A workgroup = 4 waves = 16 rows (queries times the
 // query heads that share a key head) of one sequence and key head, and a piece of its keys (qfa_paged_work.h); 32-key tiles are
-// dealt to the waves, each with its own online softmax.  A tile lives in registers, double-buffered, as there.  A page holds 16
+// dealt to the waves, each with its own online softmax.  A tile lives in registers, double-buffered (but for 256 elements) as there.  A page holds 16
 // keys or a multiple, so the two halves of a tile lie in one page each: their pages' numbers are fetched 32 tiles ahead, one
 // lane per half, and read out of the lanes as scalars, so that no load of keys waits for the page table.
 //
@@ -22,11 +22,11 @@
 namespace qfa {
 
 constexpr int PAGED_ROWS = 16;
-constexpr int paged_wgs_per_cu(int D) { return D == 256 ? 1 : 2; }
+constexpr int PAGED_WGS = 256 * 2;   // two on a CU
 
 __device__ __forceinline__ i32x4 paged_mfma_i8(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
-template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __launch_bounds__(256, paged_wgs_per_cu(D)) void paged_rows_kernel(PagedAttnKernelArgs a) {
+template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnKernelArgs a) {
   constexpr int KM = D / 64;    // 64-wide k-steps of the score product
   constexpr int DB = D / 16;    // 16-row blocks of O^T
   constexpr int VB = D / 16;    // bytes of a V row per lane
@@ -78,24 +78,34 @@ template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __la
     };
     int pg = pages_from(0), pg_next = my_tiles > 32 ? pages_from(32) : -1;
     // (every load is issued whether the tile exists or not -- a missing one has an empty descriptor and fetches nothing)
-    auto load = [&](Tile &t, int i) __attribute__((always_inline)) {
+    int64_t first[2];   // first row of each half among all rows
+    auto load_keys = [&](Tile &t, int i) __attribute__((always_inline)) {
       if (i > 0 && i % 32 == 0) {
         pg = pg_next;
         pg_next = i + 32 < my_tiles ? pages_from(i + 32) : -1;
       }
       const int tile = t0 + wave + 4 * i;
       t.ok = 0;
-      int64_t first[2];   // first row of the half among all rows
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb) {
         const int id = __builtin_amdgcn_readlane(pg, 2 * (i % 32) + rb);
         const bool ok = id >= 0;
         t.ok |= ok ? 1 << rb : 0;
         first[rb] = (((int64_t)(ok ? id : 0) * a.work.Hk + item.h) << a.page_log2) + (((2 * tile + rb) & ((1 << page_halves_log2) - 1)) << 4);
-        const rsrc_t rk = make_rsrc(a.kc + first[rb] * D, ok ? 16 * D : 0), rv = make_rsrc(a.vc + first[rb] * D, ok ? 16 * D : 0);
+        const rsrc_t rk = make_rsrc(a.kc + first[rb] * D, ok ? 16 * D : 0);
 #pragma unroll
         for (int m = 0; m < KM; ++m)
           t.k[rb][m] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off, 64 * m, HINT));
+      }
+      const int64_t at = (lane % 32 < 16 ? first[0] : first[1]) + lane % 16;
+      if constexpr (sizeof(S) == 4) t.sc = __builtin_bit_cast(unsigned, sc_base[at]);
+      else t.sc = __builtin_bit_cast(unsigned short, sc_base[at]);
+      t.zp = (unsigned)(unsigned char)zp_base[at];
+    };
+    auto load_values = [&](Tile &t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb) {
+        const rsrc_t rv = make_rsrc(a.vc + first[rb] * D, t.ok >> rb & 1 ? 16 * D : 0);
 #pragma unroll
         for (int e = 4 * rb; e < 4 * rb + 4; ++e) {
           const int soff = (e % 4) * D;
@@ -112,10 +122,10 @@ template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __la
           }
         }
       }
-      const int64_t at = (lane % 32 < 16 ? first[0] : first[1]) + lane % 16;
-      if constexpr (sizeof(S) == 4) t.sc = __builtin_bit_cast(unsigned, sc_base[at]);
-      else t.sc = __builtin_bit_cast(unsigned short, sc_base[at]);
-      t.zp = (unsigned)(unsigned char)zp_base[at];
+    };
+    auto load = [&](Tile &t, int i) __attribute__((always_inline)) {
+      load_keys(t, i);
+      load_values(t);
     };
 
     // the block's queries are requested beside the pages, and quantized while the first keys are on their way
@@ -142,7 +152,7 @@ template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __la
       lim = seen ? key : block_end;
     }
 
-    Tile ta, tb;
+    Tile ta;
     load(ta, 0);
 
     // ---- the block's queries, quantized: codes to LDS, a = scale * sm_scale * log2(e), zero point and c = sum - D * zp
@@ -178,7 +188,9 @@ template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __la
     for (int i = 0; i < DB; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     float ref = NO_KEY, l_run = 0.f, w_run = 0.f;   // p = 2^(a_i * u - ref)
 
-    auto tile = [&](const Tile &t, int i) __attribute__((always_inline)) {
+    // next: called once the tile's keys are done with
+    auto tile = [&](Tile &t, int i, auto next) __attribute__((always_inline)) {
+      const int there = t.ok;
       const int key0 = (t0 + wave + 4 * i) * SKV_TILE;
       // token constants: K (scale, zp as an integer), V (scale, the binary16 number 1152 + zp)
       {
@@ -206,13 +218,14 @@ template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __la
           f[rb][v] = (float)dot * __builtin_bit_cast(float, scw);
         }
       }
-      if (key0 + SKV_TILE - 1 > first_lim || key0 < lo || t.ok != 3) {
+      next();
+      if (key0 + SKV_TILE - 1 > first_lim || key0 < lo || there != 3) {
         const int last = lim - key0 - 4 * G, first = lo - key0 - 4 * G;   // (this lane's keys are key0 + 4 G + 16 rb + v)
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
           for (int v = 0; v < 4; ++v)
-            if (16 * rb + v > last || 16 * rb + v < first || !(t.ok >> rb & 1)) f[rb][v] = -INFINITY;
+            if (16 * rb + v > last || 16 * rb + v < first || !(there >> rb & 1)) f[rb][v] = -INFINITY;
       }
       // ---- p and its row sum, p' = p * scale_j and the largest of them
       float ps[8], mx = 0.f, l_new = 0.f;
@@ -291,11 +304,21 @@ template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __la
         oacc[j] = mfma_h16(vf, pf, oacc[j]);
       }
     };
-    for (int i = 0; i < my_tiles; i += 2) {
-      load(tb, i + 1);
-      tile(ta, i);
-      load(ta, i + 2);
-      if (i + 1 < my_tiles) tile(tb, i + 1);
+    // Rows of 256 elements: two tiles in registers would leave room for one workgroup on a CU (1 to 12 % slower); a tile's keys and values
+    // are requested anew as soon as they are done with
+    if constexpr (D == 256) {
+      for (int i = 0; i < my_tiles; ++i) {
+        tile(ta, i, [&]() __attribute__((always_inline)) { load_keys(ta, i + 1); });
+        load_values(ta);
+      }
+    } else {
+      Tile tb;
+      for (int i = 0; i < my_tiles; i += 2) {
+        load(tb, i + 1);
+        tile(ta, i, []() {});
+        load(ta, i + 2);
+        if (i + 1 < my_tiles) tile(tb, i + 1, []() {});
+      }
     }
 
     // ---- merge of the four waves, through LDS: [wave][row][D] and (m, l) behind
@@ -508,7 +531,7 @@ static int block_rows(int64_t rows, int D, int64_t problems) {
   if (rows <= PAGED_ROWS || (rows <= 2 * PAGED_ROWS && (D != 128 || problems <= 128))) return PAGED_ROWS;
   return rows <= 64 ? 64 : 128;
 }
-static int work_grid(int br, int D) { return br == PAGED_ROWS ? 256 * paged_wgs_per_cu(D) : paged_tile_grid(D); }
+static int work_grid(int br, int D) { return br == PAGED_ROWS ? PAGED_WGS : paged_tile_grid(D); }
 // bytes of a launch's slots, and of its whole items
 static int64_t slots_bytes(int br, int D) { return 2LL * work_grid(br, D) * br * (D + 2) * 4; }
 static int64_t whole_bytes(int64_t rows, int D) { return (rows * (D + 2) * 4 + 15) / 16 * 16; }
