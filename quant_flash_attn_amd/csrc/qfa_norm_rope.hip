@@ -2,8 +2,8 @@
 //     y = rot(x * r * w),   r = 1 / sqrt(mean(x^2) + eps)
 //     g = rot^T(dy),  dw = sum over rows of g x r,  dx = r (g w) - x r^3 mean((g w) x)
 // Bound by memory: the forward reads and writes each row once, the backward reads x and dy and writes dx; r is computed again
-// from x, which it reads anyway, so the forward keeps nothing.  4 x 64 heads x 4096 x 128 bf16: forward 100 us (5.4 TB/s), gradient
-// 162 us (5.0 TB/s); a copy of that size 5.0.
+// from x, which it reads anyway, so the forward keeps nothing.  4 x 64 heads x 4096 x 128 bf16: forward 102 us (5.3 TB/s), gradient
+// 150 us (5.4 TB/s); a copy of that size 5.0.
 //
 // A row is held by D/16 lanes (RopeLane), a workgroup of 256 threads holds 4096/D tokens of one head at a time and walks over
 // `heads_each` heads of these tokens, so that the angles (4 D bytes of fp32 per token against 2 D of a 16-bit row) are read once

@@ -1,6 +1,6 @@
 // Attention on a paged INT8 cache for many rows at once: a piece of a prompt, or the queries of all sequences that share a prefix.
 // The same arithmetic as qfa_paged_attn.hip; there 16 rows read a key's codes, here 64 or 128 share them.
-// 2 x 32 heads, 333 rows on 6500 keys of 128: 147 us (470 TFLOP/s); 256 rows of each of 8 heads on 16384 keys 47 us, of which start and
+// 2 x 32 heads, 333 rows on 6500 keys of 128: 146 us (480 TFLOP/s); 256 rows of each of 8 heads on 16384 keys 47 us, of which start and
 // end are 10.  Bound by the vector pipe (61 % busy; the matrix pipe 34 %) and what two waves on a SIMD leave idle of it.
 //
 // The four waves together turn a tile of 64 keys and of their values into binary16 integers code - zero_point (exact) in LDS, in
