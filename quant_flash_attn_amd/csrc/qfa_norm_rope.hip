@@ -155,12 +155,15 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_rope_dw_kerne
   else static_cast<T *>(a.dw)[o + col] = (T)s;
 }
 
-// Heads that a workgroup walks over: as many as leave the chip 2048 workgroups, eight at most.  (64 heads of 128, 4 x 4096 tokens: eight
-// 100 us forward and 162 backward, sixteen 115 and 178; the fewer partial sums of dw take 5.6 us in place of 8.)
+// Heads that a workgroup walks over: as many as leave the chip 512 workgroups, eight at most.  Forward, gradient and the weights' sums in
+// us, 4 x (32 + 8) heads of 128 in bf16, with 2048 workgroups and with 512: 256 tokens 22 and 20, 512 32 and 27, 1024 46 and 43, 2048
+// 80 and 81; 64 heads of 64 27 and 24, 43 and 38, 67 and 60 from 512 on; 4 x (16 + 4) of 256 in fp32 45 and 42, 80 and 77, 159 and 146;
+// 4 x (32 + 8) of 256 in fp16 47 and 43, 82 and 90, 160 and 157.  (64 heads of 128, 4 x 4096 tokens: eight heads 100 us forward and 162
+// backward, sixteen 115 and 178.)
 static int heads_each(int64_t tokens, int64_t H, int D) {
   const int64_t blocks = (tokens + 4096 / D - 1) / (4096 / D) * H;
   int e = 1;
-  while (e < 8 && e < H && blocks / (2 * e) >= 2048) e *= 2;
+  while (e < 8 && e < H && blocks / (2 * e) >= 512) e *= 2;
   return e;
 }
 static int64_t token_blocks(int64_t tokens, int D) { return (tokens + 4096 / D - 1) / (4096 / D); }

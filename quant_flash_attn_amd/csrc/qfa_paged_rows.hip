@@ -136,7 +136,8 @@ template <typename T, int D, bool ONCE> __global__ __launch_bounds__(256) void p
   }
 }
 
-// heads per workgroup as in qfa_norm_rope.hip: as many as leave the chip 2048 workgroups, eight at most
+// heads per workgroup: as many as leave the chip 2048 workgroups, eight at most (with 2048 and with 1024: 4 x 2048 tokens of 8 heads of 128 15 + 12.6 and
+// 14.5 + 10.5 us for append and read, 1024 tokens of 16 heads of 256 23 + 17 and 24 + 20)
 static int plan(PagedRowsKernelArgs &a, int64_t *grid) {
   const int64_t tb = (a.x.B * a.x.N + 4096 / a.x.D - 1) / (4096 / a.x.D);
   int e = 1;
