@@ -420,7 +420,8 @@ int64_t qfa_attn_bwd_split_workspace_bytes(int64_t B, int64_t H, int64_t Nq, int
 /*
  * RMSNorm of every head's row and the position rotation, in one pass, for one or two tensors (queries and keys; k nullable):
  *     y = rot(x * w / sqrt(mean(x^2) + eps)),   rot: (a, b) -> (a cos - b sin, b cos + a sin) on `rotated` elements of a row
- * Everything in fp32, rounded once.  No counterpart in the reference, whose operators take queries and keys as they come.
+ * Everything in fp32, rounded once; rows whose squares leave fp32's range are normed at another scale, so that every row that the types
+ * hold is.  No counterpart in the reference, whose operators take queries and keys as they come.
  *   x, y       [B,H,N,D] of dtype, D in {64, 128, 256}, 16-byte aligned, strides (batch, head, token) multiples of 16 bytes
  *   weight     nullable (no norm); [D], or [H,D] where weight_per_head; of w_dtype (QFA_F32 or dtype), for both tensors the same type
  *   cos, sin   [rope_rows, rotated / 2] float, dense, 16-byte aligned; rotated a multiple of 16 up to D.  NULL with rotated 0: no rotation
@@ -442,7 +443,7 @@ int qfa_norm_rope(const qfa_norm_rope_tensor *q, const qfa_norm_rope_tensor *k, 
                   int w_dtype, int64_t B, int64_t N, int D, void *stream);
 
 /*
- * Its gradient:  g = rot^T(dy),  dweight = sum over rows of g x r,  dx = r (g w) - x r^3 mean(g w x),  r = 1 / sqrt(mean(x^2) + eps).
+ * Its gradient:  g = rot^T(dy),  dweight = sum over rows of g x r,  dx = r (g w - x r mean(g w x r)),  r = 1 / sqrt(mean(x^2) + eps).
  * dx goes to y.  workspace: qfa_norm_rope_bwd_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant (not needed where no
  * dweight is asked for); the sums are added up in a fixed order.  weight_per_head as of the tensors: where the two differ, the sum of
  * what either needs alone (Hk 0).

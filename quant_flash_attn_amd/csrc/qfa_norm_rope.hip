@@ -1,6 +1,6 @@
 // RMSNorm of every head's row and the position rotation, in one pass, and its gradient:
 //     y = rot(x * r * w),   r = 1 / sqrt(mean(x^2) + eps)
-//     g = rot^T(dy),  dw = sum over rows of g x r,  dx = r (g w) - x r^3 mean((g w) x)
+//     g = rot^T(dy),  dw = sum over rows of g x r,  dx = r (g w - x r mean((g w) x r))
 // Bound by memory: the forward reads and writes each row once, the backward reads x and dy and writes dx; r is computed again
 // from x, which it reads anyway, so the forward keeps nothing.  4 x 64 heads x 4096 x 128 bf16: forward 102 us (5.3 TB/s), gradient
 // 150 us (5.4 TB/s); a copy of that size 5.0.
@@ -90,10 +90,8 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeKernelArgs p) {
     }
     if constexpr (!BACK) {
       if (a.w) {
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) ss += v[e] * v[e];
-        const float r = 1.0f / sqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
+        float k;
+        const float r = row_inverse_rms<LPR>(v, p.eps, k);
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
       }
@@ -105,19 +103,20 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeKernelArgs p) {
       load8<T>(dy + lane.b, g + 8);
       if (p.half) lane.template turn<true>(g);
       if (a.w) {
-        float ss = 0.f, dot = 0.f;
+        // xh = x r, and dx = r (g w - xh mean(g w xh)): every factor is of the size of what it stands for (r^3, and x times it, leave fp32's
+        // range where dx does not)
+        float k, dot = 0.f;
+        const float r = row_inverse_rms<LPR>(v, p.eps, k);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          ss += v[e] * v[e];
-          dot += g[e] * w[e] * v[e];
+          v[e] *= r;
+          if (live) dw[e] += g[e] * v[e];
+          g[e] *= w[e];
+          dot += g[e] * v[e];
         }
-        const float r = 1.0f / sqrtf(row_sum<LPR>(ss) * (1.0f / D) + p.eps);
-        const float c = r * r * r * (row_sum<LPR>(dot) * (1.0f / D));
+        const float n = row_sum<LPR>(dot) * (1.0f / D), rk = r * k;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (live) dw[e] += g[e] * v[e] * r;
-          v[e] = r * (g[e] * w[e]) - v[e] * c;
-        }
+        for (int e = 0; e < 16; ++e) v[e] = rk * (g[e] - v[e] * n);
       } else {
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[e] = g[e];

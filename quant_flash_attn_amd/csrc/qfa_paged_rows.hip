@@ -75,10 +75,8 @@ template <typename T, int D, bool INTERLEAVED, bool ONCE> __global__ __launch_bo
     load8<T, ONCE>(row + lane.a, v);
     load8<T, ONCE>(row + lane.b, v + 8);
     if (norm) {
-      float ss = 0.f, w[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) ss += v[e] * v[e];
-      const float r = 1.0f / sqrtf(row_sum<LPR>(ss) * (1.0f / D) + x.eps);
+      float k, w[16];
+      const float r = row_inverse_rms<LPR>(v, x.eps, k);
       const int64_t at = x.w_per_head ? (int64_t)h * D : 0;
       if (x.w_f32) {
         load8<float>(static_cast<const float *>(x.w) + at + lane.a, w);

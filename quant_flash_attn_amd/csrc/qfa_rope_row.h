@@ -47,6 +47,29 @@ template <int LPR> __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
+// 1 / sqrt(mean(x^2) + eps) of a row of LPR lanes, for v[e] as it then stands: where the squares leave fp32's range (their mean is infinite, or
+// below 2^-100, where what underflows begins to count) v, eps and the result are those of the row times `k`, a power of two, and x / rms is
+// v * result all the same; 1 for any other row.  A row with an infinity or a NaN keeps it.
+template <int LPR> __device__ __forceinline__ float row_inverse_rms(float (&v)[16], float eps, float &k) {
+  constexpr float PART = 1.0f / (16 * LPR);
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) ss += v[e] * v[e];
+  float mean = row_sum<LPR>(ss) * PART + eps;
+  k = 1.f;
+  if (!(mean >= 0x1p-100f && mean < INFINITY)) {   // (the same in all lanes of a row)
+    k = mean < 1.f ? 0x1p100f : 0x1p-70f;
+    ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      v[e] *= k;
+      ss += v[e] * v[e];
+    }
+    mean = row_sum<LPR>(ss) * PART + eps * k * k;
+  }
+  return 1.0f / sqrtf(mean);
+}
+
 // What a lane holds of a row, and the angles of its token
 template <int D, bool INTERLEAVED> struct RopeLane {
   static constexpr int LPR = D / 16;
