@@ -431,7 +431,7 @@ int64_t qfa_attn_bwd_split_workspace_bytes(int64_t B, int64_t H, int64_t Nq, int
  */
 typedef struct {
   const void *x, *weight;
-  void *y;            /* backward: dx */
+  void *y;            /* backward: dx, nullable where dweight is not */
   const void *dy;     /* backward only */
   void *dweight;      /* backward only, nullable: [D] or [H,D] of w_dtype */
   int64_t H, sx[3], sy[3], sdy[3];
@@ -444,7 +444,7 @@ int qfa_norm_rope(const qfa_norm_rope_tensor *q, const qfa_norm_rope_tensor *k, 
 
 /*
  * Its gradient:  g = rot^T(dy),  dweight = sum over rows of g x r,  dx = r (g w - x r mean(g w x r)),  r = 1 / sqrt(mean(x^2) + eps).
- * dx goes to y.  workspace: qfa_norm_rope_bwd_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant (not needed where no
+ * dx goes to y.  Without a weight x is not looked at (nullable).  workspace: qfa_norm_rope_bwd_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant (not needed where no
  * dweight is asked for); the sums are added up in a fixed order.  weight_per_head as of the tensors: where the two differ, the sum of
  * what either needs alone (Hk 0).
  */

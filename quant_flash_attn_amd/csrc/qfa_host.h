@@ -182,8 +182,8 @@ int64_t cache_workspace_bytes(int64_t B, int64_t H, int64_t Nq, int64_t Nk, int 
 // RMSNorm of every head's row and the position rotation (qfa_norm_rope.hip), after validation.  Strides: batch, head, token.
 struct NormRopeArgs {
   struct Tensor {
-    const void *x, *w;      // w: nullable (no norm)
-    void *y;                // backward: dx
+    const void *x, *w;      // w: nullable (no norm; the backward does not look at x then)
+    void *y;                // backward: dx, nullable
     const void *dy;         // backward only
     void *dw;               // backward, nullable: of w's type
     int64_t H, sx[3], sy[3], sg[3];

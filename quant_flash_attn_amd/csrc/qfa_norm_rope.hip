@@ -1,7 +1,7 @@
 // RMSNorm of every head's row and the position rotation, in one pass, and its gradient:
 //     y = rot(x * r * w),   r = 1 / sqrt(mean(x^2) + eps)
 //     g = rot^T(dy),  dw = sum over rows of g x r,  dx = r (g w - x r mean((g w) x r))
-// Bound by memory: the forward reads and writes each row once, the backward reads x and dy and writes dx; r is computed again
+// Bound by memory: the forward reads and writes each row once, the backward reads x (with a weight) and dy and writes dx; r is computed again
 // from x, which it reads anyway, so the forward keeps nothing.  4 x 64 heads x 4096 x 128 bf16: forward 102 us (5.3 TB/s), gradient
 // 150 us (5.4 TB/s); a copy of that size 5.0.
 //
@@ -17,7 +17,7 @@ namespace qfa {
 
 struct NormRopeTensor {
   const void *x, *dy, *w;
-  void *y;           // forward: y, backward: dx
+  void *y;           // forward: y, backward: dx (nullable)
   float *dw_parts;   // backward: [groups][D], groups as dw_groups counts them
   int64_t H, sxb, sxh, sxn, syb, syh, syn, sgb, sgh, sgn;
   int64_t sw;        // elements between the heads' weights (0: one for all)
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(256) void norm_rope_kernel(NormRopeKernelArgs p) {
         for (int e = 0; e < 16; ++e) v[e] = g[e];
       }
     }
-    if (live) {
+    if (live && (!BACK || a.y)) {
       T *y = static_cast<T *>(a.y) + b * a.syb + h * a.syh + n * a.syn;
       store8<T, ONCE>(y + lane.a, v);
       store8<T, ONCE>(y + lane.b, v + 8);
@@ -187,6 +187,10 @@ template <typename T, int D, bool INTERLEAVED> static int launch_typed(const Nor
     t = {s.x, s.dy, s.w, s.y, nullptr, s.H, s.sx[0], s.sx[1], s.sx[2], s.sy[0], s.sy[1], s.sy[2], s.sg[0], s.sg[1], s.sg[2],
          s.per_head ? (int64_t)D : 0, 1, 1};
     if (s.H <= 0) continue;
+    if (back && !s.w) {   // a rotation's gradient does not need x: dy's lines once more, which the caches have (a branch around the loads
+      t.x = t.dy;         // costs the others 2 %)
+      t.sxb = t.sgb; t.sxh = t.sgh; t.sxn = t.sgn;
+    }
     t.heads_each = heads_each(tokens, s.H, D);
     t.head_groups = (int)((s.H + t.heads_each - 1) / t.heads_each);
     blocks[i] = tb * t.head_groups;

@@ -42,10 +42,11 @@ static int fill_norm_rope(const char *who, bool back, NormRopeArgs *a, const qfa
     const qfa_norm_rope_tensor *s = side[i];
     if (!s) continue;
     if (s->H <= 0) return set_error(QFA_EINVAL, "%s: H must be positive", who);
-    if (!s->x || !s->y || (back && !s->dy)) return set_error(QFA_EINVAL, "%s: null pointer argument", who);
-    if (!aligned16(s->x) || !aligned16(s->y) || (back && !aligned16(s->dy)))
+    const bool in = !back || s->weight, out = !back || s->y || !s->dweight;   // of the backward: x with a weight, dx unless dweight alone is wanted
+    if ((in && !s->x) || (out && !s->y) || (back && !s->dy)) return set_error(QFA_EINVAL, "%s: null pointer argument", who);
+    if ((in && !aligned16(s->x)) || (out && !aligned16(s->y)) || (back && !aligned16(s->dy)))
       return set_error(QFA_EINVAL, "%s: tensors must be 16-byte aligned", who);
-    if (!strides_ok(s->sx[0], s->sx[1], s->sx[2], D, es) || !strides_ok(s->sy[0], s->sy[1], s->sy[2], D, es) ||
+    if ((in && !strides_ok(s->sx[0], s->sx[1], s->sx[2], D, es)) || (out && !strides_ok(s->sy[0], s->sy[1], s->sy[2], D, es)) ||
         (back && !strides_ok(s->sdy[0], s->sdy[1], s->sdy[2], D, es)))
       return set_error(QFA_EINVAL, "%s: strides must be positive multiples of 16 bytes, token stride >= D", who);
     if (int e = check_norm(who, s->weight, w_dtype, dtype, eps)) return e;

@@ -2,6 +2,7 @@
 
 The reference's operators take queries and keys as they come (quant_flash_attn.py:178); a model norms and rotates them first.
 Both entry points are differentiable (a HIP kernel of its own, csrc/qfa_norm_rope.hip; no forward-mode and no second derivative).
+An input is kept for its gradient only where it has a weight; what is rotated alone may change before the gradient is taken.
 As with every torch backward pass, one that is captured into a HIP graph needs that no eager graph of the same leaves is alive then.
 """
 from __future__ import annotations
