@@ -63,6 +63,22 @@ def test_inputs_are_kept_only_where_a_gradient_needs_them(qfa, weights, needs, k
                 assert torch.equal(g, next(a for a, b in zip(grads, wanted) if b is t))
 
 
+@pytest.mark.gpu
+def test_inputs_that_have_to_be_copied(qfa):
+    """Rows with gaps, broadcast batches and gradients: copies that a backward makes of both tensors live until its kernel has them."""
+    q, k, dq, dk, (cos, sin), w = _inputs(4)
+    gaps = lambda t: torch.stack([t, torch.zeros_like(t)], -1).flatten(-2)[..., ::2]   # noqa: E731
+    wide = lambda t: t[:1].expand_as(t)                                            # noqa: E731
+
+    def step(view, dense):
+        leaves = [(view(t).contiguous() if dense else view(t)).requires_grad_(True) for t in (q, k)]
+        out = qfa.norm_rope_pair(*leaves, *w, cos, sin)
+        return [*(o.detach() for o in out), *torch.autograd.grad(out, leaves, [view(d).contiguous() if dense else view(d) for d in (dq, dk)])]
+    for view in (gaps, wide):
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(step(view, False), step(view, True)))
+
+
 def test_pointers_that_the_backward_does_without_need_no_gpu(qfa):
     from quant_flash_attn_amd import _lib
     L, p = _lib.lib(), 0x1000   # never dereferenced: validation fails first
