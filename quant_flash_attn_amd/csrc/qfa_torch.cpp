@@ -138,12 +138,13 @@ template <typename... T> void require_gpu(const Tensor &first, const T &...rest)
 }
 void *stream_of(const Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
-// [B,H,N,D] tensor whose rows are contiguous and whose strides and base are multiples of `align` bytes
+// [B,H,N,D] tensor whose rows are contiguous and whose strides and base are multiples of `align` bytes.  (A copy, not contiguous():
+// that leaves a dense tensor where it is, at any address, and sizes of one with any stride.)
 Tensor rows_aligned(const Tensor &t, int64_t align) {
   const int64_t es = t.element_size();
   bool ok = t.stride(3) == 1 && t.stride(2) >= t.size(3) && reinterpret_cast<uintptr_t>(t.data_ptr()) % align == 0;
   for (int i = 0; i < 3; ++i) ok = ok && t.stride(i) > 0 && (t.stride(i) * es) % align == 0;
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 Tensor rows16(const Tensor &t) { return rows_aligned(t, 16); }
 // the n values of a per-token vector, dense
