@@ -15,7 +15,7 @@ import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
-from . import acc_check
+from . import acc_check, save_check
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -31,6 +31,9 @@ PER_FILE = {f: ["-ffp-contract=off", "-fno-fast-math"] for f in ("qfa_quant.hip"
 # accumulators in AccVGPRs by hand (see qfa_acc.h): other MFMA results in vector registers, and the assembly is checked
 _BWD_PAIR = tuple(f"qfa_bwd_pair_{x}.hip" for x in ("128_bf16", "128_f16", "256_bf16", "256_f16", "64_bf16", "64_f16"))
 BY_HAND = ("qfa_fwd_wide.hip", *_BWD_PAIR, "qfa_skv_pass.hip")
+# kernels with hardly a register to spare, in which the compiler once saved some where lanes were off (see save_check.py): the assembly is checked
+NO_SPARE = ("qfa_norm_rope.hip", "qfa_paged_rows.hip", "qfa_paged_attn.hip", "qfa_paged_tile.hip")
+CHECKS = {**{f: acc_check.check for f in BY_HAND}, **{f: save_check.check for f in NO_SPARE}}
 # MFMA results in vector registers: head_dim 256 with four waves side by side then spills none instead of 5 (dQ) and 1 instead of 4 (forward);
 # elsewhere only the forward of 64 with four waves does, 4 registers, with and without (dKV: no difference in registers)
 PER_FILE["qfa_skv_tile.hip"] = PER_FILE["qfa_skv_dkv.hip"] = PER_FILE["qfa_skv_pass64.hip"] = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
@@ -51,14 +54,14 @@ def _hipcc() -> str:
 def _compile(src: str, extra=()) -> str:
     obj = os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
     cmd = [_hipcc(), *COMMON, *PER_FILE.get(src, []), *extra, "-x", "hip", "-c", os.path.join(CSRC, src), "-o", obj]
-    if src in BY_HAND:
+    if src in CHECKS:
         return _compile_checked(src, cmd, obj)
     _run(src, cmd)
     return obj
 
 
 def assembly_path(src: str) -> str:
-    """The device assembly that the build keeps of a file in BY_HAND."""
+    """The device assembly that the build keeps of a file in CHECKS."""
     return os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".s")
 
 
@@ -68,9 +71,9 @@ def _compile_checked(src: str, cmd, obj: str) -> str:
         _run(src, [*cmd[:-1], made, "--save-temps=obj"])
         asm, = (f for f in os.listdir(tmp) if f.endswith("gfx950.s"))
         os.replace(os.path.join(tmp, asm), assembly_path(src))
-        found = acc_check.check(assembly_path(src))
+        found = CHECKS[src](assembly_path(src))
         if found:
-            raise RuntimeError(f"{src}: the compiler's output breaks the rules of qfa_acc.h:\n" + "\n".join(found))
+            raise RuntimeError(f"{src}: the compiler's output breaks the rules of {CHECKS[src].__module__}:\n" + "\n".join(found))
         os.replace(made, obj)
     return obj
 
