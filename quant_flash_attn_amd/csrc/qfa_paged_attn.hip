@@ -69,12 +69,13 @@ template <typename S, int D, bool SHARED, bool ONE, bool STREAM> __global__ __la
     const int seq = SHARED ? 0 : item.p;   // whose pages
     const int nrows = min(PAGED_ROWS, deal.rows - PAGED_ROWS * item.rb);
 
-    // pages of this wave's tiles: lane 2 i + half of tile i of 32
+    // pages of this wave's tiles: lane 2 i + half of tile i of 32 (a place past the last one is read as the last one, and counts for nothing:
+    // no branch that some lanes take, see qfa_paged_work.h)
     auto pages_from = [&](int i0) __attribute__((always_inline)) -> int {
       const int i = i0 + lane / 2, half = 2 * (t0 + wave + 4 * i) + lane % 2, at = half >> page_halves_log2;
-      int id = -1;
-      if (i < my_tiles && at < a.width) id = a.page_table[seq * a.stb + at * a.stw];
-      return id >= 0 && id < a.pages ? id : -1;
+      const int id = a.page_table[seq * a.stb + min(at, a.width - 1) * a.stw];
+      const bool there = (i < my_tiles) & (at < a.width) & (id >= 0) & (id < a.pages);
+      return there ? id : -1;
     };
     int pg = pages_from(0), pg_next = my_tiles > 32 ? pages_from(32) : -1;
     // (every load is issued whether the tile exists or not -- a missing one has an empty descriptor and fetches nothing)
