@@ -498,6 +498,8 @@ int qfa_paged_read(const qfa_paged_cache *cache, const int32_t *page_table, int6
  *     are many for the sequences and rows: qfa_attn_paged_shared_prefix says whether (prefix, or 0: every sequence's own pages then,
  *     which have to hold them too).
  *   workspace  qfa_attn_paged_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant; one for each call under way.
+ * B H N is below 2^30, and the tiles of keys that the page tables have room for, counted for every block of rows that reads them, below
+ * 2^31 (32 keys for 16 rows, 64 for up to 128).
  * The lengths are read on the device: a captured call follows them.  Keys are dealt to workgroups evenly over the whole batch, so
  * the last bits of a sequence's O depend on the lengths of the others; a call repeated gives the same bits.
  */

@@ -234,6 +234,7 @@ struct PagedAttnArgs {
 };
 int launch_paged_attn(const PagedAttnArgs &a, hipStream_t st);
 int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
+double paged_attn_most_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix, int64_t keys);
 int64_t paged_attn_shared_prefix(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
 
 }  // namespace qfa

@@ -190,10 +190,9 @@ int qfa_attn_paged(const qfa_paged_cache *cache, const void *q, int q_dtype, int
   if (!(sm_scale > 0.f) || isinf(sm_scale)) return set_error(QFA_EINVAL, "%s: sm_scale must be positive and finite", who);
   if (prefix < 0 || prefix > width * cache->page_size)
     return set_error(QFA_EINVAL, "%s: a prefix of %lld keys does not fit the page table", who, (long long)prefix);
-  // rows, and tiles of keys with what is counted for an item's start, are counted in 31 bits
-  const double rows = (double)B * (double)H * (double)N, tiles = ((double)width * cache->page_size / 32 + 13) * (double)B * (double)cache->H *
-                                                               ((double)(H / cache->H) * (double)N / 16 + 1);
-  if (rows * 2 > 2147483647.0 || tiles > 2147483647.0)
+  // rows, and units of work, are counted in 31 bits
+  if ((double)B * (double)H * (double)N > 1073741823.0 ||
+      paged_attn_most_units(B, H, cache->H, N, cache->D, prefix, width * cache->page_size) > 2147483647.0)
     return set_error(QFA_EUNSUPPORTED, "%s: too many rows, or sequences times the keys that a page table has room for, for one call", who);
   const int64_t need = paged_attn_workspace_bytes(B, H, cache->H, N, cache->D, prefix);
   if (!workspace || !aligned16(workspace) || workspace_bytes < need)

@@ -532,6 +532,8 @@ static int block_rows(int64_t rows, int D, int64_t problems) {
   if (rows <= PAGED_ROWS || (rows <= 2 * PAGED_ROWS && (D != 128 || problems <= 128))) return PAGED_ROWS;
   return rows <= 64 ? 64 : 128;
 }
+static int tile_keys(int br) { return br == PAGED_ROWS ? SKV_TILE : PAGED_TILE; }
+static int item_units(int br) { return br == PAGED_ROWS ? 12 : 4; }   // beside its tiles, see qfa_paged_work.h
 static int work_grid(int br, int D) { return br == PAGED_ROWS ? PAGED_WGS : paged_tile_grid(D); }
 // bytes of a launch's slots, and of its whole items
 static int64_t slots_bytes(int br, int D) { return 2LL * work_grid(br, D) * br * (D + 2) * 4; }
@@ -545,6 +547,16 @@ int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, 
   if (prefix > 0) bytes += slots_bytes(shared, D) + 2 * whole_bytes(B * H * N, D);
   if (own > PAGED_ROWS || shared > PAGED_ROWS) bytes += quantized_bytes(B * H * N, D);   // (blocks of 16 quantize their own)
   return bytes;
+}
+
+// Units of work (qfa_paged_work.h) that a launch of the call has at most, if every sequence fills its `keys` keys
+double paged_attn_most_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix, int64_t keys) {
+  const auto most = [&](int64_t problems, int64_t rows, int64_t n) {
+    const int br = block_rows(rows, D, problems);
+    return (double)problems * (double)((rows + br - 1) / br) * ((double)n / tile_keys(br) + 2 + item_units(br));
+  };
+  const double own = most(B * Hk, N * (H / Hk), keys), shared = prefix > 0 ? most(Hk, B * N * (H / Hk), prefix) : 0.0;
+  return own > shared ? own : shared;
 }
 
 // How long a pass over `keys` keys takes for problems * rows rows beside its start, in us: every block of rows reads them again, at the
@@ -589,7 +601,7 @@ template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
   for (int i = 0; i < 2; ++i) {
     const int br = block_rows(problem[i], D, (i == 0 ? x.B : 1) * x.Hk), grid = x.prefix > 0 || i == 0 ? work_grid(br, D) : 0;
     w[i] = {x.starts, x.counts, (int)x.B, (int)x.Hk, G, (int)x.N, x.causal, (int)x.prefix, (int)(x.width << x.page_log2), grid, br,
-            br == PAGED_ROWS ? SKV_TILE : PAGED_TILE, br == PAGED_ROWS ? 12 : 4, nullptr, nullptr, nullptr, nullptr, nullptr};
+            tile_keys(br), item_units(br), nullptr, nullptr, nullptr, nullptr, nullptr};
     if (grid == 0) continue;
     if (i == 0) {
       w[i].first = reinterpret_cast<unsigned *>(mem);
