@@ -427,7 +427,8 @@ int64_t qfa_attn_bwd_split_workspace_bytes(int64_t B, int64_t H, int64_t Nq, int
  *   cos, sin   [rope_rows, rotated / 2] float, dense, 16-byte aligned; rotated a multiple of 16 up to D.  NULL with rotated 0: no rotation
  *   interleaved  pairs (2i, 2i + 1) instead of (i, i + rotated / 2)
  *   positions  nullable; token n of sequence b has position positions[b * spb + n * spn] + step * n (step 0 or 1; without
- *              positions: step * n).  The rotated elements of a token whose position is not in [0, rope_rows) are NaN.
+ *              positions: step * n).  The rotated elements of a token whose position is not in [0, rope_rows) are NaN, and so are its dx
+ *              and what it adds to dweight.
  */
 typedef struct {
   const void *x, *weight;
@@ -496,7 +497,7 @@ int qfa_paged_read(const qfa_paged_cache *cache, const int32_t *page_table, int6
  *     h / (H / cache->H).  o [B,H,N,D] of q_dtype, dense.
  *   prefix  the first `prefix` keys are the same for all sequences: they are read once, from sequence 0's pages.  That pays where they
  *     are many for the sequences and rows: qfa_attn_paged_shared_prefix says whether (prefix, or 0: every sequence's own pages then,
- *     which have to hold them too).
+ *     which have to hold them too).  Sequence 0's pages hold them also where it brings no token.
  *   workspace  qfa_attn_paged_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant; one for each call under way.
  * B H N is below 2^30, and the tiles of keys that the page tables have room for, counted for every block of rows that reads them, below
  * 2^31 (32 keys for 16 rows, 64 for up to 128).

@@ -155,10 +155,10 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_rope_dw_kerne
 }
 
 // Heads that a workgroup walks over: as many as leave the chip 512 workgroups, eight at most.  Forward, gradient and the weights' sums in
-// us, 4 x (32 + 8) heads of 128 in bf16, with 2048 workgroups and with 512: 256 tokens 22 and 20, 512 32 and 27, 1024 46 and 43, 2048
-// 80 and 81; 64 heads of 64 27 and 24, 43 and 38, 67 and 60 from 512 on; 4 x (16 + 4) of 256 in fp32 45 and 42, 80 and 77, 159 and 146;
-// 4 x (32 + 8) of 256 in fp16 47 and 43, 82 and 90, 160 and 157.  (64 heads of 128, 4 x 4096 tokens: eight heads 100 us forward and 162
-// backward, sixteen 115 and 178.)
+// us, of four sequences of 256, 512, 1024 and 2048 tokens, with 2048 workgroups and with 512: 32 + 8 heads of 128 in bf16 25 and 22, 35 and 30,
+// 50 and 43, 85 and 95; 64 + 64 of 64 31 and 26, 46 and 39, 67 and 64, 128 and 126; 16 + 4 of 256 in fp32 31 and 30, 48 and 44, 83 and 81, 150
+// and 152; 32 + 8 of 256 in fp16 37 and 31, 50 and 43, 88 and 89, 157 and 153: 2 to 16 % less up to 512 tokens, and 11 % more at one of the
+// larger ones.  (64 heads of 128, 4 x 4096 tokens: eight heads 100 us forward and 162 backward, sixteen 115 and 178.)
 static int heads_each(int64_t tokens, int64_t H, int D) {
   const int64_t blocks = (tokens + 4096 / D - 1) / (4096 / D) * H;
   int e = 1;

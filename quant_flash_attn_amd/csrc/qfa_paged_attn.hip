@@ -626,8 +626,12 @@ template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
       return e;
     a.q_codes = codes; a.q_scale = scale; a.q_zero = zero;
   }
-  // Non-temporal loads (LOAD_ONCE) where the keys and values that a call may reach outgrow the last-level cache (550 MB, 64 sequences:
-  // 104.9 us with plain loads, 98.5 with these; 67 MB: 17.7 and 18.0, 34 MB behind a prefix 16.2 and 17.8)
+  // Non-temporal loads (LOAD_ONCE) where the keys and values that a call may reach outgrow the last-level cache (256 MiB) for good.  One token
+  // of 64 sequences, 8 key heads of 64, 128 and 256 elements, us with plain loads and with these: 128 MiB 29.1, 27.4, 28.4 and 28.8, 28.1,
+  // 28.3; 256 MiB 49.2, 46.3, 47.4 and 49.7, 48.1, 47.7; 320 MiB 65.4, 61.5, 62.1 and 60.8, 58.1, 57.1; 512 MiB 105, 99, 100 and 93, 88, 87.
+  // The lengths are not known here: short sequences under a table of 4 GiB are read with these too, 16 to 128 MiB of them in the same time
+  // and 256 in 49.0 us in place of 46.7.  Two blocks of rows, which read every key twice, keep plain loads (20 rows, 512 MiB, 64, 128 and 256
+  // elements: 200, 176 and 191 us; with these 180, 182 and 181).
   const bool stream = (double)(x.pages < x.B * x.width ? x.pages : x.B * x.width) * (double)(x.Hk << x.page_log2) * 2 * D >= 320.0 * (1 << 20);
   for (int i = 1; i >= 0; --i) {
     if (w[i].grid == 0) continue;

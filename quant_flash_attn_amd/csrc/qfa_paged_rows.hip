@@ -4,11 +4,12 @@
 // arithmetic and go to the page and row of their position:  page_table[b, p / page], row p % page,  p = starts[b] + n.
 // Read: rows of positions starts[b] .. as the values they stand for, (code - zero point) * scale, rounded once.
 //
-// Both are bound by memory: 2 D bytes (16-bit rows) against D + 3 in the cache; 4 x 32 heads x 4096 x 128: 86 and 72 us (4.7 and
-// 5.6 TB/s).  The work is dealt as in the kernel that norms
-// and rotates (qfa_norm_rope.hip): D/16 lanes hold a row, a workgroup 4096/D tokens, and it walks over some heads of them with
-// their angles and places in registers.  Nothing is written for a token that has no place (see qfa.h): position, page and
-// angle are checked here, since the host does not see them.
+// Both are bound by memory: 2 D bytes (16-bit rows) against D + 3 in the cache; 4 x 32 heads x 4096 x 128: 87 and 74 us (4.6 and
+// 5.5 TB/s).  A call whose sequences bring fewer tokens than it has room for computes the padding too and stores nothing of it (16 x 16
+// heads, up to 517 tokens of 64, half of it padding: 16 us).  The work is dealt as in the kernel that norms and rotates
+// (qfa_norm_rope.hip): D/16 lanes hold a row, a workgroup 4096/D tokens, and it walks over some heads of them with their angles and places
+// in registers.  Nothing is written for a token that has no place (see qfa.h): position, page and angle are checked here, since the
+// host does not see them.
 #include "qfa_quant_row.h"
 #include "qfa_rope_row.h"
 

@@ -1,13 +1,16 @@
 // Attention on a paged INT8 cache for many rows at once: a piece of a prompt, or the queries of all sequences that share a prefix.
 // The same arithmetic as qfa_paged_attn.hip; there 16 rows read a key's codes, here 64 or 128 share them.
 // 2 x 32 heads, 333 rows on 6500 keys of 128: 146 us (480 TFLOP/s); 256 rows of each of 8 heads on 16384 keys 47 us, of which start and
-// end are 10.  Bound by the vector pipe (61 % busy; the matrix pipe 34 %) and what two waves on a SIMD leave idle of it.
+// end are 10.  Of the former the vector pipe is busy for 48 %, the matrix pipe for 22 %, LDS for 30 %, and the waves wait for 36 % of their
+// cycles: two waves on a SIMD, each of them a chain of scores, probabilities and products, fill none of the three.  The expansion of the
+// codes is about 120 of a wave's 315 vector instructions of a tile, the keys' half of it.
 //
 // The four waves together turn a tile of 64 keys and of their values into binary16 integers code - zero_point (exact) in LDS, in
 // the layout of the shared-KV kernels (qfa_skv_tile.h): rows come out of it for the score product, columns (transposing reads) for
 // the P.V product, and nothing has to be corrected afterwards.  The queries are integers of that kind too, so a score is the same
-// exact integer as on INT8 MFMA (255 * 255 * 256 < 2^24): that product would take half the matrix cycles, but its zero-point terms
-// cost four vector instructions more for every score, and the vector pipe is what bounds this kernel.
+// exact integer as on INT8 MFMA (255 * 255 * 256 < 2^24): that product would take half the matrix cycles and leave the keys unexpanded,
+// but its zero-point terms, formed for every score, cost four vector instructions each.  (The dense forward, qfa_fwd.hip, takes them in a
+// correction product; that has not been tried here.)
 //
 // A wave takes 32 rows.  Four waves side by side (128 rows) take both blocks of 32 keys of a tile, two (64 rows) share them with the
 // other two and meet in LDS at the end.  The next tile's codes are on their way in registers while a tile is worked on; pieces of

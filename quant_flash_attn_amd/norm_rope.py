@@ -30,7 +30,8 @@ def norm_rope(x: torch.Tensor, weight: Optional[torch.Tensor], cos: Optional[tor
     cos, sin: fp32 [positions, rotated / 2] (rope_table); None: no rotation.  The first `rotated` elements of a row are turned, a
         multiple of 16 up to D: pairs (i, i + rotated / 2), or (2i, 2i + 1) where interleaved.
     positions: int32 [B,N], or [B] (of every sequence's first token; the others follow), or None (0 to N - 1).  The rotated elements of
-        a token whose position is outside the table are NaN.
+        a token whose position is outside the table are NaN, and with them its row's gradient and the weight's: give padding a position
+        in the table.
     """
     return _lib.host().norm_rope(x, weight, cos, sin, positions, float(eps), bool(interleaved))
 

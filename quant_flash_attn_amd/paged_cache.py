@@ -73,7 +73,8 @@ def quant_flash_attn_paged(q: torch.Tensor, cache, page_table: torch.Tensor, sta
     Token n < counts[b] is at position starts[b] + n and sees the keys up to itself (causal False: all starts[b] + counts[b]); its own
     key has to be in the cache.  Padding tokens, and tokens that see no key, get zeros.
     prefix_len: the first prefix_len positions hold the same rows for all sequences, as a common system prompt (in pages that stand in all
-        their page tables, or in copies).  Where that pays they are read once for all of them, from sequence 0's pages.
+        their page tables, or in copies).  Where that pays they are read once for all of them, from sequence 0's pages: its row of the page table has
+        to hold them also if it brings no token to this call.
     sm_scale: 1 / sqrt(D) if not given.
     The keys are dealt to workgroups evenly over the whole batch: the last bits of a sequence's O depend on the other sequences'
     lengths; the same call gives the same bits.
