@@ -568,8 +568,8 @@ static double pass_us(int64_t problems, int64_t rows, int64_t keys, int D) {
 }
 // Whether a prefix gets a pass of its own.  That one has its start, its queries quantized and results of all rows written and joined
 // again against it: where it saves less, every sequence reads the prefix from its own pages.  Of 240 calls timed both ways (4 to 64
-// sequences, 1 to 300 rows, prefixes of 400, 2000 and 8000 keys, D 64, 128 and 256) 34 get one, which take 0.29 to 0.98 of the time
-// without; of the others 200 take 0.41 to 1.0 of the time with it, six 1.02 to 1.25.
+// sequences, 1 to 300 rows, prefixes of 400, 2000 and 8000 keys, D 64, 128 and 256) 34 get one: 31 of them take 0.33 to 1.0 of the time
+// without and three, of 256 elements, 1.09 to 1.29; of the others 201 take 1.01 to 2.4 of the time with it, five 0.78 to 0.95.
 int64_t paged_attn_shared_prefix(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix) {
   const int64_t rows = N * (H / Hk);
   const double start = block_rows(B * rows, D, Hk) == PAGED_ROWS ? 6.0 + D / 64 : 13.0 + 3.5 * (D / 64);
