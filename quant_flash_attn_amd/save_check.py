@@ -2,7 +2,7 @@
 
 Where a branch that some lanes take joins again, the compiler has saved registers that all lanes need (a thread's own index among
 them) before it turned the other lanes back on; these then read back what the place of the save held before, and stored out of bounds.
-So the build looks at every save -- of a vector register to an accumulation register or to scratch -- and wants it where all lanes are
+So the build looks at every save -- of a vector register to an accumulation register, of either to scratch -- and wants it where all lanes are
 on, on every path, or of a value made under the same mask (the other lanes have none that could be lost).
 
 All lanes are on at a kernel's start (workgroups are whole waves) and wherever exec is set from a scalar register that was written from
@@ -20,7 +20,7 @@ from typing import Dict, FrozenSet, List, Optional, Tuple
 from .acc_check import _kernels
 
 _SGPR = re.compile(r"^s(?:(\d+)|\[(\d+):(\d+)\])$")
-_SAVE = re.compile(r"v_accvgpr_write_b32 a\S+ (v\d+)$|scratch_store_\w+ \S+ (v\d+|v\[\d+:\d+\]),? ?")
+_SAVE = re.compile(r"v_accvgpr_write_b32 a\S+ v\d+$|scratch_store_\w+ \S+ [av]")
 
 # what is known at an instruction: whether all lanes are on, and the scalar halves ("s", n) or spilled ones ("v", n, lane) that hold the
 # low (0) or high (1) half of a mask of all lanes
@@ -87,7 +87,7 @@ def _saved(i) -> Optional[FrozenSet[Tuple[str, int]]]:
     m = _SAVE.match(i.text)
     if i.inline or not m:
         return None
-    return frozenset(r for r in i.reads if r[0] == "v") or None
+    return i.reads or None
 
 
 def check(path: str) -> List[str]:

@@ -16,7 +16,7 @@ def _found(tmp_path, *lines):
     return len(save_check.check(str(path)))
 
 
-@pytest.mark.parametrize("save", [TO_ACC, TO_SCRATCH, "scratch_store_dwordx2 off, v[27:28], off"])
+@pytest.mark.parametrize("save", [TO_ACC, TO_SCRATCH, "scratch_store_dwordx2 off, v[27:28], off", "scratch_store_dword off, a3, off"])
 def test_a_save_where_a_branch_joins(tmp_path, save):
     """As it was found: at the join, in front of the instruction that turns the other lanes on."""
     branch = ["s_and_saveexec_b64 s[2:3], vcc", "s_cbranch_execz .LBB0_2", "v_mov_b32_e32 v1, 0", ".LBB0_2:"]
