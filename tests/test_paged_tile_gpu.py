@@ -146,7 +146,7 @@ def test_prefix_types(qfa, dtype, scale_dtype):
 
 @pytest.mark.gpu
 def test_prefix_pages_that_are_not_there(qfa):
-    """... in the row that the pass reads, sequence 0's: hidden from all of them; in another one's, unless a pass reads that: from it alone."""
+    """A page that is missing in the row that the pass reads, sequence 0's, is hidden from all sequences."""
     prefix, N = 192, 3
     q, cache, table, starts, _, ks, vs, v_scale = _problem(6, 8, 2, N, 128, 32, [prefix + N + 20 * i for i in range(6)], prefix=prefix, seed=2)
     table[0, 1] = -1
