@@ -511,6 +511,92 @@ int qfa_attn_paged(const qfa_paged_cache *cache, const void *q, int q_dtype, int
                    int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, void *o, int64_t B, int64_t H, int64_t N,
                    int64_t prefix, float sm_scale, int causal, void *workspace, int64_t workspace_bytes, void *stream);
 
+/*
+ * qfa_attn_paged, which also hands out the log-sum-exp of every row's scaled scores: lse [B,H,N] float, dense; -infinity for rows that see
+ * no key.  O has the same bits.  workspace: qfa_attn_paged_lse_workspace_bytes(...) bytes.
+ */
+int64_t qfa_attn_paged_lse_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
+
+int qfa_attn_paged_lse(const qfa_paged_cache *cache, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn, const int32_t *page_table,
+                       int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, void *o, float *lse, int64_t B, int64_t H, int64_t N,
+                       int64_t prefix, float sm_scale, int causal, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Bounds of the keys of a cache's pages: of every page and key head a low and a high row (the smallest and the largest value of every
+ * element over the page's rows, as fp32 values scale * (code - zero_point)), each quantized by the arithmetic of qfa_quant_per_token.
+ *   codes [pages,H,2,D] 16-byte aligned, scale [pages,H,2] float (8-byte), zero [pages,H,2] (2-byte), dense; H, D of the cache
+ * qfa_paged_bounds makes those of the pages in which positions starts[b] .. starts[b] + n - 1 lie, n = min(counts[b], N) (counts NULL: N), from
+ * the pages' rows before starts[b] + n.  Called after every qfa_paged_append with its arguments, it keeps all of them up to date.  A
+ * page that is written may stand only once in the call's page table.  No counterpart in the reference.
+ */
+typedef struct {
+  int8_t *codes; float *scale; int8_t *zero;
+} qfa_page_bounds;
+
+int qfa_paged_bounds(const qfa_paged_cache *cache, const qfa_page_bounds *bounds, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw,
+                     const int32_t *starts, const int32_t *counts, int64_t B, int64_t N, void *stream);
+
+/*
+ * The blocks (pages) that a token's attention shall read.  A block's score for a token and key head is the largest over the query heads
+ * that share the key head of
+ *     s (s_high sum_d max(e_d, 0) (c_high,d - z_high) + s_low sum_d min(e_d, 0) (c_low,d - z_low)),
+ * the query quantized per token (e = code - zero point, s its scale): no key of the block has a larger product with the query, but for
+ * the roundings to codes.  Rounded to fp32 once, from 64 bits; what is not a number, or below -FLT_MAX, counts as -FLT_MAX.  Candidates of token n < counts[b] are the blocks
+ * 0 .. (starts[b] + n) / page_size that the page table holds and whose page is in [0, pages).
+ *   blocks  [B,cache->H,N,keep]: the numbers of the `keep` candidates with the largest scores (ties: the lowest number), the `first` first blocks and the
+ *           `last` last ones that the token sees always among them; ascending, -1 behind.  first + last <= keep.
+ *   scores  nullable, [B,cache->H,N,width]: of all candidates, -infinity elsewhere; without it a workspace of
+ *           qfa_paged_select_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant, one for each call under way
+ */
+int64_t qfa_paged_select_workspace_bytes(int64_t B, int64_t Hk, int64_t N, int64_t width);
+
+int qfa_paged_select(const qfa_paged_cache *cache, const qfa_page_bounds *bounds, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn,
+                     const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, int32_t *blocks,
+                     float *scores, int64_t B, int64_t H, int64_t N, int64_t keep, int64_t first, int64_t last, void *workspace, int64_t workspace_bytes,
+                     void *stream);
+
+/*
+ * qfa_attn_paged (causal) on listed blocks: token n of sequence b and the query heads of key head h see the keys j <= starts[b] + n of the blocks
+ * in blocks[b,h,n,:] (int32, dense), in any order; a block that stands there twice counts twice.  Of a list only the first places are looked at, as many as there are
+ * blocks up to the token's own; numbers outside [0, width) and blocks without a page are passed over.  Rows that see no key get zeros.
+ *   workspace  qfa_attn_paged_blocks_workspace_bytes(...) bytes (possibly 0), 16-byte aligned, contents irrelevant; one for each call under way
+ * A call repeated gives the same bits; the last bits of a row depend on B, N, H and keep, not on the other sequences.
+ */
+int64_t qfa_attn_paged_blocks_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t keep, int page_size);
+
+int qfa_attn_paged_blocks(const qfa_paged_cache *cache, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn, const int32_t *page_table,
+                          int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, const int32_t *blocks, int64_t keep, void *o,
+                          int64_t B, int64_t H, int64_t N, float sm_scale, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * The attention weight that every key gets from the rows of a call:
+ *     out[b,h,j] = decay * before[b,h,j] + sum over n < counts[b] and the query heads g of key head h of exp(sm_scale q^_gn . k^_j - lse[b,g,n])
+ * over the rows that see key j, as in qfa_attn_paged (causal or not); lse as qfa_attn_paged_lse hands it out for the same arguments.
+ *   before  nullable (zeros); out: [B,cache->H,width * page_size] float, dense, all of it written; it may be `before` itself
+ *   workspace  qfa_paged_weights_workspace_bytes(...) bytes (possibly 0), 16-byte aligned, contents irrelevant; one for each call under way
+ * Every sum is made in a fixed order, in fp32.  A query row that is not finite leaves its key head's weights not finite.
+ */
+int64_t qfa_paged_weights_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D);
+
+int qfa_paged_weights(const qfa_paged_cache *cache, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn, const float *lse,
+                      const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, const float *before,
+                      float decay, float *out, int64_t B, int64_t H, int64_t N, float sm_scale, int causal, void *workspace, int64_t workspace_bytes,
+                      void *stream);
+
+/*
+ * Eviction: of sequence b's slots 0 .. lengths[b] - 1 every key head keeps min(lengths[b], keep): the `first` first ones and the `last` last ones
+ * always, of the others those with the largest weights (ties: the lowest slot; NaN lies below all numbers).  Their rows, keys and values,
+ * go in order to positions 0, 1, ... of the pages of new_table.  first + last <= keep.
+ *   weights [B,cache->H,width * page_size] float;  new_table as page_table, with room for min(keep, width * page_size) rows; its pages must not
+ *     stand in page_table, nor twice in new_table (the old pages stay as they are, so sequences may share them)
+ *   kept [B,cache->H,keep]: the slots, ascending, -1 behind;  new_weights [B,cache->H,new_width * page_size]: their weights, zeros behind;
+ *   new_lengths [B]: min(lengths[b], keep), at least 0
+ * A row whose old page is none of the cache's becomes zeros; one whose new page is none is not written.
+ */
+int qfa_paged_evict(const qfa_paged_cache *cache, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *lengths,
+                    const float *weights, const int32_t *new_table, int64_t new_width, int64_t ntb, int64_t ntw, int32_t *kept, float *new_weights,
+                    int32_t *new_lengths, int64_t B, int64_t keep, int64_t first, int64_t last, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

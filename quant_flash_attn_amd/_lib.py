@@ -34,6 +34,11 @@ class PagedCacheStruct(ctypes.Structure):
                 ("v_zero", c_void_p), ("pages", c_int64), ("H", c_int64), ("page_size", c_int), ("D", c_int), ("scale_dtype", c_int)]
 
 
+class PageBoundsStruct(ctypes.Structure):
+    """qfa_page_bounds"""
+    _fields_ = [("codes", c_void_p), ("scale", c_void_p), ("zero", c_void_p)]
+
+
 # argument lists mirror include/qfa.h one to one
 _P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
 _SIGNATURES = {
@@ -82,6 +87,16 @@ _SIGNATURES = {
     "qfa_attn_paged_shared_prefix": (c_int64, [_L, _L, _L, _L, _I, _L]),
     "qfa_attn_paged_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _L]),
     "qfa_attn_paged": (c_int, [_P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _L, _L, _L, _L, _F, _I, _P, _L, _P]),
+    "qfa_attn_paged_lse_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _L]),
+    "qfa_attn_paged_lse": (c_int, [_P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _L, _L, _L, _L, _F, _I, _P, _L, _P]),
+    "qfa_paged_bounds": (c_int, [_P, _P, _P, _L, _L, _L, _P, _P, _L, _L, _P]),
+    "qfa_paged_select_workspace_bytes": (c_int64, [_L, _L, _L, _L]),
+    "qfa_paged_select": (c_int, [_P, _P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P] + [_L] * 6 + [_P, _L, _P]),
+    "qfa_attn_paged_blocks_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _L, _I]),
+    "qfa_attn_paged_blocks": (c_int, [_P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _L, _P, _L, _L, _L, _F, _P, _L, _P]),
+    "qfa_paged_weights_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I]),
+    "qfa_paged_weights": (c_int, [_P, _P, _I, _L, _L, _L, _P, _P, _L, _L, _L, _P, _P, _P, _F, _P, _L, _L, _L, _F, _I, _P, _L, _P]),
+    "qfa_paged_evict": (c_int, [_P, _P, _L, _L, _L, _P, _P, _P, _L, _L, _L, _P, _P, _P, _L, _L, _L, _L, _P]),
     "qfa_attn_bwd": (c_int, [_P] * 13 + [_L] + [_P] * 3 + [_I, _L, _L, _L, _L, _I] + [_L] * 24 + [_F, _I, _P]),
 }
 

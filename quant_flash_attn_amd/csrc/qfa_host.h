@@ -231,10 +231,61 @@ struct PagedAttnArgs {
   int64_t sq[3];
   float sm_scale;
   void *workspace;
+  float *lse;               // nullable; dense [B, H, N]
 };
 int launch_paged_attn(const PagedAttnArgs &a, hipStream_t st);
-int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
+int64_t paged_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix, bool lse);
 double paged_attn_most_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix, int64_t keys);
 int64_t paged_attn_shared_prefix(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t prefix);
+
+// The same on lists of blocks, [B, Hk, N, keep] (qfa_paged_list.hip)
+struct PagedListArgs {
+  PagedAttnArgs x;
+  const int32_t *blocks;
+  int64_t keep;
+};
+int launch_paged_list(const PagedListArgs &a, hipStream_t st);
+int64_t paged_list_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t keep, int page_log2);
+double paged_list_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t keep, int page_log2);
+
+// Bounds of the pages' keys, and the blocks that they promise the largest scores of (qfa_paged_select.hip)
+struct PagedSelectArgs {
+  PagedCachePtrs cache;
+  int8_t *codes; float *scale; int8_t *zero;   // the bounds: [pages, Hk, 2, D], [pages, Hk, 2]
+  const int32_t *page_table, *starts, *counts;
+  int64_t pages, Hk, width, stb, stw, B, H, N;
+  int page_log2, scale_dtype, D, q_dtype;
+  const void *q;
+  int64_t sq[3];
+  int32_t *blocks;                             // [B, Hk, N, keep]
+  float *scores;                               // [B, Hk, N, width]
+  int64_t keep, first, last;
+  int all_scores;                              // those of blocks that a token does not see are written too (-inf)
+};
+int launch_paged_bounds(const PagedSelectArgs &a, hipStream_t st);
+int launch_paged_select(const PagedSelectArgs &a, hipStream_t st);
+
+// The attention weight that keys get from the rows of a call (qfa_paged_weigh.hip)
+struct PagedWeighArgs {
+  PagedAttnArgs x;                             // o is not used
+  const float *lse;                            // [B, H, N]
+  const float *before;                         // nullable; [B, Hk, width << page_log2], as out
+  float *out;
+  float decay;
+};
+int launch_paged_weigh(const PagedWeighArgs &a, hipStream_t st);
+int64_t paged_weigh_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D);
+
+// The heaviest rows of every key head to new pages (qfa_paged_evict.hip)
+struct PagedEvictArgs {
+  PagedCachePtrs cache;
+  const int32_t *page_table, *new_table, *lengths;
+  const float *weights;                        // [B, Hk, width << page_log2]
+  int32_t *kept, *new_lengths;                 // [B, Hk, keep], [B]
+  float *new_weights;                          // [B, Hk, new_width << page_log2]
+  int64_t pages, Hk, width, stb, stw, new_width, ntb, ntw, B, keep, first, last;
+  int page_log2, scale_dtype, D;
+};
+int launch_paged_evict(const PagedEvictArgs &a, hipStream_t st);
 
 }  // namespace qfa

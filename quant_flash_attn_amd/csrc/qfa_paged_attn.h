@@ -14,6 +14,8 @@ struct PagedAttnKernelArgs {
   const int8_t *q_codes; const float *q_scale; const int8_t *q_zero;   // the queries quantized, dense (for many rows)
   int width, page_log2, q_dtype;
   float sm_scale_log2;
+  const int32_t *blocks;   // of lists: [B, Hk, N, keep]
+  int keep;
 };
 
 // log2 of the largest p' = p * scale_j at a new reference, and the p' past which the reference moves (see CACHE_P_REF in

@@ -1,0 +1,113 @@
+// The heaviest rows of a paged INT8 cache, per sequence and key head, to new pages: eviction from a cache that has grown too long.
+//
+// Two launches.  A workgroup for each sequence and key head finds the `keep` slots with the largest weights (qfa_topk.h; the first and the last
+// ones always, ties to the lowest slot) and writes down, in order, which they are and their weights.  Then the rows move, codes, scales
+// and zero points of keys and values, each to its place in the new pages: what is kept stays in order, so the last slots are the newest
+// ones again, and pages that other sequences share are not touched.
+#include "qfa_host.h"
+#include "qfa_topk.h"
+
+namespace qfa {
+
+constexpr int EVICT_THREADS = 1024;
+
+__global__ __launch_bounds__(EVICT_THREADS) void evict_select_kernel(PagedEvictArgs x) {
+  __shared__ TopSearch<EVICT_THREADS, 11> top;
+  const int64_t bh = blockIdx.x, b = index_div(bh, x.Hk);
+  const int tid = threadIdx.x;
+  const int64_t slots = x.width << x.page_log2, new_slots = x.new_width << x.page_log2;
+  const int n = (int)max((int64_t)0, min((int64_t)x.lengths[b], slots)), keep = (int)x.keep, k = min(n, keep);
+  const float *weights = x.weights + bh * slots;
+  int32_t *kept = x.kept + bh * keep;
+  float *new_weights = x.new_weights + bh * new_slots;
+  if (bh == b * x.Hk && tid == 0) x.new_lengths[b] = k;
+  if (n > k) {
+    auto key = [&](int i) __attribute__((always_inline)) -> unsigned { return ((i < x.first) | (i >= n - x.last)) ? TOP_ALWAYS : top_key(weights[i]); };
+    unsigned at, equal;
+    top.threshold(n, (unsigned)k, key, at, equal);
+    top.walk(n, at, equal, key, [&](unsigned place, int i) __attribute__((always_inline)) {
+      kept[place] = i;
+      new_weights[place] = weights[i];
+    });
+  } else {
+    for (int i = tid; i < n; i += EVICT_THREADS) {
+      kept[i] = i;
+      new_weights[i] = weights[i];
+    }
+  }
+  for (int64_t i = k + tid; i < keep; i += EVICT_THREADS) kept[i] = -1;
+  for (int64_t i = k + tid; i < new_slots; i += EVICT_THREADS) new_weights[i] = 0.f;
+}
+
+// D/16 lanes hold a row; a workgroup moves some rows of one sequence and key head, of keys or of values
+constexpr int EVICT_UNROLL = 4;
+template <typename S, int D> __global__ __launch_bounds__(256) void evict_move_kernel(PagedEvictArgs x, int chunks) {
+  constexpr int LPR = D / 16, ROWS = 256 / LPR;
+  unsigned id = blockIdx.x;
+  const int chunk = (int)(id % (unsigned)chunks);
+  id /= (unsigned)chunks;
+  const bool values = id & 1;
+  const int64_t bh = id >> 1, b = index_div(bh, x.Hk), h = bh - b * x.Hk;
+  const int tid = threadIdx.x, sub = tid % LPR;
+  const int64_t slots = x.width << x.page_log2;
+  const int k = (int)max((int64_t)0, min(min((int64_t)x.lengths[b], slots), x.keep));
+  int8_t *codes = values ? x.cache.v_codes : x.cache.k_codes, *zero = values ? x.cache.v_zero : x.cache.k_zero;
+  S *scale = static_cast<S *>(values ? x.cache.v_scale : x.cache.k_scale);
+  const int row_mask = (1 << x.page_log2) - 1;
+  int64_t from[EVICT_UNROLL], to[EVICT_UNROLL];
+#pragma unroll
+  for (int u = 0; u < EVICT_UNROLL; ++u) {
+    const int i = (chunk * EVICT_UNROLL + u) * ROWS + tid / LPR;
+    from[u] = to[u] = -1;
+    if (i >= k) continue;
+    const int slot = x.kept[bh * x.keep + i];
+    const int page = x.page_table[b * x.stb + (int64_t)(slot >> x.page_log2) * x.stw];
+    const int new_page = x.new_table[b * x.ntb + (int64_t)(i >> x.page_log2) * x.ntw];
+    if (page >= 0 && page < x.pages) from[u] = (((int64_t)page * x.Hk + h) << x.page_log2) + (slot & row_mask);
+    if (new_page >= 0 && new_page < x.pages) to[u] = (((int64_t)new_page * x.Hk + h) << x.page_log2) + (i & row_mask);
+  }
+  u32x4 w[EVICT_UNROLL];
+  S s[EVICT_UNROLL];
+  int8_t z[EVICT_UNROLL];
+#pragma unroll
+  for (int u = 0; u < EVICT_UNROLL; ++u) {   // (a row without a page becomes zeros)
+    w[u] = u32x4{0, 0, 0, 0};
+    s[u] = (S)0.f;
+    z[u] = 0;
+    if (from[u] < 0 || to[u] < 0) continue;
+    w[u] = *reinterpret_cast<const u32x4 *>(codes + from[u] * D + 16 * sub);
+    if (sub == 0) {
+      s[u] = scale[from[u]];
+      z[u] = zero[from[u]];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < EVICT_UNROLL; ++u) {
+    if (to[u] < 0) continue;
+    *reinterpret_cast<u32x4 *>(codes + to[u] * D + 16 * sub) = w[u];
+    if (sub == 0) {
+      scale[to[u]] = s[u];
+      zero[to[u]] = z[u];
+    }
+  }
+}
+
+template <typename S> static int launch_move(const PagedEvictArgs &x, int64_t chunks, hipStream_t st) {
+  const dim3 grid((unsigned)(x.B * x.Hk * 2 * chunks)), block(256);
+  if (x.D == 64) evict_move_kernel<S, 64><<<grid, block, 0, st>>>(x, (int)chunks);
+  else if (x.D == 128) evict_move_kernel<S, 128><<<grid, block, 0, st>>>(x, (int)chunks);
+  else evict_move_kernel<S, 256><<<grid, block, 0, st>>>(x, (int)chunks);
+  return check_launch("qfa_paged_evict (rows)");
+}
+int launch_paged_evict(const PagedEvictArgs &x, hipStream_t st) {
+  const int64_t most = x.keep < x.width << x.page_log2 ? x.keep : x.width << x.page_log2, rows = EVICT_UNROLL * 4096 / x.D;
+  const int64_t chunks = (most + rows - 1) / rows;
+  if ((double)x.B * (double)x.Hk * 2 * (double)chunks > 2147483647.0) return set_error(QFA_EUNSUPPORTED, "paged_evict: too many rows for one launch");
+  evict_select_kernel<<<dim3((unsigned)(x.B * x.Hk)), dim3(EVICT_THREADS), 0, st>>>(x);
+  if (int e = check_launch("qfa_paged_evict")) return e;
+  if (x.scale_dtype == QFA_F32) return launch_move<float>(x, chunks, st);
+  if (x.scale_dtype == QFA_F16) return launch_move<_Float16>(x, chunks, st);
+  return launch_move<__bf16>(x, chunks, st);
+}
+
+}  // namespace qfa

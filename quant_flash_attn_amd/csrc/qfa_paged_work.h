@@ -36,6 +36,7 @@ struct PagedWork {
   unsigned *first;                  // [items] the unit of an item's first tile, [items] that one's units per workgroup (own keys)
   float *slots, *slots_ml;          // [2 * grid][br][D] and (m in log2 units, l): of a piece that does not begin its item, one that does
   float *whole, *whole_ml;          // nullable: items in one piece, [problem, head, row] (null: they are normalised and stored)
+  unsigned list_tiles, list_each;   // of lists: tiles of an item, units of a workgroup
 };
 
 // A sequence's position of its first new token, and how many it brings
@@ -54,6 +55,7 @@ __device__ __forceinline__ unsigned wave_scan(unsigned x) {
 
 // ONE: a problem has a single block of rows
 template <bool SHARED, bool ONE> struct PagedDeal {
+  static constexpr bool ONE_PROBLEM = SHARED, LIST = false;
   const PagedWork &a;
   const int BR, TK;                 // work.br and work.tk, constants in the kernels that are made for them
   int rows, blocks, problems;       // rows and blocks of rows of a problem
@@ -206,6 +208,65 @@ template <bool SHARED, bool ONE> struct PagedDeal {
   __device__ __forceinline__ int last_key(const Row &r, const PagedSeq &s) const {
     const int64_t k = (int64_t)s.start + (a.causal ? r.i : s.tokens - 1);
     return (int)max((int64_t)-1, min(k, (int64_t)(SHARED ? a.prefix : a.capacity) - 1));
+  }
+};
+
+// Lists of blocks: a problem is a token, its rows the query heads that share a key head, and its keys the blocks of its list, which are as many
+// for all tokens.  So every item has the same number of units, the host divides them, and nothing has to be noted for the kernel that joins
+// the pieces.
+struct PagedListDeal {
+  static constexpr bool ONE_PROBLEM = false, LIST = true;
+  const PagedWork &a;
+  const int BR;
+  int rows, blocks;
+  unsigned total, each, per_item;
+  typedef PagedDeal<false, false> Keys;
+  typedef Keys::Row Row;
+  struct Item { int p, h, rb; unsigned at, tiles, first; PagedSeq s; };
+  __device__ __forceinline__ PagedListDeal(const PagedWork &a_, int br, int) : a(a_), BR(br) {
+    rows = a.G;
+    blocks = (rows + BR - 1) / BR;
+    per_item = a.list_tiles + (unsigned)a.extra;
+    each = a.list_each;
+    total = (unsigned)(a.B * a.N * a.Hk * blocks) * per_item;
+  }
+  __device__ __forceinline__ PagedSeq seq(int p) const {
+    const int b = p / a.N, n = a.counts ? max(0, min(a.counts[b], a.N)) : a.N;
+    return {__builtin_amdgcn_readfirstlane(a.starts[b]), __builtin_amdgcn_readfirstlane(n)};
+  }
+  // The item of that number: row blocks of a head, heads of a token, tokens
+  __device__ __forceinline__ void item(unsigned n, Item &it) const {
+    const unsigned bh = n / (unsigned)blocks;
+    it.rb = (int)(n - bh * (unsigned)blocks);
+    it.p = (int)(bh / (unsigned)a.Hk);
+    it.h = (int)(bh - (unsigned)it.p * (unsigned)a.Hk);
+    it.tiles = a.list_tiles;
+    it.first = n * per_item + (unsigned)a.extra;
+    it.at = 0;
+    it.s = seq(it.p);
+  }
+  __device__ __forceinline__ bool find(unsigned &x, Item &it) const {
+    x = blockIdx.x * each;
+    if (x >= total) return false;
+    item(x / per_item, it);
+    x = max(x, it.first);
+    it.at = x - it.first;
+    return x < total;
+  }
+  __device__ __forceinline__ bool next(unsigned &x, unsigned x_end, Item &it) const {
+    x += (unsigned)a.extra;
+    if (x >= x_end) return false;
+    item(x / per_item, it);
+    return true;
+  }
+  __device__ __forceinline__ int begin() const { return 0; }
+  __device__ __forceinline__ Row row(int p, int h, int r) const {
+    const int b = p / a.N;
+    return {b, p - b * a.N, h * a.G + r};
+  }
+  __device__ __forceinline__ int last_key(const Row &r, const PagedSeq &s) const {
+    const int64_t k = (int64_t)s.start + r.i;
+    return r.i >= s.tokens ? -1 : (int)max((int64_t)-1, min(k, (int64_t)a.capacity - 1));
   }
 };
 

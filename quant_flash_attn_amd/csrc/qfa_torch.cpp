@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 #include <ATen/DeviceGuard.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
@@ -64,6 +65,16 @@ struct Api {
   QFA_ENTRY(qfa_attn_paged_shared_prefix);
   QFA_ENTRY(qfa_attn_paged_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged);
+  QFA_ENTRY(qfa_attn_paged_lse_workspace_bytes);
+  QFA_ENTRY(qfa_attn_paged_lse);
+  QFA_ENTRY(qfa_paged_bounds);
+  QFA_ENTRY(qfa_paged_select);
+  QFA_ENTRY(qfa_paged_select_workspace_bytes);
+  QFA_ENTRY(qfa_attn_paged_blocks_workspace_bytes);
+  QFA_ENTRY(qfa_attn_paged_blocks);
+  QFA_ENTRY(qfa_paged_weights_workspace_bytes);
+  QFA_ENTRY(qfa_paged_weights);
+  QFA_ENTRY(qfa_paged_evict);
 #undef QFA_ENTRY
 };
 Api api;
@@ -108,6 +119,16 @@ void init(const py::dict &address) {
   QFA_ENTRY(qfa_attn_paged_shared_prefix);
   QFA_ENTRY(qfa_attn_paged_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged);
+  QFA_ENTRY(qfa_attn_paged_lse_workspace_bytes);
+  QFA_ENTRY(qfa_attn_paged_lse);
+  QFA_ENTRY(qfa_paged_bounds);
+  QFA_ENTRY(qfa_paged_select);
+  QFA_ENTRY(qfa_paged_select_workspace_bytes);
+  QFA_ENTRY(qfa_attn_paged_blocks_workspace_bytes);
+  QFA_ENTRY(qfa_attn_paged_blocks);
+  QFA_ENTRY(qfa_paged_weights_workspace_bytes);
+  QFA_ENTRY(qfa_paged_weights);
+  QFA_ENTRY(qfa_paged_evict);
 #undef QFA_ENTRY
 }
 
@@ -906,6 +927,7 @@ Tensor shared(const Tensor &q, const Tensor &kv_fp16, const Tensor &codes, const
 }
 
 #include "qfa_torch_paged.inc"
+#include "qfa_torch_long.inc"
 
 }  // namespace
 
@@ -921,6 +943,10 @@ TORCH_LIBRARY(quant_flash_attn_amd, m) {
         "bool interleaved) -> (Tensor, Tensor)", &norm_rope_pair_op);
   m.def("paged(Tensor q, Tensor k_codes, Tensor k_scale, Tensor k_zero_point, Tensor v_codes, Tensor v_scale, Tensor v_zero_point, "
         "Tensor page_table, Tensor starts, Tensor? counts, bool causal, float sm_scale, int prefix_len) -> Tensor", &paged_attn_op);
+  m.def("paged_lse(Tensor q, Tensor k_codes, Tensor k_scale, Tensor k_zero_point, Tensor v_codes, Tensor v_scale, Tensor v_zero_point, "
+        "Tensor page_table, Tensor starts, Tensor? counts, bool causal, float sm_scale, int prefix_len) -> (Tensor, Tensor)", &paged_attn_lse_op);
+  m.def("paged_blocks(Tensor q, Tensor k_codes, Tensor k_scale, Tensor k_zero_point, Tensor v_codes, Tensor v_scale, Tensor v_zero_point, "
+        "Tensor page_table, Tensor starts, Tensor blocks, Tensor? counts, float sm_scale) -> Tensor", &paged_blocks_op);
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -948,4 +974,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_append", &paged_append, nogil());
   m.def("paged_read", &paged_read, nogil());
   m.def("paged_attn", &paged_attn, nogil());
+  m.def("paged_attn_lse", &paged_attn_lse, nogil());
+  m.def("paged_bounds", &paged_bounds, nogil());
+  m.def("paged_select", &paged_select, nogil());
+  m.def("paged_blocks", &paged_blocks, nogil());
+  m.def("paged_weights", &paged_weights, nogil());
+  m.def("paged_evict", &paged_evict, nogil());
 }

@@ -14,7 +14,7 @@ call's N tokens a sequence brings (the others are padding behind them).
 from __future__ import annotations
 
 import math
-from typing import NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 
@@ -65,7 +65,7 @@ def paged_cache_read(cache, page_table: torch.Tensor, starts: torch.Tensor, N: i
 
 def quant_flash_attn_paged(q: torch.Tensor, cache, page_table: torch.Tensor, starts: torch.Tensor,
                            counts: Optional[torch.Tensor] = None, causal: bool = True, sm_scale: Optional[float] = None,
-                           prefix_len: int = 0) -> torch.Tensor:
+                           prefix_len: int = 0, return_lse: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """Attention of the tokens at the end of every sequence, q [B,H,N,D], on its pages; H a multiple of the cache's heads (query head h
     reads key head h // (H // heads)).  O [B,H,N,D] of q's type.  The arithmetic is quant_flash_attn_quantized_kv's for short query
     blocks: queries quantized per token inside, INT8 scores, V as its exact codes.  No gradient.
@@ -76,8 +76,10 @@ def quant_flash_attn_paged(q: torch.Tensor, cache, page_table: torch.Tensor, sta
         their page tables, or in copies).  Where that pays they are read once for all of them, from sequence 0's pages: its row of the page table has
         to hold them also if it brings no token to this call.
     sm_scale: 1 / sqrt(D) if not given.
+    return_lse: also the log-sum-exp of every row's scaled scores, fp32 [B,H,N] (-inf where a row sees no key); O has the same bits.
     The keys are dealt to workgroups evenly over the whole batch: the last bits of a sequence's O depend on the other sequences'
     lengths; the same call gives the same bits.
     """
     sm = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
-    return _lib.host().paged_attn(q, tuple(cache), page_table, starts, counts, bool(causal), sm, int(prefix_len))
+    call = _lib.host().paged_attn_lse if return_lse else _lib.host().paged_attn
+    return call(q, tuple(cache), page_table, starts, counts, bool(causal), sm, int(prefix_len))
