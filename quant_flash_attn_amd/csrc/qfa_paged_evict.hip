@@ -9,10 +9,9 @@
 
 namespace qfa {
 
-constexpr int EVICT_THREADS = 1024;
-
-__global__ __launch_bounds__(EVICT_THREADS) void evict_select_kernel(PagedEvictArgs x) {
-  __shared__ TopSearch<EVICT_THREADS, 11> top;
+// Top: TopHeld, of T threads
+template <typename Top, int T> __global__ __launch_bounds__(T) void evict_select_kernel(PagedEvictArgs x) {
+  __shared__ Top top;
   const int64_t bh = blockIdx.x, b = index_div(bh, x.Hk);
   const int tid = threadIdx.x;
   const int64_t slots = x.width << x.page_log2, new_slots = x.new_width << x.page_log2;
@@ -22,21 +21,21 @@ __global__ __launch_bounds__(EVICT_THREADS) void evict_select_kernel(PagedEvictA
   float *new_weights = x.new_weights + bh * new_slots;
   if (bh == b * x.Hk && tid == 0) x.new_lengths[b] = k;
   if (n > k) {
-    auto key = [&](int i) __attribute__((always_inline)) -> unsigned { return ((i < x.first) | (i >= n - x.last)) ? TOP_ALWAYS : top_key(weights[i]); };
-    unsigned at, equal;
-    top.threshold(n, (unsigned)k, key, at, equal);
-    top.walk(n, at, equal, key, [&](unsigned place, int i) __attribute__((always_inline)) {
-      kept[place] = i;
-      new_weights[place] = weights[i];
-    });
+    const int first = (int)x.first, last = n - (int)x.last;
+    top.run(n, (unsigned)k, [&](int i) __attribute__((always_inline)) { return weights[i]; },
+            [&](int i, float w) __attribute__((always_inline)) -> unsigned { return ((i < first) | (i >= last)) ? TOP_ALWAYS : top_key(w); },
+            [&](unsigned place, int i, float w) __attribute__((always_inline)) {
+              kept[place] = i;
+              new_weights[place] = w;
+            });
   } else {
-    for (int i = tid; i < n; i += EVICT_THREADS) {
+    for (int i = tid; i < n; i += T) {
       kept[i] = i;
       new_weights[i] = weights[i];
     }
   }
-  for (int64_t i = k + tid; i < keep; i += EVICT_THREADS) kept[i] = -1;
-  for (int64_t i = k + tid; i < new_slots; i += EVICT_THREADS) new_weights[i] = 0.f;
+  for (int64_t i = k + tid; i < keep; i += T) kept[i] = -1;
+  for (int64_t i = k + tid; i < new_slots; i += T) new_weights[i] = 0.f;
 }
 
 // D/16 lanes hold a row; a workgroup moves some rows of one sequence and key head, of keys or of values
@@ -99,11 +98,18 @@ template <typename S> static int launch_move(const PagedEvictArgs &x, int64_t ch
   else evict_move_kernel<S, 256><<<grid, block, 0, st>>>(x, (int)chunks);
   return check_launch("qfa_paged_evict (rows)");
 }
+template <typename Top, int T> static void launch_top(const PagedEvictArgs &x, hipStream_t st) {
+  evict_select_kernel<Top, T><<<dim3((unsigned)(x.B * x.Hk)), dim3(T), 0, st>>>(x);
+}
 int launch_paged_evict(const PagedEvictArgs &x, hipStream_t st) {
   const int64_t most = x.keep < x.width << x.page_log2 ? x.keep : x.width << x.page_log2, rows = EVICT_UNROLL * 4096 / x.D;
   const int64_t chunks = (most + rows - 1) / rows;
   if ((double)x.B * (double)x.Hk * 2 * (double)chunks > 2147483647.0) return set_error(QFA_EUNSUPPORTED, "paged_evict: too many rows for one launch");
-  evict_select_kernel<<<dim3((unsigned)(x.B * x.Hk)), dim3(EVICT_THREADS), 0, st>>>(x);
+  const int64_t slots = x.width << x.page_log2;
+  // more sequences and heads than CUs share one: 512 x 3000 slots 10.9 us with 512 threads and with 1024, 8 x 5120 9.7 and 8.1
+  if (slots <= 4096 && x.B * x.Hk > 256) launch_top<TopHeld<512, 4096, 11>, 512>(x, st);
+  else if (slots <= 16384) launch_top<TopHeld<1024, 16384, 11>, 1024>(x, st);
+  else launch_top<TopHeld<1024, 0, 11>, 1024>(x, st);
   if (int e = check_launch("qfa_paged_evict")) return e;
   if (x.scale_dtype == QFA_F32) return launch_move<float>(x, chunks, st);
   if (x.scale_dtype == QFA_F16) return launch_move<_Float16>(x, chunks, st);

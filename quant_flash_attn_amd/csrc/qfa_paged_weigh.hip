@@ -6,7 +6,8 @@
 // One pass over the keys (D + 3 bytes of each), no exchange between workgroups and no atomics: a wave holds 64 keys, all rows pass by, and a
 // key's sum is made in a fixed order.  Rows are the rows of the product and keys its columns, so a key's scale and zero point are one value
 // per lane and its sum is three lane exchanges for 64 keys.  Up to 16 rows are quantized in the workgroup and stay in registers while it
-// takes several times 256 keys; more are quantized once by a launch in front and pass through LDS 64 at a time.
+// takes several times 256 keys; more are quantized once by a launch in front, and pass through LDS in panels of 64, the next one on its way while
+// one is worked on.
 #include "qfa_host.h"
 #include "qfa_quant_row.h"
 #include "qfa_skv_common.h"
@@ -17,42 +18,118 @@ struct WeighKernelArgs {
   PagedWeighArgs w;
   int G, steps, chunks, rows;
   float sm_scale_log2;
-  const int8_t *q_codes; const float *q_scale; const int8_t *q_zero; const int32_t *q_sum;   // many rows: quantized, dense
+  const unsigned char *panels;   // many rows: those of every sequence and key head, ready to be copied to LDS
+  int panels_each;
 };
 
-template <int D, int PR> struct WeighPanel {
+template <int D, int PR> struct __attribute__((aligned(16))) WeighPanel {
   static constexpr int CPR = D / 16;
   unsigned char codes[PR * D];   // rows, their chunks of 16 bytes moved by the row: 16 rows at one chunk lie in different banks
   float a[PR], lse[PR];          // scale * sm_scale * log2(e); the log-sum-exp in log2 units (infinite: the row counts for nothing)
-  int zero[PR], c[PR], last[PR]; // zero point; code sum - D * zero point; the last key that the row sees
+  int zero[PR], c[PR], last[PR]; // - zero point; D * zero point - code sum; the last key that the row sees
   static __device__ __forceinline__ int chunk(int row, int c) { return row * D + ((c ^ (row % CPR)) << 4); }
+  // the constants of a row, token i's of `tokens`
+  __device__ __forceinline__ void constants(int at, bool there, float scale, int z, int sum, float row_lse, int row_last) {
+    a[at] = there ? (scale < 0x1p-126f ? 0x1p-126f : scale) : 0.f;
+    lse[at] = there ? row_lse * kLog2e : INFINITY;
+    zero[at] = -z;
+    c[at] = D * z - sum;
+    last[at] = row_last;
+  }
 };
 
-template <typename S, int D, bool ONE> __global__ __launch_bounds__(256) void paged_weigh_kernel(WeighKernelArgs p) {
-  constexpr int KM = D / 64, PR = ONE ? 16 : 64;
+// A sequence's tokens and the last keys that they see
+struct WeighSeq {
+  int start, tokens, slots, last;   // last: of any row
+  __device__ __forceinline__ WeighSeq(const PagedAttnArgs &x, int64_t b) {
+    start = x.starts[b];
+    tokens = (int)(x.counts ? max((int64_t)0, min((int64_t)x.counts[b], x.N)) : x.N);
+    slots = (int)(x.width << x.page_log2);
+    last = tokens == 0 ? -1 : (int)max((int64_t)-1, min((int64_t)start + tokens - 1, (int64_t)slots - 1));
+  }
+  __device__ __forceinline__ int last_of(const PagedAttnArgs &x, int i) const {   // token i's
+    return x.causal ? (int)max((int64_t)-1, min((int64_t)start + i, (int64_t)slots - 1)) : last;
+  }
+};
+
+// 16 rows of a sequence and key head (row = token * G + head), quantized into a panel at r0 % PR: D/8 lanes hold a row.  A row that is not there, or is
+// padding, counts for nothing
+template <int D> struct WeighRows {
+  static constexpr int LPT = D / 8, TPP = 256 / LPT, PASSES = (16 + TPP - 1) / TPP;
+  float v[PASSES][8], lse[PASSES];
+  __device__ __forceinline__ void load(const WeighKernelArgs &p, int64_t b, int64_t h, int r0) {
+    const PagedAttnArgs &x = p.w.x;
+#pragma unroll
+    for (int ps = 0; ps < PASSES; ++ps) {
+      const int row = ps * TPP + threadIdx.x / LPT, sub = threadIdx.x % LPT, r = min(r0 + row, p.rows - 1), i = r / p.G;
+      const int64_t head = h * p.G + r - i * p.G, off = b * x.sq[0] + head * x.sq[1] + i * x.sq[2] + sub * 8;
+      lse[ps] = p.w.lse[(b * x.H + head) * x.N + i];
+      if (x.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(x.q) + off, v[ps]);
+      else if (x.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(x.q) + off, v[ps]);
+      else Load8<_Float16>::run(static_cast<const _Float16 *>(x.q) + off, v[ps]);
+    }
+  }
+  template <typename Panel> __device__ __forceinline__ void put(const WeighKernelArgs &p, const WeighSeq &seq, Panel &panel, int r0) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+#pragma unroll
+    for (int ps = 0; ps < PASSES; ++ps) {
+      const int row = ps * TPP + threadIdx.x / LPT, sub = threadIdx.x % LPT, r = r0 + row;
+      if (r0 + ps * TPP + wave * (64 / LPT) >= p.rows) break;   // (uniform over the wave)
+      const QuantRow<8> q = quant_row<LPT, false, 8>(v[ps], true);
+      if (row < 16 && r < p.rows) {
+        const int at = r % (int)(sizeof(panel.a) / 4), i = r / p.G;
+        *reinterpret_cast<u32x2 *>(panel.codes + Panel::chunk(at, sub / 2) + 8 * (sub % 2)) = u32x2{q.codes[0], q.codes[1]};
+        const bool there = i < seq.tokens;
+        if (sub == 0) panel.constants(at, there, q.scale * p.sm_scale_log2, (int)q.zp, q.sum, lse[ps], there ? seq.last_of(p.w.x, i) : seq.last);
+      }
+    }
+    const int r = r0 + threadIdx.x;   // (the codes behind hold anything)
+    if (threadIdx.x < 16 && r >= p.rows) panel.constants(r % (int)(sizeof(panel.a) / 4), false, 0.f, 0, 0, 0.f, seq.last);
+  }
+};
+
+constexpr int WEIGH_PANEL = 64;
+// Many rows: the panels of every sequence and key head, 16 rows of one a workgroup
+template <int D> __global__ __launch_bounds__(256) void weigh_rows_kernel(WeighKernelArgs p) {
+  typedef WeighPanel<D, WEIGH_PANEL> Panel;
+  const int per = p.panels_each * (WEIGH_PANEL / 16);
+  const int64_t bh = index_div(blockIdx.x, per), b = index_div(bh, p.w.x.Hk), h = bh - b * p.w.x.Hk;
+  const int r0 = 16 * (int)(blockIdx.x - bh * per);
+  const WeighSeq seq(p.w.x, b);
+  WeighRows<D> rows;
+  rows.load(p, b, h, r0);
+  rows.put(p, seq, reinterpret_cast<Panel *>(const_cast<unsigned char *>(p.panels))[bh * p.panels_each + r0 / WEIGH_PANEL], r0);
+}
+
+template <typename S, int D, bool ONE> __global__ __launch_bounds__(256, D == 256 ? 2 : ONE ? 5 : 4) void paged_weigh_kernel(WeighKernelArgs p) {
+  constexpr int KM = D / 64, PR = ONE ? 16 : WEIGH_PANEL;
   typedef WeighPanel<D, PR> Panel;
-  __shared__ __attribute__((aligned(16))) Panel panel;
+  // many rows: two panels, each with room for whole copies of 1024 bytes
+  constexpr int PIECES = (sizeof(Panel) + 1023) / 1024, BUF = ONE ? sizeof(Panel) : 1024 * PIECES;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[ONE ? BUF : 2 * BUF];
   const PagedAttnArgs &x = p.w.x;
   const int tid = threadIdx.x, lane = tid % 64, c16 = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
-  const int64_t bh = index_div(blockIdx.x, p.chunks), chunk = blockIdx.x - bh * p.chunks, b = index_div(bh, x.Hk), h = bh - b * x.Hk;
-  const int start = x.starts[b], tokens = (int)(x.counts ? max((int64_t)0, min((int64_t)x.counts[b], x.N)) : x.N);
-  const int slots = (int)(x.width << x.page_log2);
-  // the last key that any row sees
-  const int last = tokens == 0 ? -1 : (int)max((int64_t)-1, min((int64_t)start + tokens - 1, (int64_t)slots - 1));
+  // (sequences before chunks of keys: not every sequence has keys in the later ones)
+  const unsigned unit = blockIdx.x / (unsigned)x.Hk;
+  const int64_t chunk = unit / (unsigned)x.B, b = unit - (unsigned)chunk * (unsigned)x.B, h = blockIdx.x % (unsigned)x.Hk, bh = b * x.Hk + h;
+  const WeighSeq seq(x, b);
+  const int slots = seq.slots, last = seq.last;
   const float *before = p.w.before ? p.w.before + bh * slots : nullptr;
   float *out = p.w.out + bh * slots;
   const int begin = (int)chunk * 256 * p.steps;
-  if (begin > last && before == out && p.w.decay == 1.0f) return;
-  auto last_of = [&](int i) __attribute__((always_inline)) -> int {   // token i's
-    return x.causal ? (int)max((int64_t)-1, min((int64_t)start + i, (int64_t)slots - 1)) : last;
-  };
-  const bool work = begin <= last;   // (uniform)
+  if (begin > last) {   // slots behind the last key, all loads at once (step by step these workgroups would keep the others from the CUs for several waits)
+    const int end = min(slots, begin + 256 * p.steps);
+    if (before == out && p.w.decay == 1.0f) return;
+#pragma unroll 4
+    for (int i = begin + tid; i < end; i += 256) out[i] = before ? p.w.decay * before[i] : 0.f;
+    return;
+  }
   const i32x4 ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
   i32x4 qf[KM];
   float a[4], lse[4];
-  int zq[4], cq[4], lim[4], least = 0;
-  auto rows_from = [&](int r0) __attribute__((always_inline)) {   // 16 rows out of the panel
+  int zq[4], cq[4], lim[4];
+  auto rows_from = [&](const Panel &panel, int r0) __attribute__((always_inline)) {   // 16 rows out of the panel
 #pragma unroll
     for (int m = 0; m < KM; ++m) qf[m] = *reinterpret_cast<const i32x4 *>(panel.codes + Panel::chunk(r0 + c16, 4 * m + g));
     const f32x4 av = *reinterpret_cast<const f32x4 *>(panel.a + r0 + 4 * g), lv = *reinterpret_cast<const f32x4 *>(panel.lse + r0 + 4 * g);
@@ -66,80 +143,84 @@ template <typename S, int D, bool ONE> __global__ __launch_bounds__(256) void pa
       cq[v] = cv[v];
       lim[v] = kv[v];
     }
-    least = min(min(lim[0], lim[1]), min(lim[2], lim[3]));
-    least = min(least, __shfl_xor(least, 16, 64));
-    least = __builtin_amdgcn_readfirstlane(min(least, __shfl_xor(least, 32, 64)));
   };
-  // constants of row r (of the call's sequence and key head), for lane 0 of those that hold it
-  auto constants = [&](int at, int r, float scale, int zero, int sum) __attribute__((always_inline)) {
-    const int i = min(r, p.rows - 1) / p.G;
-    const int64_t row = (b * x.H + h * p.G + min(r, p.rows - 1) - i * p.G) * x.N + i;
-    const float f = scale * p.sm_scale_log2;
-    const bool there = r < p.rows && i < tokens;
-    panel.a[at] = there ? (f < 0x1p-126f ? 0x1p-126f : f) : 0.f;
-    panel.lse[at] = there ? p.w.lse[row] * kLog2e : INFINITY;
-    panel.zero[at] = zero;
-    panel.c[at] = sum - D * zero;
-    panel.last[at] = there ? last_of(i) : last;
+  // 64 keys of a step: the page of each, a key's constants in its lane, the codes of four tiles of 16
+  struct Keys {
+    i32x4 k[4][KM];
+    float scale;
+    int zero, there;   // there: bit per tile, its page exists
   };
-  if (ONE && work) {
-    constexpr int LPT = D / 8, TPP = 256 / LPT, PASSES = (16 + TPP - 1) / TPP;
+  const S *scales = static_cast<const S *>(x.cache.k_scale);
+  auto page_of = [&](int key) __attribute__((always_inline)) -> int {
+    const int at = key >> x.page_log2;
+    const int page = x.page_table[b * x.stb + min(at, (int)x.width - 1) * x.stw];
+    return at < x.width && page >= 0 && page < x.pages && key <= last ? page : -1;
+  };
+  auto load = [&](Keys &t, int key0, int id) __attribute__((always_inline)) {
+    const int64_t row = (((int64_t)max(id, 0) * x.Hk + h) << x.page_log2) + ((key0 + lane) & ((1 << x.page_log2) - 1));
+    t.scale = (float)scales[row];
+    t.zero = x.cache.k_zero[row];
+    t.there = 0;
 #pragma unroll
-    for (int ps = 0; ps < PASSES; ++ps) {
-      const int row = ps * TPP + tid / LPT, sub = tid % LPT, r = min(row, p.rows - 1), i = r / p.G;
-      const int64_t off = b * x.sq[0] + (h * p.G + r - i * p.G) * x.sq[1] + i * x.sq[2] + sub * 8;
-      float v[8];
-      if (x.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(x.q) + off, v);
-      else if (x.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(x.q) + off, v);
-      else Load8<_Float16>::run(static_cast<const _Float16 *>(x.q) + off, v);
-      const QuantRow<8> q = quant_row<LPT, false, 8>(v, true);
-      if (row < 16) {
-        *reinterpret_cast<u32x2 *>(panel.codes + Panel::chunk(row, sub / 2) + 8 * (sub % 2)) = u32x2{q.codes[0], q.codes[1]};
-        if (sub == 0) constants(row, row, q.scale, (int)q.zp, q.sum);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int id_t = __builtin_amdgcn_readlane(id, 16 * i);   // (-1 behind the last key: of a tile that ends in a sequence the first keys exist)
+      t.there |= id_t >= 0 ? 1 << i : 0;
+      const int64_t first = (((int64_t)max(id_t, 0) * x.Hk + h) << x.page_log2) + ((key0 + 16 * i) & ((1 << x.page_log2) - 1));
+      const rsrc_t rs = make_rsrc(x.cache.k_codes + first * D, id_t >= 0 ? 16 * D : 0);
+#pragma unroll
+      for (int m = 0; m < KM; ++m) t.k[i][m] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c16 * D + 16 * g, 64 * m, 0));
     }
+  };
+  int page = page_of(begin + 64 * wave + lane);
+  Keys keys;
+  const rsrc_t panels = make_rsrc(ONE ? nullptr : p.panels + bh * p.panels_each * (int64_t)sizeof(Panel), ONE ? 0u : (unsigned)(p.panels_each * sizeof(Panel)));
+  auto fetch = [&](int panel) __attribute__((always_inline)) {   // (past the last panel's end: zeros)
+#pragma unroll
+    for (int e = 0; e < (PIECES + 3) / 4; ++e) {
+      const int piece = wave + 4 * e;
+      if (PIECES % 4 == 0 || piece < PIECES)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(panels, (lptr_t)(smem + (panel & 1) * BUF + 1024 * piece), 16, 16 * lane, panel * (int)sizeof(Panel) + 1024 * piece, 0, 0);
+    }
+  };
+  if constexpr (ONE) {
+    WeighRows<D> rows;
+    rows.load(p, b, h, 0);
+    rows.put(p, seq, *reinterpret_cast<Panel *>(smem), 0);
     __syncthreads();
-    rows_from(0);
+    rows_from(*reinterpret_cast<const Panel *>(smem), 0);
+  } else {
+    fetch(0);
+    load(keys, begin + 64 * wave, page);
   }
 
-  const S *scales = static_cast<const S *>(x.cache.k_scale);
   for (int step = 0; step < p.steps; ++step) {
     const int key0 = begin + 256 * step + 64 * wave, key = key0 + lane;
     if (ONE && key0 >= slots) break;   // (many rows: all waves go to the barriers)
     const bool mine = key0 <= last;    // (uniform over the wave)
+    const float was = before ? before[min(key, slots - 1)] : 0.f;   // (asked for beside the keys: behind them a step would wait for it alone)
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    if (mine || (!ONE && work)) {
-      // ---- 64 keys: the page of each, a key's constants in its lane, the codes of four tiles of 16
-      const int at = key >> x.page_log2;
-      const int page = x.page_table[b * x.stb + min(at, (int)x.width - 1) * x.stw];
-      const int id = at < x.width && page >= 0 && page < x.pages && key <= last ? page : -1;
-      const int64_t row = (((int64_t)max(id, 0) * x.Hk + h) << x.page_log2) + (key & ((1 << x.page_log2) - 1));
-      const float scale_mine = (float)scales[row];
-      const int zero_mine = x.cache.k_zero[row];
-      i32x4 k[4][KM];
-      int rk[4], zk[4], there = 0;
+    if (mine || !ONE) {   // (of one block of rows a wave that is past the last key stays so)
+      if constexpr (ONE) {   // (many rows: one step, and its keys are on their way already)
+        load(keys, key0, page);
+        if (step + 1 < p.steps) page = page_of(key + 256);
+      }
+      i32x4 (&k)[4][KM] = keys.k;
+      const int there = keys.there;
+      int rk[4], zk[4];
       float sk[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const int id_t = __builtin_amdgcn_readlane(id, 16 * t);   // (-1 behind the last key: of a tile that ends in a sequence the first keys exist)
-        there |= id_t >= 0 ? 1 << t : 0;
-        const int64_t first = (((int64_t)max(id_t, 0) * x.Hk + h) << x.page_log2) + ((key0 + 16 * t) & ((1 << x.page_log2) - 1));
-        const rsrc_t rs = make_rsrc(x.cache.k_codes + first * D, id_t >= 0 ? 16 * D : 0);
-#pragma unroll
-        for (int m = 0; m < KM; ++m) k[t][m] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c16 * D + 16 * g, 64 * m, 0));
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        sk[t] = __shfl(scale_mine, 16 * t + c16, 64);
-        zk[t] = __shfl(zero_mine, 16 * t + c16, 64);
+        sk[t] = __shfl(keys.scale, 16 * t + c16, 64);
+        zk[t] = __shfl(keys.zero, 16 * t + c16, 64);
         i32x4 r = {0, 0, 0, 0};
 #pragma unroll
         for (int m = 0; m < KM; ++m) r = __builtin_amdgcn_mfma_i32_16x16x64_i8(ones, k[t][m], r, 0, 0, 0);
         rk[t] = r[0];
       }
       // ---- the weights that 16 rows give
-      auto add = [&]() __attribute__((always_inline)) {
-        const bool masked = key0 + 63 > least || there != 15;
+      auto add = [&](int first_row) __attribute__((always_inline)) {
+        // (rows are in the order of their tokens: the first one sees the least)
+        const bool masked = key0 + 63 > seq.last_of(x, first_row / p.G) || there != 15;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           i32x4 s = {0, 0, 0, 0};
@@ -148,7 +229,7 @@ template <typename S, int D, bool ONE> __global__ __launch_bounds__(256) void pa
           float w[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const int dot = s[v] - __mul24(zq[v], rk[t]) - __mul24(zk[t], cq[v]);
+            const int dot = s[v] + __mul24(zq[v], rk[t]) + __mul24(cq[v], zk[t]);
             w[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(a[v], (float)dot * sk[t], -lse[v]));
           }
           if (masked) {
@@ -160,27 +241,18 @@ template <typename S, int D, bool ONE> __global__ __launch_bounds__(256) void pa
         }
       };
       if constexpr (ONE) {
-        add();
+        add(0);
       } else {
-        for (int r0 = 0; r0 < p.rows; r0 += PR) {
-          __syncthreads();   // the rows before are done with
-          for (int y = tid; y < PR * Panel::CPR; y += 256) {
-            const int at_row = y / Panel::CPR, r = min(r0 + at_row, p.rows - 1), i = r / p.G;
-            const int64_t from = (b * x.H + h * p.G + r - i * p.G) * x.N + i;
-            *reinterpret_cast<u32x4 *>(panel.codes + Panel::chunk(at_row, y % Panel::CPR)) =
-                *reinterpret_cast<const u32x4 *>(p.q_codes + from * D + 16 * (y % Panel::CPR));
-          }
-          if (tid < PR) {
-            const int r = min(r0 + tid, p.rows - 1), i = r / p.G;
-            const int64_t from = (b * x.H + h * p.G + r - i * p.G) * x.N + i;
-            constants(tid, r0 + tid, p.q_scale[from], p.q_zero[from], p.q_sum[from]);
-          }
-          __syncthreads();
+        for (int i = 0; i < p.panels_each; ++i) {
+          dma_wait();
+          __syncthreads();   // this panel is there, and nobody looks at the one before any more
+          if (i + 1 < p.panels_each) fetch(i + 1);
           if (mine) {
-            const int n = min(PR, p.rows - r0);
+            const Panel &panel = *reinterpret_cast<const Panel *>(smem + (i & 1) * BUF);
+            const int n = min(PR, p.rows - PR * i);
             for (int r = 0; r < n; r += 16) {
-              rows_from(r);
-              add();
+              rows_from(panel, r);
+              add(PR * i + r);
             }
           }
         }
@@ -195,34 +267,37 @@ template <typename S, int D, bool ONE> __global__ __launch_bounds__(256) void pa
     }
     const float keep = g & 1 ? y[1] : y[0], send = g & 1 ? y[0] : y[1];
     const float total = keep + __shfl_xor(send, 16, 64);
-    if (key < slots) out[key] = before ? __builtin_fmaf(p.w.decay, before[key], total) : total;
+    if (key < slots) out[key] = before ? __builtin_fmaf(p.w.decay, was, total) : total;
   }
 }
 
-// (rows as the launch in front quantizes them)
+// (the panels that the launch in front makes)
+static int64_t panel_count(int64_t rows) { return (rows + WEIGH_PANEL - 1) / WEIGH_PANEL; }
 int64_t paged_weigh_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D) {
-  return N * (H / Hk) <= 16 ? 0 : (B * H * N * (D + 9) + 15) / 16 * 16;
+  const int64_t rows = N * (H / Hk);
+  return rows <= 16 ? 0 : B * Hk * panel_count(rows) * (WEIGH_PANEL * (D + 20));
 }
 template <typename S, int D> static int launch_sd(const PagedWeighArgs &w, hipStream_t st) {
   const PagedAttnArgs &x = w.x;
+  static_assert(sizeof(WeighPanel<D, WEIGH_PANEL>) == WEIGH_PANEL * (D + 20), "as the workspace counts them");
   WeighKernelArgs p = {};
   p.w = w;
   p.G = (int)(x.H / x.Hk);
   p.rows = (int)(x.N * p.G);
   p.sm_scale_log2 = x.sm_scale * kLog2e;
+  p.panels = static_cast<const unsigned char *>(x.workspace);
+  p.panels_each = (int)panel_count(p.rows);
   const int64_t BH = x.B * x.Hk, slots = x.width << x.page_log2;
   const bool one = p.rows <= 16;
   p.steps = 1;
   while (one && p.steps < 4 && BH * ((slots + 512 * p.steps - 1) / (512 * p.steps)) >= 2048) p.steps *= 2;
   p.chunks = (int)((slots + 256 * p.steps - 1) / (256 * p.steps));
-  if ((double)BH * p.chunks > 2147483647.0) return set_error(QFA_EUNSUPPORTED, "paged_weights: too many keys for one launch");
+  const double quarters = (double)BH * p.panels_each * (WEIGH_PANEL / 16);
+  if ((double)BH * p.chunks > 2147483647.0 || quarters > 2147483647.0 || (double)p.panels_each * (WEIGH_PANEL * (D + 20)) > 2147483647.0)
+    return set_error(QFA_EUNSUPPORTED, "paged_weights: too many keys or rows for one launch");
   if (!one) {
-    const int64_t rows = x.B * x.H * x.N;
-    int8_t *codes = static_cast<int8_t *>(x.workspace), *zero = codes + rows * (D + 8);
-    float *scale = reinterpret_cast<float *>(codes + rows * D);
-    int32_t *sum = reinterpret_cast<int32_t *>(codes + rows * (D + 4));
-    if (int e = launch_quant(x.q, x.q_dtype, codes, scale, nullptr, 0, zero, sum, x.B, x.H, x.N, D, x.sq[0], x.sq[1], x.sq[2], x.H * x.N * D, x.N * D, D, st)) return e;
-    p.q_codes = codes; p.q_scale = scale; p.q_zero = zero; p.q_sum = sum;
+    weigh_rows_kernel<D><<<dim3((unsigned)quarters), dim3(256), 0, st>>>(p);
+    if (int e = check_launch("qfa_paged_weights (rows)")) return e;
   }
   const dim3 grid((unsigned)(BH * p.chunks)), block(256);
   if (one) paged_weigh_kernel<S, D, true><<<grid, block, 0, st>>>(p);
