@@ -34,7 +34,7 @@ template <typename S, int D, typename Deal, bool STREAM> __global__ __launch_bou
   unsigned x;
   typename Deal::Item item;
   if (!deal.find(x, item)) return;
-  const unsigned x_end = min((blockIdx.x + 1) * deal.each, deal.total);
+  const unsigned x_end = min((deal.workgroup() + 1) * deal.each, deal.total);
   if (x >= x_end) return;
   const int tid = threadIdx.x, lane = tid % 64, q16 = lane % 16, G = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -62,9 +62,6 @@ template <typename S, int D, typename Deal, bool STREAM> __global__ __launch_bou
     if constexpr (LIST) {
       list = a.blocks + ((int64_t)deal.row(item.p, item.h, 0).b * a.work.Hk + item.h) * a.work.N * a.keep + (int64_t)deal.row(item.p, item.h, 0).i * a.keep;
       last_of_list = deal.last_key(deal.row(item.p, item.h, 0), item.s);
-      // (a list's blocks are in its first places, as many as the token sees at most)
-      const int places = min(a.keep, (last_of_list >> a.page_log2) + 1), used = (int)((((int64_t)places << a.page_log2) + SKV_TILE - 1) / SKV_TILE) - t0;
-      my_tiles = min(my_tiles, used > wave ? (used - wave + 3) / 4 : 0);
     }
     const int seq = SHARED ? 0 : LIST ? deal.row(item.p, item.h, 0).b : item.p;   // whose pages
     const int nrows = min(PAGED_ROWS, deal.rows - PAGED_ROWS * item.rb);
@@ -86,6 +83,10 @@ template <typename S, int D, typename Deal, bool STREAM> __global__ __launch_bou
     };
     int pos = 0, pos_next = 0;   // of a list: where the halves' keys begin
     int pg = pages_from(0, pos), pg_next = my_tiles > 32 ? pages_from(32, pos_next) : -1;
+    if constexpr (LIST) {   // nothing is done for what stands behind a short list's blocks
+      const uint64_t there = __builtin_amdgcn_ballot_w64((pg >= 0) & (pos <= last_of_list));
+      if (my_tiles <= 32) my_tiles = there != 0 ? (63 - __builtin_clzll(there)) / 2 + 1 : 0;
+    }
     // (every load is issued whether the tile exists or not -- a missing one has an empty descriptor and fetches nothing)
     int64_t first[2];   // first row of each half among all rows
     auto load_keys = [&](Tile &t, int i) __attribute__((always_inline)) {
@@ -376,7 +377,7 @@ template <typename S, int D, typename Deal, bool STREAM> __global__ __launch_bou
         a.work.first[2 * deal.item_index(item.p, item.h, item.rb) + 1] = deal.each;
       }
     }
-    const int64_t slot = ((int64_t)blockIdx.x * 2 + (item.at == 0 ? 1 : 0)) * PAGED_ROWS;
+    const int64_t slot = ((int64_t)deal.workgroup() * 2 + (item.at == 0 ? 1 : 0)) * PAGED_ROWS;
     for (int y = tid; y < nrows * (D / 4); y += 256) {
       const int q = y / (D / 4), d = 4 * (y % (D / 4)), r = PAGED_ROWS * item.rb + q;
       float m = NO_KEY, l = 0.f;

@@ -39,8 +39,8 @@ template <typename Top, int T> __global__ __launch_bounds__(T) void evict_select
 }
 
 // D/16 lanes hold a row; a workgroup moves some rows of one sequence and key head, of keys or of values
-constexpr int EVICT_UNROLL = 4;
-template <typename S, int D> __global__ __launch_bounds__(256) void evict_move_kernel(PagedEvictArgs x, int chunks) {
+constexpr int EVICT_UNROLL = 2;   // rows of a thread (1 x 8 heads x 4096 and 16 x 32 x 1900 rows of 128, us: 2 6.1 and 128, 4 6.9 and 135, 8 11.2 and 150)
+template <typename S, int D, bool ONCE> __global__ __launch_bounds__(256) void evict_move_kernel(PagedEvictArgs x, int chunks) {
   constexpr int LPR = D / 16, ROWS = 256 / LPR;
   unsigned id = blockIdx.x;
   const int chunk = (int)(id % (unsigned)chunks);
@@ -74,7 +74,8 @@ template <typename S, int D> __global__ __launch_bounds__(256) void evict_move_k
     s[u] = (S)0.f;
     z[u] = 0;
     if (from[u] < 0 || to[u] < 0) continue;
-    w[u] = *reinterpret_cast<const u32x4 *>(codes + from[u] * D + 16 * sub);
+    const u32x4 *at = reinterpret_cast<const u32x4 *>(codes + from[u] * D + 16 * sub);
+    w[u] = ONCE ? __builtin_nontemporal_load(at) : *at;
     if (sub == 0) {
       s[u] = scale[from[u]];
       z[u] = zero[from[u]];
@@ -91,11 +92,18 @@ template <typename S, int D> __global__ __launch_bounds__(256) void evict_move_k
   }
 }
 
+template <typename S, int D> static void launch_move_d(const PagedEvictArgs &x, dim3 grid, int chunks, hipStream_t st) {
+  // Non-temporal loads of the old rows where what is moved, codes in and out, is 128 MiB or more: two caches in turn, 64, 128 and 256 elements, us with plain loads and
+  // with these: 64 MiB 24, 22, 18 and 29, 25, 24; 128 MiB 51, 46, 41 and 47, 41, 38; 256 MiB 104, 83, 75 and 96, 75, 67; 512 MiB 197, 160, 140 and 196, 156, 138
+  const int64_t rows = x.keep < x.width << x.page_log2 ? x.keep : x.width << x.page_log2;
+  if (4.0 * (double)(x.B * x.Hk * rows) * D >= 128.0 * (1 << 20)) evict_move_kernel<S, D, true><<<grid, dim3(256), 0, st>>>(x, chunks);
+  else evict_move_kernel<S, D, false><<<grid, dim3(256), 0, st>>>(x, chunks);
+}
 template <typename S> static int launch_move(const PagedEvictArgs &x, int64_t chunks, hipStream_t st) {
-  const dim3 grid((unsigned)(x.B * x.Hk * 2 * chunks)), block(256);
-  if (x.D == 64) evict_move_kernel<S, 64><<<grid, block, 0, st>>>(x, (int)chunks);
-  else if (x.D == 128) evict_move_kernel<S, 128><<<grid, block, 0, st>>>(x, (int)chunks);
-  else evict_move_kernel<S, 256><<<grid, block, 0, st>>>(x, (int)chunks);
+  const dim3 grid((unsigned)(x.B * x.Hk * 2 * chunks));
+  if (x.D == 64) launch_move_d<S, 64>(x, grid, (int)chunks, st);
+  else if (x.D == 128) launch_move_d<S, 128>(x, grid, (int)chunks, st);
+  else launch_move_d<S, 256>(x, grid, (int)chunks, st);
   return check_launch("qfa_paged_evict (rows)");
 }
 template <typename Top, int T> static void launch_top(const PagedEvictArgs &x, hipStream_t st) {

@@ -67,25 +67,28 @@ template <int D> __global__ __launch_bounds__(256) void paged_list_merge_kernel(
   }
 }
 
-// How the items are divided: whole ones while that keeps the workgroups evenly busy, else all units evenly
+// How the items are divided: each to a workgroup of its own, or, where few items with long lists leave CUs idle, all units evenly to two workgroups on
+// every CU.  The kernel that joins the pieces costs 5.5 us, as much as about 32 tiles of a workgroup (20 of 256 elements).  Items of T
+// tiles, us whole and cut:  64 elements 8 items T 32: 10.5, 11.7, T 48: 13.2, 11.6; 192 items T 64: 16.6, 19.6, T 256: 49, 43.8;  128: 8 items T 32: 12.4, 12.0,
+// 64 items T 32: 12.7, 12.6, T 64: 19.8, 16.1, 192 items T 128: 36.3, 39.8;  256: 8 items T 16: 11.9, 13.6, T 32: 16.4, 13.8, 64 items T 32: 18.1, 15.6,
+// 192 items T 256: 142, 151.
 struct PagedListPlan {
   unsigned tiles, each;
   int grid;
   bool cut;
 };
-static PagedListPlan list_plan(int64_t items, int64_t keep, int page_log2) {
+static PagedListPlan list_plan(int64_t items, int64_t keep, int page_log2, int D) {
   PagedListPlan p;
   p.tiles = (unsigned)(((keep << page_log2) + SKV_TILE - 1) / SKV_TILE);
-  const int64_t unit = p.tiles + LIST_EXTRA, total = items * unit;
-  const int64_t whole = (items + LIST_WGS - 1) / LIST_WGS * unit, even = max((int64_t)LIST_EXTRA, (total + LIST_WGS - 1) / LIST_WGS);
-  p.cut = even + LIST_EXTRA < whole;   // (the kernel that joins them costs about a start)
-  p.each = (unsigned)(p.cut ? even : whole);
+  const int64_t unit = p.tiles + LIST_EXTRA, total = items * unit, full = D == 256 ? 192 : 256;   // items that keep the chip busy
+  p.cut = items < full && (int64_t)p.tiles * (full - items) > (D == 256 ? 20 : 32) * full;
+  p.each = (unsigned)(p.cut ? max((int64_t)LIST_EXTRA, (total + LIST_WGS - 1) / LIST_WGS) : unit);
   p.grid = (int)((total + p.each - 1) / p.each);
   return p;
 }
 static int64_t list_items(int64_t B, int64_t N, int64_t Hk, int64_t G) { return B * N * Hk * ((G + PAGED_ROWS - 1) / PAGED_ROWS); }
 int64_t paged_list_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t keep, int page_log2) {
-  const PagedListPlan p = list_plan(list_items(B, N, Hk, H / Hk), keep, page_log2);
+  const PagedListPlan p = list_plan(list_items(B, N, Hk, H / Hk), keep, page_log2, D);
   return p.cut ? 2LL * p.grid * PAGED_ROWS * (D + 2) * 4 : 0;
 }
 double paged_list_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t keep, int page_log2) {
@@ -96,7 +99,7 @@ template <int D> static int launch_d(const PagedListArgs &l, hipStream_t st) {
   const PagedAttnArgs &x = l.x;
   const int G = (int)(x.H / x.Hk);
   const int64_t items = list_items(x.B, x.N, x.Hk, G);
-  const PagedListPlan p = list_plan(items, l.keep, x.page_log2);
+  const PagedListPlan p = list_plan(items, l.keep, x.page_log2, D);
   PagedAttnKernelArgs a = {};
   a.q = x.q; a.kc = x.cache.k_codes; a.ks = x.cache.k_scale; a.kz = x.cache.k_zero;
   a.vc = x.cache.v_codes; a.vs = x.cache.v_scale; a.vz = x.cache.v_zero; a.o = x.o; a.page_table = x.page_table;

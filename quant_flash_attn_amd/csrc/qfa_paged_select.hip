@@ -9,7 +9,7 @@
 // it is computed.  e+ and e- reach 255: the operands are e+ - 128 and e- - 128, and 128 times the bounds' own sums (a product with ones)
 // come on top.
 //
-// Two launches: scores, then for every token and key head the `keep` best (qfa_topk.h).
+// Scores, then for every token and key head the `keep` best (qfa_topk.h), in one launch or two.
 #include <cfloat>
 
 #include "qfa_host.h"
@@ -92,6 +92,22 @@ int launch_paged_bounds(const PagedSelectArgs &a, hipStream_t st) {
   return launch_bounds_s<__bf16>(a, st);
 }
 
+// The list of one token, by T threads (tid: which of them): the blocks with the `keep` largest scores, number(i) of block i
+template <int T, typename Top, typename Number>
+__device__ __forceinline__ void select_blocks(Top &top, const PagedSelectArgs &x, int64_t item, int64_t pos, int tid, Number number) {
+  const int64_t own = pos >> x.page_log2, last = own - x.last;   // (past the table's width: the last blocks are counted from there)
+  const int blocks = pos < 0 ? 0 : (int)min(own + 1, x.width), keep = (int)x.keep, first = (int)x.first;
+  int32_t *to = x.blocks + item * keep;
+  unsigned taken = 0;
+  if (blocks > 0)
+    taken = top.run(blocks, (unsigned)keep, number,
+                    [&](int i, float s) __attribute__((always_inline)) -> unsigned {
+                      return s == -INFINITY ? 0u : ((i < first) | (i > last)) ? TOP_ALWAYS : top_key(s);
+                    },
+                    [&](unsigned place, int i, float) __attribute__((always_inline)) { to[place] = i; });
+  for (int i = (int)taken + tid; i < keep; i += T) to[i] = -1;
+}
+
 // ---------------------------------------------------------------------------------------------------------------- scores
 struct SelectKernelArgs {
   PagedSelectArgs x;
@@ -128,11 +144,13 @@ struct SelectPlace {
     start = x.starts[b];
     brings = x.counts ? max((int64_t)0, min((int64_t)x.counts[b], x.N)) : x.N;
   }
-  // the last block that token t of the tile sees (-1: none)
-  __device__ __forceinline__ int64_t last_block(const PagedSelectArgs &x, int t) const {
+  // the position of token t of the tile (-1: it sees nothing), and its last block
+  __device__ __forceinline__ int64_t position(int t) const {
     const int64_t pos = start + n0 + t;
-    return t >= 0 && t < tokens && n0 + t < brings && pos >= 0 ? pos >> x.page_log2 : -1;
+    return t >= 0 && t < tokens && n0 + t < brings && pos >= 0 ? pos : -1;
   }
+  __device__ __forceinline__ int64_t last_block(const PagedSelectArgs &x, int t) const { return position(t) >> x.page_log2; }
+  __device__ __forceinline__ int64_t item(const PagedSelectArgs &x, int t) const { return (b * x.Hk + h) * x.N + n0 + t; }
   // ... and that any of them sees
   __device__ __forceinline__ int64_t last_block(const PagedSelectArgs &x) const { return last_block(x, (int)min((int64_t)tokens, brings - n0) - 1); }
 };
@@ -199,8 +217,11 @@ __device__ __forceinline__ float block_score(int dot_high, int dot_low, int own_
 
 // Up to four rows (a token's heads, mostly): they stand four times among the 16 rows of a product, so that every group of lanes has the products of all
 // rows with all of four tiles of 16 blocks, and goes on with one of them: a lane has one block.  A wave takes 64 blocks at a time.
-template <int D> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void block_scores_few_kernel(SelectKernelArgs p) {
+// WHOLE: a workgroup has all blocks of its tokens, keeps their scores, and selects.
+constexpr int SELECT_WHOLE_FEW = 1024, SELECT_WHOLE = 256;   // blocks at most
+template <int D, bool WHOLE> __global__ __launch_bounds__(256, 2) void block_scores_few_kernel(SelectKernelArgs p) {
   constexpr int KM = D / 64;
+  __shared__ float held[WHOLE ? 4 : 1][WHOLE ? SELECT_WHOLE_FEW : 1];
   __shared__ __attribute__((aligned(16))) typename SplitRows<D>::Lds lds;
   const PagedSelectArgs &x = p.x;
   const int tid = threadIdx.x, lane = tid % 64, c16 = lane % 16, g = lane / 16;
@@ -222,6 +243,8 @@ template <int D> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void block_
     if (x.all_scores)
       for (int64_t i = begin + tid; i < end; i += 256)
         for (int t = 0; t < at.tokens; ++t) to[t * x.width + i] = -INFINITY;
+    if (WHOLE)
+      for (int64_t i = tid; i < at.tokens * x.keep; i += 256) x.blocks[at.item(x, 0) * x.keep + i] = -1;
     return;
   }
   i32x4 qf[2][KM];
@@ -282,10 +305,20 @@ template <int D> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void block_
 #pragma unroll
         for (int v = 0; v < 4; ++v)
           if (v / p.G == t) best = fmaxf(best, y[v]);
-        if (j < end) to[t * x.width + j] = there && j <= at.last_block(x, t) ? best : -INFINITY;
+        const float score = there && j <= at.last_block(x, t) ? best : -INFINITY;
+        if (WHOLE && j < end) held[t][j] = score;
+        if ((!WHOLE || x.all_scores) && j < end) to[t * x.width + j] = score;
       }
     } else if (x.all_scores && j < end) {
       for (int t = 0; t < at.tokens; ++t) to[t * x.width + j] = -INFINITY;
+    }
+  }
+  if constexpr (WHOLE) {
+    __shared__ TopHeld<256, SELECT_WHOLE_FEW, 8> top;
+    __syncthreads();
+    for (int t = 0; t < at.tokens; ++t) {
+      if (t > 0) __syncthreads();   // the token before is done with
+      select_blocks<256>(top, x, at.item(x, t), at.position(t), tid, [&](int i) __attribute__((always_inline)) { return held[t][i]; });
     }
   }
 }
@@ -294,8 +327,9 @@ template <int D> __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void block_
 // of the product, blocks its columns.  The pages of up to four steps are one load, a step's bounds are requested a step ahead, and the
 // first ones before the queries are quantized.
 constexpr int SELECT_STEPS = 4;
-template <int D> __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void block_scores_kernel(SelectKernelArgs p) {
+template <int D, bool WHOLE> __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void block_scores_kernel(SelectKernelArgs p) {
   constexpr int KM = D / 64;
+  __shared__ float held[WHOLE ? 16 : 1][WHOLE ? SELECT_WHOLE : 1];
   __shared__ __attribute__((aligned(16))) typename SplitRows<D>::Lds lds;
   __shared__ float out[4][16][17];       // per wave: rows, blocks
   const PagedSelectArgs &x = p.x;
@@ -315,6 +349,8 @@ template <int D> __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void block_
     if (x.all_scores)
       for (int64_t i = begin + tid; i < end; i += 256)
         for (int t = 0; t < tokens; ++t) to[t * x.width + i] = -INFINITY;
+    if (WHOLE)
+      for (int64_t i = tid; i < tokens * x.keep; i += 256) x.blocks[at.item(x, 0) * x.keep + i] = -1;
     return;
   }
   struct Bounds {
@@ -381,8 +417,10 @@ template <int D> __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void block_
       // ---- of a token's heads the largest
       auto store = [&](int t, float best) __attribute__((always_inline)) {
         if (t >= tokens || j >= end) return;
-        if (rb > 0) best = fmaxf(best, to[t * x.width + j]);   // (this lane wrote it)
-        to[t * x.width + j] = k.there && j <= at.last_block(x, t) ? best : -INFINITY;
+        if (rb > 0) best = fmaxf(best, WHOLE ? held[t][j] : to[t * x.width + j]);   // (this lane wrote it)
+        const float score = k.there && j <= at.last_block(x, t) ? best : -INFINITY;
+        if (WHOLE) held[t][j] = score;
+        if (!WHOLE || x.all_scores) to[t * x.width + j] = score;
       };
       if (folds) {
         if (p.G == 1) {
@@ -414,6 +452,12 @@ template <int D> __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void block_
   if (x.all_scores)   // blocks behind the last one that is seen, of waves that have left the loop above
     for (int64_t i = (seen + 15) / 16 * 16 + tid; i < end; i += 256)
       for (int t = 0; t < tokens; ++t) to[t * x.width + i] = -INFINITY;
+  if constexpr (WHOLE) {   // a wave for each token
+    __syncthreads();
+    TopFew top;
+    for (int t = wave; t < tokens; t += 4)
+      select_blocks<64>(top, x, at.item(x, t), at.position(t), lane, [&](int i) __attribute__((always_inline)) { return held[t][i]; });
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------- the best
@@ -421,26 +465,20 @@ template <int D> __global__ __launch_bounds__(256, D == 256 ? 2 : 3) void block_
 template <typename Top, int T> __global__ __launch_bounds__(T) void block_select_kernel(PagedSelectArgs x) {
   __shared__ Top top;
   const int64_t item = blockIdx.x, bh = index_div(item, x.N), n = item - bh * x.N, b = index_div(bh, x.Hk);
-  const int64_t pos = token_position(x, b, n), own = pos >> x.page_log2;   // (past the table's width: the last blocks are counted from there)
-  const int blocks = pos < 0 ? 0 : (int)min(own + 1, x.width), keep = (int)x.keep;
   const float *scores = x.scores + item * x.width;
-  int32_t *to = x.blocks + item * keep;
-  unsigned taken = 0;
-  if (blocks > 0) {
-    const int first = (int)x.first;
-    const int64_t last = own - x.last;
-    taken = top.run(blocks, (unsigned)keep, [&](int i) __attribute__((always_inline)) { return scores[i]; },
-                    [&](int i, float s) __attribute__((always_inline)) -> unsigned {
-                      return s == -INFINITY ? 0u : ((i < first) | (i > last)) ? TOP_ALWAYS : top_key(s);
-                    },
-                    [&](unsigned place, int i, float) __attribute__((always_inline)) { to[place] = i; });
-  }
-  for (int i = (int)taken + (int)threadIdx.x; i < keep; i += T) to[i] = -1;
+  select_blocks<T>(top, x, item, token_position(x, b, n), threadIdx.x, [&](int i) __attribute__((always_inline)) { return scores[i]; });
 }
 template <typename Top, int T> static void launch_top(const PagedSelectArgs &x, hipStream_t st) {
   block_select_kernel<Top, T><<<dim3((unsigned)(x.B * x.Hk * x.N)), dim3(T), 0, st>>>(x);
 }
 
+template <int D> static void launch_scores(const SelectKernelArgs &p, bool few, bool whole, dim3 grid, hipStream_t st) {
+  const dim3 block(256);
+  if (few && whole) block_scores_few_kernel<D, true><<<grid, block, 0, st>>>(p);
+  else if (few) block_scores_few_kernel<D, false><<<grid, block, 0, st>>>(p);
+  else if (whole) block_scores_kernel<D, true><<<grid, block, 0, st>>>(p);
+  else block_scores_kernel<D, false><<<grid, block, 0, st>>>(p);
+}
 int launch_paged_select(const PagedSelectArgs &x, hipStream_t st) {
   SelectKernelArgs p;
   p.x = x;
@@ -452,21 +490,24 @@ int launch_paged_select(const PagedSelectArgs &x, hipStream_t st) {
   const bool few = p.row_blocks == 1 && p.tokens_each * p.G <= 4;
   const int step = few ? 256 : 64;   // blocks of a workgroup's step
   p.steps = 1;
-  while (p.steps < SELECT_STEPS && groups * ((x.width + 2 * step * p.steps - 1) / (2 * step * p.steps)) >= 512) p.steps *= 2;
+  // Scores and selection in one launch where a workgroup can hold all blocks of its tokens, and has one step of them or enough others beside it.  Four query
+  // heads of 128 elements, us with two launches and with one: 256 blocks of 1, 8 and 32 sequences with 8 key heads 10.3, 10.6, 10.9 and 9.1, 8.9, 9.4;
+  // 1000 blocks 14.5, 15.1, 23 and 20.3, 20.7, 22.4
+  const bool whole = x.width <= SELECT_WHOLE || (few && x.width <= SELECT_WHOLE_FEW && groups >= 256);
+  if (whole) p.steps = (int)((x.width + step - 1) / step);   // (SELECT_STEPS at most)
+  while (!whole && p.steps < SELECT_STEPS && groups * ((x.width + 2 * step * p.steps - 1) / (2 * step * p.steps)) >= 512) p.steps *= 2;
   p.chunks = (int)((x.width + step * p.steps - 1) / (step * p.steps));
   const int64_t outer = x.B * p.chunks;
   p.round = xcd_whole_heads(outer);
   const int64_t outer_grid = p.round ? (outer + 7) / 8 * 8 : outer, grid_size = outer_grid * x.Hk * p.token_tiles;
   const double most = (double)outer_grid * (double)x.Hk * (double)p.token_tiles, items = (double)x.B * (double)x.Hk * (double)x.N;
   if (most > 2147483647.0 || items > 2147483647.0) return set_error(QFA_EUNSUPPORTED, "paged_select: too many tokens and blocks for one launch");
-  const dim3 grid((unsigned)grid_size), block(256);
-  if (few && x.D == 64) block_scores_few_kernel<64><<<grid, block, 0, st>>>(p);
-  else if (few && x.D == 128) block_scores_few_kernel<128><<<grid, block, 0, st>>>(p);
-  else if (few) block_scores_few_kernel<256><<<grid, block, 0, st>>>(p);
-  else if (x.D == 64) block_scores_kernel<64><<<grid, block, 0, st>>>(p);
-  else if (x.D == 128) block_scores_kernel<128><<<grid, block, 0, st>>>(p);
-  else block_scores_kernel<256><<<grid, block, 0, st>>>(p);
+  const dim3 grid((unsigned)grid_size);
+  if (x.D == 64) launch_scores<64>(p, few, whole, grid, st);
+  else if (x.D == 128) launch_scores<128>(p, few, whole, grid, st);
+  else launch_scores<256>(p, few, whole, grid, st);
   if (int e = check_launch("qfa_paged_select (scores)")) return e;
+  if (whole) return 0;
   // one wave for a few blocks (3330 x 219: 5.8 us, with a wave and counters in LDS 7.5, with four 9.3), more for many
   if (x.width <= 256) launch_top<TopFew, 64>(x, st);
   else if (x.width <= 1024) launch_top<TopHeld<256, 1024, 8>, 256>(x, st);

@@ -56,6 +56,7 @@ __device__ __forceinline__ unsigned wave_scan(unsigned x) {
 // ONE: a problem has a single block of rows
 template <bool SHARED, bool ONE> struct PagedDeal {
   static constexpr bool ONE_PROBLEM = SHARED, LIST = false;
+  static __device__ __forceinline__ unsigned workgroup() { return blockIdx.x; }
   const PagedWork &a;
   const int BR, TK;                 // work.br and work.tk, constants in the kernels that are made for them
   int rows, blocks, problems;       // rows and blocks of rows of a problem
@@ -234,19 +235,25 @@ struct PagedListDeal {
     const int b = p / a.N, n = a.counts ? max(0, min(a.counts[b], a.N)) : a.N;
     return {__builtin_amdgcn_readfirstlane(a.starts[b]), __builtin_amdgcn_readfirstlane(n)};
   }
-  // The item of that number: row blocks of a head, heads of a token, tokens
+  // Consecutive workgroups go round the 8 XCDs.  Where a sequence has several tokens, whose lists share blocks, each XCD takes an eighth of the work side by
+  // side: the tokens of a key head then find each other's keys in one L2 (2 x 333 tokens, 8 key heads, 2048 keys each: LIST_US)
+  __device__ __forceinline__ unsigned workgroup() const {
+    const unsigned n = gridDim.x, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
+    return a.N == 1 ? blockIdx.x : xcd * (n / 8) + min(xcd, n % 8) + at;
+  }
+  // The item of that number: blocks of rows of a token, tokens of a head, heads, sequences
   __device__ __forceinline__ void item(unsigned n, Item &it) const {
-    const unsigned bh = n / (unsigned)blocks;
-    it.rb = (int)(n - bh * (unsigned)blocks);
-    it.p = (int)(bh / (unsigned)a.Hk);
-    it.h = (int)(bh - (unsigned)it.p * (unsigned)a.Hk);
+    const unsigned token = n / (unsigned)blocks, bh = token / (unsigned)a.N, b = bh / (unsigned)a.Hk;
+    it.rb = (int)(n - token * (unsigned)blocks);
+    it.h = (int)(bh - b * (unsigned)a.Hk);
+    it.p = (int)(b * (unsigned)a.N + token - bh * (unsigned)a.N);
     it.tiles = a.list_tiles;
     it.first = n * per_item + (unsigned)a.extra;
     it.at = 0;
     it.s = seq(it.p);
   }
   __device__ __forceinline__ bool find(unsigned &x, Item &it) const {
-    x = blockIdx.x * each;
+    x = workgroup() * each;
     if (x >= total) return false;
     item(x / per_item, it);
     x = max(x, it.first);

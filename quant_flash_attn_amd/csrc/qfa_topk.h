@@ -23,7 +23,7 @@ __device__ __forceinline__ unsigned top_key(float x) {
 struct TopFew {
   template <typename Number, typename Key, typename Take>
   __device__ __forceinline__ unsigned run(int n, unsigned k, Number number, Key key_of, Take take) {
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x % 64;
     float x[4];
     unsigned u[4];
 #pragma unroll

@@ -69,8 +69,7 @@ def quant_flash_attn_paged_blocks(q: torch.Tensor, cache, page_table: torch.Tens
     arithmetic.  No gradient.
 
     A token sees the keys up to itself in the blocks of its list.  The order of a list does not matter, a block that stands in it twice
-    counts twice, numbers outside the page table and blocks without a page are passed over; of a list only the first places
-    are looked at, as many as there are blocks up to the token's own.  Tokens that see no key, and padding, get zeros.
+    counts twice, numbers outside the page table and blocks without a page are passed over.  Tokens that see no key, and padding, get zeros.
     """
     sm = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else float(sm_scale)
     return _lib.host().paged_blocks(q, tuple(cache), page_table, starts, blocks, counts, sm)

@@ -21,7 +21,7 @@ def _expect(p, blocks, sm):
             pos = int(p.starts[b]) + n
             for h in range(p.Hk):
                 at = []
-                for j in blocks[b, h, n].tolist()[:max(0, pos // p.page + 1)]:
+                for j in blocks[b, h, n].tolist():
                     if 0 <= j < p.width and 0 <= int(p.table[b, j]) < p.pages:
                         at += [i for i in range(j * p.page, (j + 1) * p.page) if i <= pos and i < L]
                 if not at:
@@ -90,8 +90,7 @@ def test_padding(qfa, keep):
 @pytest.mark.gpu
 @pytest.mark.parametrize("keep", [6, 60])
 def test_lists_as_they_may_come(qfa, keep):
-    """Blocks twice, behind the token, outside the table, without a page, holes between them, a list of nothing; entries behind the last place
-    that counts are garbage."""
+    """Blocks twice, behind the token, outside the table, without a page, holes between them and in front, a list of nothing."""
     p = lm.Problem(4, 4, 2, 2, 64, 16, [1000, 1000, 70, 1000], seed=7)
     p.table[1, 5], p.table[1, 6], p.table[3, 2] = -1, p.pages, 1 << 30
     g = torch.Generator().manual_seed(keep)
@@ -99,7 +98,9 @@ def test_lists_as_they_may_come(qfa, keep):
     blocks[0, 0, 0, :4] = torch.tensor([3, 3, -1, 2147483647])
     blocks[0, 1] = -1
     blocks[1, :, :, :3] = torch.tensor([5, 6, 7])
-    blocks[2, :, :, 5:] = -2147483648   # (70 keys: five blocks)
+    blocks[2, :, :, 5:] = -2147483648
+    blocks[2, 1, 1, :] = -1
+    blocks[2, 1, 1, -1] = 4
     _check(qfa, p, keep, blocks)
 
 
@@ -123,6 +124,30 @@ def test_all_blocks_are_all_keys(qfa, B, H, Hk, N, keys):
     full = qfa.quant_flash_attn_paged(*args)
     _, size = _expect(p, blocks, m.sm_of(128))
     assert ((o.float() - full.float()).abs().cpu() <= 2 * m.HALF[torch.bfloat16] * full.float().abs().cpu() + 2.0 ** -9 * size + 1e-5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,Hk,G,N,D,keys", [(50, 4, 1, 1, 64, 4800), (2, 2, 4, 40, 128, 9000), (5, 7, 20, 1, 64, 3000), (1, 3, 2, 900, 64, 2000)])
+def test_workgroups_with_parts_of_several_lists(qfa, B, Hk, G, N, D, keys):
+    """Enough long lists that a workgroup ends one and begins the next, and more than are under way at once: every block in any order, against
+    quant_flash_attn_paged.  Both round probabilities times scales to binary16 (2^-11 each, relative to a sum of p |v|), the offsets' sums, and the result."""
+    g, page = torch.Generator().manual_seed(B), 16
+    width = keys // page
+    table = torch.randperm(B * width, generator=g).int().view(B, width).to(DEV)
+    zero = torch.zeros(B, dtype=torch.int32, device=DEV)
+    q = (2 * torch.randn(B, Hk * G, N, D, generator=g)).bfloat16().to(DEV)
+    k, v = (torch.randn(B, Hk, keys, D, device=DEV).bfloat16() for _ in range(2))
+    starts = torch.full((B,), keys - N - 3, dtype=torch.int32, device=DEV)
+    blocks = torch.rand(B, Hk, N, width, device=DEV).argsort(-1).int()
+    outs = []
+    for values in (v, v.abs()):
+        cache = qfa.make_paged_cache(B * width, Hk, page, D, device=DEV)
+        qfa.paged_cache_append(cache, k, values, table, zero)
+        outs.append(qfa.quant_flash_attn_paged(q, cache, table, starts).double())
+        if values is v:
+            o = qfa.quant_flash_attn_paged_blocks(q, cache, table, starts, blocks).double()
+    full, size = outs
+    assert bool(((o - full).abs() <= 2 * m.HALF[torch.bfloat16] * full.abs() + 2.0 ** -9 * size + 2 * (32 + keys / 32) * m.U32 * 1407 * 0.05).all())
 
 
 @pytest.mark.gpu
