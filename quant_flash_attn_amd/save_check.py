@@ -9,6 +9,8 @@ All lanes are on at a kernel's start (workgroups are whole waves) and wherever e
 exec while they all were; such registers are followed through copies and through the lanes of vector registers that hold spilled
 scalars.  Whatever else happens to exec counts as turning lanes off.
 
+Kernels that wait for loads by their number (COUNTING) may have no scratch at all: what the compiler spills counts among the loads.
+
     python -m quant_flash_attn_amd.save_check FILE.s
 """
 from __future__ import annotations
@@ -21,6 +23,8 @@ from .acc_check import _kernels
 
 _SGPR = re.compile(r"^s(?:(\d+)|\[(\d+):(\d+)\])$")
 _SAVE = re.compile(r"v_accvgpr_write_b32 a\S+ v\d+$|scratch_store_\w+ \S+ [av]")
+
+COUNTING = ("paged_list_few_kernel",)
 
 # what is known at an instruction: whether all lanes are on, and the scalar halves ("s", n) or spilled ones ("v", n, lane) that hold the
 # low (0) or high (1) half of a mask of all lanes
@@ -93,7 +97,9 @@ def _saved(i) -> Optional[FrozenSet[Tuple[str, int]]]:
 def check(path: str) -> List[str]:
     """What is wrong, one line each; empty: nothing."""
     bad: List[str] = []
-    for name, ins, labels, _ in _kernels(path):
+    for name, ins, labels, scratch in _kernels(path):
+        if scratch and any(k in name for k in COUNTING):
+            bad.append(f"{path}: {name}: counts its loads, and has {scratch} bytes of scratch")
         if not any(_saved(i) for i in ins):
             continue
         after: Dict[int, List[int]] = {}

@@ -104,6 +104,24 @@ def test_lists_as_they_may_come(qfa, keep):
     _check(qfa, p, keep, blocks)
 
 
+# more lists than the chip works on at once, of few query heads each; of more than 32 tiles of 64 keys; a third of the places without a block
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,N,D,page,keep,keys,dtype,scale_dtype", [
+    (3, 8, 2, 90, 64, 16, 150, 2600, torch.float16, torch.float32), (2, 3, 1, 270, 128, 128, 19, 2500, torch.bfloat16, torch.float16),
+    (1, 4, 4, 130, 128, 32, 5, 500, torch.float32, torch.bfloat16), (66, 20, 10, 1, 64, 64, 3, 700, torch.bfloat16, torch.float32),
+    (300, 2, 2, 1, 128, 16, 9, 333, torch.bfloat16, torch.float16)])
+def test_many_lists(qfa, B, H, Hk, N, D, page, keep, keys, dtype, scale_dtype):
+    p = lm.Problem(B, H, Hk, N, D, page, [max(N, keys - 37 * i) for i in range(B)], counts=[max(0, N - 3 * i) if N > 1 else 1 for i in range(B)], seed=H + N,
+                   dtype=dtype, scale_dtype=scale_dtype)
+    g = torch.Generator().manual_seed(B)
+    blocks = torch.rand(B, Hk, N, p.width, generator=g).argsort(-1)[..., :keep].int()
+    if blocks.shape[-1] < keep:
+        blocks = torch.cat([blocks, torch.full((B, Hk, N, keep - blocks.shape[-1]), -1, dtype=torch.int32)], -1)
+    blocks[torch.rand(blocks.shape, generator=g) < 1 / 3] = -1
+    blocks[0, 0, 0] = -1
+    _check(qfa, p, keep, blocks.contiguous())
+
+
 @pytest.mark.gpu
 def test_rows_that_see_nothing_are_zero(qfa):
     p = lm.Problem(3, 4, 2, 6, 128, 16, [50, 6, 20], seed=1)
