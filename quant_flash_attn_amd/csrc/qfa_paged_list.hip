@@ -20,7 +20,7 @@ constexpr int LIST_EXTRA = 12;      // units of an item beside its tiles, as the
 // (96 %): 2.9 GB, 16 TB/s.  No unit is busy more than two thirds of the time; 270 vector instructions of 64 keys and wave, 128 of
 // them the values' conversion, are the most of them.
 constexpr int FEW_ROWS = 4, FEW_TILE = 64, FEW_WAVES = 2;
-template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, 3) void paged_list_few_kernel(PagedAttnKernelArgs a) {
+template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 256 ? 2 : 3) void paged_list_few_kernel(PagedAttnKernelArgs a) {
   constexpr int KM = D / 64, DB = D / 16, VB = D / 16, VD = VB / 4;   // as in paged_rows_kernel
   constexpr int LPT = D / 8;
   constexpr int OFF_ONES = (FEW_ROWS + 1) * D, OFF_ST = OFF_ONES + 16, OFF_TC = OFF_ST + 3 * 16;   // (query codes; D bytes of zeros; ones)
@@ -46,10 +46,12 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, 3) voi
   // Keys are loaded into LDS as they lie, 16 bytes a lane, and read from there in the fragments' order: loaded in that order,
   // neighbouring lanes' bytes are of different rows, and each lane is an access of its own to the L1 cache.  Within a row the 16-byte
   // parts are exchanged by its number, for the banks.
-  constexpr int PARTS = D / 16, PER_LINE = 8 / PARTS;   // rows in 128 bytes
-  auto k_at = [](int row, int part) __attribute__((always_inline)) -> int { return row * D + 16 * (part ^ (row / PER_LINE % PARTS)); };
+  constexpr int PARTS = D / 16, PER_LINE = PARTS < 8 ? 8 / PARTS : 1, TURNS = PARTS < 8 ? PARTS : 8;   // (rows in 128 bytes)
+  auto k_at = [](int row, int part) __attribute__((always_inline)) -> int { return row * D + 16 * (part ^ (row / PER_LINE % TURNS)); };
   unsigned char *kl = smem + OFF_K;
-  const int k_off = k_at(lane / PARTS, lane % PARTS);   // (1024 / D rows further on the exchange is the same)
+  int k_off[4];   // (KM of them)
+#pragma unroll
+  for (int m = 0; m < KM; ++m) k_off[m] = k_at(m * (1024 / D) + lane / PARTS, lane % PARTS) - 1024 * m;
   const int page_parts_log2 = a.page_log2 - 4;
   unsigned *tc = reinterpret_cast<unsigned *>(smem + OFF_TC);
   const int32_t *list = a.blocks + (((int64_t)token.b * a.work.Hk + item.h) * a.work.N + token.i) * a.keep;
@@ -98,7 +100,7 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, 3) voi
     for (int g = 0; g < 4; ++g) {
       const rsrc_t rk = make_rsrc(a.kc + (int64_t)first[g] * D, t.ok >> g & 1 ? 16 * D : 0);
 #pragma unroll
-      for (int m = 0; m < KM; ++m) __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lptr_t)(kl + 16 * D * g + 1024 * m), 16, k_off, 1024 * m, 0, 0);
+      for (int m = 0; m < KM; ++m) __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lptr_t)(kl + 16 * D * g + 1024 * m), 16, k_off[m], 1024 * m, 0, 0);
     }
   };
   auto load_values = [&](Tile &t) __attribute__((always_inline)) {
@@ -107,7 +109,11 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, 3) voi
       const rsrc_t rv = make_rsrc(a.vc + (int64_t)first[g] * D, t.ok >> g & 1 ? 16 * D : 0);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        if constexpr (VD == 2) {
+        if constexpr (VD == 4) {
+          const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off, e * D, 0));
+#pragma unroll
+          for (int y = 0; y < 4; ++y) t.v[4 * g + e][y] = w[y];
+        } else if constexpr (VD == 2) {
           const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_off, e * D, 0));
           t.v[4 * g + e][0] = w[0];
           t.v[4 * g + e][1] = w[1];
@@ -119,13 +125,15 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, 3) voi
   };
 
   // the queries are requested beside the pages, and quantized while the first keys are on their way
-  float qv[8];
-  {
-    const auto r = deal.row(item.p, item.h, min(lane / LPT, nrows - 1));
+  constexpr int PASSES = D == 256 ? 2 : 1;
+  float qv[PASSES][8];
+#pragma unroll
+  for (int ps = 0; ps < PASSES; ++ps) {
+    const auto r = deal.row(item.p, item.h, min(ps * (64 / LPT) + lane / LPT, nrows - 1));
     const int64_t off = r.b * a.sqb + r.qh * a.sqh + r.i * a.sqn + lane % LPT * 8;
-    if (a.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(a.q) + off, qv);
-    else if (a.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(a.q) + off, qv);
-    else Load8<_Float16>::run(static_cast<const _Float16 *>(a.q) + off, qv);
+    if (a.q_dtype == QFA_F32) Load8<float>::run(static_cast<const float *>(a.q) + off, qv[ps]);
+    else if (a.q_dtype == QFA_BF16) Load8<__bf16>::run(static_cast<const __bf16 *>(a.q) + off, qv[ps]);
+    else Load8<_Float16>::run(static_cast<const _Float16 *>(a.q) + off, qv[ps]);
   }
   Tile ta;
   load_keys(ta, 0);
@@ -135,9 +143,10 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, 3) voi
   int *st_z = reinterpret_cast<int *>(smem + OFF_ST + 16), *st_c = reinterpret_cast<int *>(smem + OFF_ST + 32);
   if (lane <= D / 16)   // (the zeros, and the ones behind them)
     *reinterpret_cast<i32x4 *>(smem + FEW_ROWS * D + 16 * lane) = lane < D / 16 ? i32x4{0, 0, 0, 0} : i32x4{0x01010101, 0x01010101, 0x01010101, 0x01010101};
-  {
-    const QuantRow<8> row = quant_row<LPT, false, 8>(qv, true);
-    const int r = lane / LPT;
+#pragma unroll
+  for (int ps = 0; ps < PASSES; ++ps) {
+    const QuantRow<8> row = quant_row<LPT, false, 8>(qv[ps], true);
+    const int r = ps * (64 / LPT) + lane / LPT;
     if (r < FEW_ROWS) {
       *reinterpret_cast<u32x2 *>(smem + r * D + lane % LPT * 8) = u32x2{row.codes[0], row.codes[1]};
       if (lane % LPT == 0) {
@@ -394,9 +403,11 @@ template <int D> __global__ __launch_bounds__(256) void paged_list_merge_kernel(
 // tiles, us whole and cut:  64 elements 8 items T 32: 10.5, 11.7, T 48: 13.2, 11.6; 192 items T 64: 16.6, 19.6, T 256: 49, 43.8;  128: 8 items T 32: 12.4, 12.0,
 // 64 items T 32: 12.7, 12.6, T 64: 19.8, 16.1, 192 items T 128: 36.3, 39.8;  256: 8 items T 16: 11.9, 13.6, T 32: 16.4, 13.8, 64 items T 32: 18.1, 15.6,
 // 192 items T 256: 142, 151.
-// The kernel for up to four rows is as fast or faster from 512 items on, and for few keys: items x keys, us of paged_rows_kernel (whole
-// or cut) and of it:  64 elements 8 x 128: 6.5, 6.2, 8 x 512: 7.9, 8.4, 256 x 512: 8.0, 8.6, 512 x 512: 11.7, 11.0, 1024 x 64: 10.6, 6.2, 1024 x 4096:
-// 106, 104;  128: 8 x 256: 7.8, 7.2, 8 x 1024: 12.4, 14.6, 128 x 4096: 29.9, 44.6, 512 x 256: 11.9, 10.2, 512 x 4096: 99.4, 100.6, 1024 x 64: 14.6, 8.4.
+// The kernel for up to four rows is as fast or faster from 512 items on (1024 of 256 elements), and for few keys: items x keys, us of
+// paged_rows_kernel (whole or cut) and of it:  64 elements 8 x 128: 6.5, 6.2, 8 x 512: 7.9, 8.4, 256 x 512: 8.0, 8.6, 512 x 512: 11.7, 11.0,
+// 1024 x 64: 10.6, 6.2, 1024 x 4096: 106, 104;  128: 8 x 256: 7.8, 7.2, 8 x 1024: 12.4, 14.6, 128 x 4096: 29.9, 44.6, 512 x 256: 11.9, 10.2,
+// 512 x 4096: 99.4, 100.6, 1024 x 64: 14.6, 8.4;  256: 8 x 128: 8.6, 9.3, 512 x 512: 26.6, 29.1, 512 x 2048: 97, 102, 1024 x 64: 19.2, 14.3,
+// 1024 x 2048: 189, 190, 2664 (333 tokens of one sequence) x 2048: 216, 170.
 struct PagedListPlan {
   unsigned tiles, each;
   int grid;
@@ -404,7 +415,7 @@ struct PagedListPlan {
 };
 static PagedListPlan list_plan(int64_t items, int64_t keep, int page_log2, int64_t G, int D) {
   PagedListPlan p;
-  p.few = D <= 128 && G <= FEW_ROWS && (items >= 512 || keep << page_log2 <= 256);
+  p.few = G <= FEW_ROWS && (items >= (D == 256 ? 1024 : 512) || (D < 256 && keep << page_log2 <= 256));
   if (p.few) {
     p.tiles = (unsigned)(((keep << page_log2) + FEW_TILE - 1) / FEW_TILE);
     p.each = 0;
@@ -429,13 +440,8 @@ double paged_list_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t kee
 }
 
 template <typename S, int D> static void launch_list(const PagedAttnKernelArgs &a, bool few, dim3 grid, hipStream_t st) {
-  if constexpr (D <= 128) {
-    if (few) {
-      paged_list_few_kernel<S, D><<<grid, dim3(64 * FEW_WAVES), 0, st>>>(a);
-      return;
-    }
-  }
-  paged_rows_kernel<S, D, PagedListDeal, false><<<grid, dim3(256), 0, st>>>(a);
+  if (few) paged_list_few_kernel<S, D><<<grid, dim3(64 * FEW_WAVES), 0, st>>>(a);
+  else paged_rows_kernel<S, D, PagedListDeal, false><<<grid, dim3(256), 0, st>>>(a);
 }
 template <int D> static int launch_d(const PagedListArgs &l, hipStream_t st) {
   const PagedAttnArgs &x = l.x;

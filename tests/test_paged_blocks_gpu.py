@@ -109,7 +109,8 @@ def test_lists_as_they_may_come(qfa, keep):
 @pytest.mark.parametrize("B,H,Hk,N,D,page,keep,keys,dtype,scale_dtype", [
     (3, 8, 2, 90, 64, 16, 150, 2600, torch.float16, torch.float32), (2, 3, 1, 270, 128, 128, 19, 2500, torch.bfloat16, torch.float16),
     (1, 4, 4, 130, 128, 32, 5, 500, torch.float32, torch.bfloat16), (66, 20, 10, 1, 64, 64, 3, 700, torch.bfloat16, torch.float32),
-    (300, 2, 2, 1, 128, 16, 9, 333, torch.bfloat16, torch.float16)])
+    (300, 2, 2, 1, 128, 16, 9, 333, torch.bfloat16, torch.float16), (2, 6, 2, 260, 256, 64, 37, 2400, torch.float16, torch.float16),
+    (1, 2, 1, 1030, 256, 16, 7, 1100, torch.float32, torch.float32)])
 def test_many_lists(qfa, B, H, Hk, N, D, page, keep, keys, dtype, scale_dtype):
     p = lm.Problem(B, H, Hk, N, D, page, [max(N, keys - 37 * i) for i in range(B)], counts=[max(0, N - 3 * i) if N > 1 else 1 for i in range(B)], seed=H + N,
                    dtype=dtype, scale_dtype=scale_dtype)
