@@ -6,8 +6,11 @@
 // One pass over the keys (D + 3 bytes of each), no exchange between workgroups and no atomics: a wave holds 64 keys, all rows pass by, and a
 // key's sum is made in a fixed order.  Rows are the rows of the product and keys its columns, so a key's scale and zero point are one value
 // per lane and its sum is three lane exchanges for 64 keys.  Up to 16 rows are quantized in the workgroup and stay in registers while it
-// takes several times 256 keys; more are quantized once by a launch in front, and pass through LDS in panels of 64, the next one on its way while
-// one is worked on.
+// takes several times 256 keys; more are quantized once by a launch in front (up to 32 by every workgroup, where those are few), and pass
+// through LDS in panels of 64, the next one on its way while one is worked on.
+//
+// Bound by reading the keys: 64 sequences of 65 to 8192 keys, 8 key heads of 4 x 128, 16 keys a page: 71 us, 4.4 TB/s (floor at the 5 TB/s of a large copy: 62 us).
+// Many rows are bound by the vector pipe, seven instructions a score: 128 rows on 4 x 4000 to 8000 keys, 8 key heads of 128: 18.5 us beside 4.1 of the launch in front.
 #include "qfa_host.h"
 #include "qfa_quant_row.h"
 #include "qfa_skv_common.h"
@@ -20,6 +23,7 @@ struct WeighKernelArgs {
   float sm_scale_log2;
   const unsigned char *panels;   // many rows: those of every sequence and key head, ready to be copied to LDS
   int panels_each;
+  bool here;   // ... made by every workgroup itself
 };
 
 template <int D, int PR> struct __attribute__((aligned(16))) WeighPanel {
@@ -189,8 +193,14 @@ template <typename S, int D, bool ONE> __global__ __launch_bounds__(256, D == 25
     __syncthreads();
     rows_from(*reinterpret_cast<const Panel *>(smem), 0);
   } else {
-    fetch(0);
+    if (!p.here) fetch(0);
     load(keys, begin + 64 * wave, page);
+    if (p.here)
+      for (int r0 = 0; r0 < p.rows; r0 += 16) {
+        WeighRows<D> rows;
+        rows.load(p, b, h, r0);
+        rows.put(p, seq, *reinterpret_cast<Panel *>(smem), r0);
+      }
   }
 
   for (int step = 0; step < p.steps; ++step) {
@@ -295,7 +305,11 @@ template <typename S, int D> static int launch_sd(const PagedWeighArgs &w, hipSt
   const double quarters = (double)BH * p.panels_each * (WEIGH_PANEL / 16);
   if ((double)BH * p.chunks > 2147483647.0 || quarters > 2147483647.0 || (double)p.panels_each * (WEIGH_PANEL * (D + 20)) > 2147483647.0)
     return set_error(QFA_EUNSUPPORTED, "paged_weights: too many keys or rows for one launch");
-  if (!one) {
+  // Up to two blocks of rows are quantized by every workgroup itself where those are few: the launch in front costs more.  8 key heads, keys x sequences, us
+  // with the launch and without:  32 rows of 64 elements 512 x 1: 10.3, 6.4, 2048 x 16: 10.8, 9.2, 8192 x 16: 24.4, 31.1;  of 128 512 x 1: 8.7, 6.4, 32768 x 1: 13.3,
+  // 12.6, 8192 x 16: 31.4, 37.0;  of 256 512 x 1: 10.9, 9.2, 2048 x 16: 21.0, 23.8;  64 rows of 128 512 x 1: 9.4, 9.4, 8192 x 4: 15.7, 19.0
+  p.here = !one && p.rows <= 32 && BH * p.chunks <= (D == 256 ? 512 : 1024);
+  if (!one && !p.here) {
     weigh_rows_kernel<D><<<dim3((unsigned)quarters), dim3(256), 0, st>>>(p);
     if (int e = check_launch("qfa_paged_weights (rows)")) return e;
   }
