@@ -9,7 +9,7 @@
 // takes several times 256 keys; more are quantized once by a launch in front (up to 32 by every workgroup, where those are few), and pass
 // through LDS in panels of 64, the next one on its way while one is worked on.
 //
-// Bound by reading the keys: 64 sequences of 65 to 8192 keys, 8 key heads of 4 x 128, 16 keys a page: 71 us, 4.4 TB/s (floor at the 5 TB/s of a large copy: 62 us).
+// Bound by reading the keys: 64 sequences of 65 to 8192 keys, 8 key heads of 4 x 128, 16 keys a page: 64 us, 4.9 TB/s (floor at the 5 TB/s of a large copy: 62 us).
 // Many rows are bound by the vector pipe, seven instructions a score: 128 rows on 4 x 4000 to 8000 keys, 8 key heads of 128: 18.5 us beside 4.1 of the launch in front.
 #include "qfa_host.h"
 #include "qfa_quant_row.h"
@@ -105,12 +105,13 @@ template <int D> __global__ __launch_bounds__(256) void weigh_rows_kernel(WeighK
   rows.put(p, seq, reinterpret_cast<Panel *>(const_cast<unsigned char *>(p.panels))[bh * p.panels_each + r0 / WEIGH_PANEL], r0);
 }
 
-template <typename S, int D, bool ONE> __global__ __launch_bounds__(256, D == 256 ? 2 : ONE ? 5 : 4) void paged_weigh_kernel(WeighKernelArgs p) {
+template <typename S, int D, bool ONE, bool STREAM> __global__ __launch_bounds__(256, D == 256 ? 2 : ONE && !STREAM ? 5 : 4) void paged_weigh_kernel(WeighKernelArgs p) {
   constexpr int KM = D / 64, PR = ONE ? 16 : WEIGH_PANEL;
   typedef WeighPanel<D, PR> Panel;
   // many rows: two panels, each with room for whole copies of 1024 bytes
   constexpr int PIECES = (sizeof(Panel) + 1023) / 1024, BUF = ONE ? sizeof(Panel) : 1024 * PIECES;
   __shared__ __attribute__((aligned(16))) unsigned char smem[ONE ? BUF : 2 * BUF];
+  __shared__ __attribute__((aligned(16))) unsigned char held[STREAM ? 256 * D : 16];   // the keys of a step
   const PagedAttnArgs &x = p.w.x;
   const int tid = threadIdx.x, lane = tid % 64, c16 = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -154,6 +155,15 @@ template <typename S, int D, bool ONE> __global__ __launch_bounds__(256, D == 25
     float scale;
     int zero, there;   // there: bit per tile, its page exists
   };
+  // Keys that are not to stay in the caches (STREAM) are loaded into LDS as they lie, 16 bytes a lane, and read from there in the fragments'
+  // order: loaded in that order, two loads of 64 bytes share a line, which would be fetched twice.  Within a row the 16-byte parts are
+  // exchanged by its number, for the banks.
+  constexpr int PARTS = D / 16, PER_LINE = PARTS < 8 ? 8 / PARTS : 1, TURNS = PARTS < 8 ? PARTS : 8;   // (rows in 128 bytes)
+  auto k_at = [](int row, int part) __attribute__((always_inline)) -> int { return row * D + 16 * (part ^ (row / PER_LINE % TURNS)); };
+  unsigned char *kl = held + 64 * D * wave;
+  int k_off[4];   // (KM of them)
+#pragma unroll
+  for (int m = 0; m < KM; ++m) k_off[m] = k_at(m * (1024 / D) + lane / PARTS, lane % PARTS) - 1024 * m;
   const S *scales = static_cast<const S *>(x.cache.k_scale);
   auto page_of = [&](int key) __attribute__((always_inline)) -> int {
     const int at = key >> x.page_log2;
@@ -172,7 +182,9 @@ template <typename S, int D, bool ONE> __global__ __launch_bounds__(256, D == 25
       const int64_t first = (((int64_t)max(id_t, 0) * x.Hk + h) << x.page_log2) + ((key0 + 16 * i) & ((1 << x.page_log2) - 1));
       const rsrc_t rs = make_rsrc(x.cache.k_codes + first * D, id_t >= 0 ? 16 * D : 0);
 #pragma unroll
-      for (int m = 0; m < KM; ++m) t.k[i][m] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c16 * D + 16 * g, 64 * m, 0));
+      for (int m = 0; m < KM; ++m)
+        if constexpr (STREAM) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lptr_t)(kl + 16 * D * i + 1024 * m), 16, k_off[m], 1024 * m, 0, LOAD_ONCE);
+        else t.k[i][m] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c16 * D + 16 * g, 64 * m, 0));
     }
   };
   int page = page_of(begin + 64 * wave + lane);
@@ -211,8 +223,16 @@ template <typename S, int D, bool ONE> __global__ __launch_bounds__(256, D == 25
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     if (mine || !ONE) {   // (of one block of rows a wave that is past the last key stays so)
       if constexpr (ONE) {   // (many rows: one step, and its keys are on their way already)
+        if constexpr (STREAM) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the keys before are read)
         load(keys, key0, page);
         if (step + 1 < p.steps) page = page_of(key + 256);
+        if constexpr (STREAM) {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the keys are in LDS
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int m = 0; m < KM; ++m) keys.k[t][m] = *reinterpret_cast<const i32x4 *>(kl + 16 * D * t + k_at(c16, 4 * m + g));
+        }
       }
       i32x4 (&k)[4][KM] = keys.k;
       const int there = keys.there;
@@ -314,8 +334,13 @@ template <typename S, int D> static int launch_sd(const PagedWeighArgs &w, hipSt
     if (int e = check_launch("qfa_paged_weights (rows)")) return e;
   }
   const dim3 grid((unsigned)(BH * p.chunks)), block(256);
-  if (one) paged_weigh_kernel<S, D, true><<<grid, block, 0, st>>>(p);
-  else paged_weigh_kernel<S, D, false><<<grid, block, 0, st>>>(p);
+  // Keys that outgrow the last-level cache, with what else is read of it, are not to stay there.  One token, 32 sequences with 8 key heads, keys in MiB, us without
+  // and with:  64 elements 128: 32.4, 36.0, 256: 58.0, 63.5, 384: 100.9, 93.3, 1024: 265, 237;  128: 256: 49.8, 55.4, 384: 90.6, 82.0, 1024: 238, 215;  256: 256: 48.7,
+  // 54.6, 384: 83.2, 83.3, 1024: 217, 208.  (Non-temporal loads in the fragments' order: 64 sequences of 65 to 8192 keys 83 instead of 72 and, these, 64.)
+  const bool stream = one && (double)BH * (double)slots * D > 320.0 * (1 << 20);
+  if (stream) paged_weigh_kernel<S, D, true, true><<<grid, block, 0, st>>>(p);
+  else if (one) paged_weigh_kernel<S, D, true, false><<<grid, block, 0, st>>>(p);
+  else paged_weigh_kernel<S, D, false, false><<<grid, block, 0, st>>>(p);
   return check_launch("qfa_paged_weights");
 }
 template <typename S> static int launch_s(const PagedWeighArgs &w, hipStream_t st) {

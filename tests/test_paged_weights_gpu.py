@@ -58,6 +58,17 @@ def test_lengths(qfa, D, page, keys):
     _check(qfa, lm.Problem(4, 2, 2, 1, D, page, keys, seed=D + page))
 
 
+# a table so wide that keys are not to stay in the caches; pages of all sizes, rows that a block holds and does not
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,page,H,N,scale_dtype", [(64, 16, 2, 1, torch.float16), (128, 128, 8, 4, torch.float32), (128, 16, 6, 2, torch.bfloat16), (256, 32, 4, 3, torch.float16)])
+def test_wide_tables(qfa, D, page, H, N, scale_dtype):
+    p = lm.Problem(4, H, 2, N, D, page, [max(N, 1), 700, 257, 530], counts=[N, N, 0, 1], seed=D + page, scale_dtype=scale_dtype)
+    width = 330 * 2 ** 20 // (8 * D * page)
+    p.table = torch.cat([p.table, torch.full((4, width - p.width), -1, dtype=torch.int32)], 1)
+    p.width = width
+    _check(qfa, p)
+
+
 # rows that fill a block, do not, several blocks, several panels of 64
 @pytest.mark.gpu
 @pytest.mark.parametrize("H,Hk,N", [(8, 2, 1), (16, 1, 1), (6, 2, 3), (17, 1, 1), (40, 2, 1), (4, 4, 16), (3, 1, 17), (10, 2, 13), (2, 1, 65)])
