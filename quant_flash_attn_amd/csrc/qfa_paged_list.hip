@@ -3,6 +3,9 @@
 // with the arithmetic of attention on all keys (qfa_paged_attn.hip), and its kernel, or one for few rows.  A token and key head are an item: the query heads that
 // share the key head are its rows, the list's blocks one behind the other its keys.  A half of a tile lies in one block, so what the mask
 // asks is where each half's keys begin; the list is read beside the page numbers, 32 tiles ahead.
+//
+// Lists of one token each are bound by reading the cache, 64 sequences, 8 key heads of 4 x 128, 1024 keys of each, 134 MB in 29 us (4.6 TB/s), or by a start and a
+// few tiles that wait for each other: 8 x 5 tokens, 4 key heads of 4 x 256, 640 keys 15.3 us.
 #include "qfa_paged_block.h"
 
 namespace qfa {
@@ -17,8 +20,8 @@ constexpr int LIST_EXTRA = 12;      // units of an item beside its tiles, as the
 // as the waves do: two, so that an item costs little beside its tiles.  2 x 333 tokens, 8 key heads of 4 x 128, 2048 keys each, us: 179 against 278 of
 // paged_rows_kernel; of one block of 64 keys each 32 against 65.  With one wave to an item 180 and 20, with four 207; with one copy of the
 // rows to a workgroup's four waves and keys read in the fragments' order 278; the values through LDS as well 198.  Keys and values come from L2
-// (96 %): 2.9 GB, 16 TB/s.  No unit is busy more than two thirds of the time; 270 vector instructions of 64 keys and wave, 128 of
-// them the values' conversion, are the most of them.
+// (98 %): 2.9 GB, 16 TB/s.  The way from the L1 cache to registers is busy for 81 % of the time, its tags for 67 %, the vector pipe for 56 %, the matrix pipe
+// for 21 %: a tile takes 270 vector instructions, 128 of them the values' conversion.
 constexpr int FEW_ROWS = 4, FEW_TILE = 64, FEW_WAVES = 2;
 template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 256 ? 2 : 3) void paged_list_few_kernel(PagedAttnKernelArgs a) {
   constexpr int KM = D / 64, DB = D / 16, VB = D / 16, VD = VB / 4;   // as in paged_rows_kernel

@@ -10,6 +10,11 @@
 // come on top.
 //
 // Scores, then for every token and key head the `keep` best (qfa_topk.h), in one launch or two.
+//
+// Waits bound all of it, not the 2 (D + 5) bytes of a block: page number, bounds, the digits of a selection come one behind the other.  One token of 64 sequences
+// of 5 to 512 blocks, 8 key heads of 4 x 128, 34 MB: 18.2 us (2 TB/s), vector pipe 10 % busy; 333 tokens of 2 sequences of 219 blocks, 5 key heads of 4 x 64:
+// 15.8; one token of 2048 blocks: 6.0 and 8.2 for the selection.  Not faster: eight waves that take all blocks at once (22.8; with 128 registers each 32), bounds
+// brought in the order in which they lie and turned in LDS (17.6; 256 elements run out of registers).
 #include <cfloat>
 
 #include "qfa_host.h"
@@ -20,7 +25,8 @@
 namespace qfa {
 
 // ---------------------------------------------------------------------------------------------------------------- bounds
-// A wave takes a page and key head: D/16 lanes hold a row, each its minima and maxima of 16 elements, which meet at the end
+// A wave takes a page and key head: D/16 lanes hold a row, each its minima and maxima of 16 elements, which meet at the end.  A launch with its waits: one token of
+// 64 sequences, 8 key heads of 128, 16 rows a page 4.5 us, 64 rows 4.9
 template <typename S, int D> __global__ __launch_bounds__(256) void page_bounds_kernel(PagedSelectArgs a, int pages_each) {
   constexpr int LPR = D / 16, RPW = 64 / LPR;
   const int lane = threadIdx.x % 64, sub = lane % LPR, rg = lane / LPR;
