@@ -67,7 +67,7 @@ template <int T, int N, int BITS> struct TopHeld {
   static_assert(BINS % T == 0, "every thread owns some of the digit's values");
   float held[N > 0 ? N : 1];
   unsigned count[BINS];
-  unsigned sums[2][WAVES];
+  unsigned sums[3][WAVES];
   unsigned found[3];
 
   // number(i) of places i = 0 .. n - 1, n <= N, its key(i, x); take(place among the taken ones, i, x) for the k largest of those whose key is not 0 (of
@@ -139,26 +139,31 @@ template <int T, int N, int BITS> struct TopHeld {
       }
     }
     // ---- their places
-    unsigned mine = 0;
+    unsigned mine_gt = 0, mine_eq = 0;   // (each its own count: there may be more than 2^16 of both)
 #pragma unroll AT_ONCE
     for (int i = i0; i < i1; i += 64) {
       const unsigned u = key_of(i, again(i));
-      mine += (u > at ? 1u << 16 : 0u) + (((u == at) & (at != 0)) ? 1u : 0u);
+      mine_gt += u > at ? 1u : 0u;
+      mine_eq += ((u == at) & (at != 0)) ? 1u : 0u;
     }
-    const unsigned of_wave = __builtin_amdgcn_readlane((int)wave_scan(mine), 63);
-    unsigned before = 0, total = of_wave;
+    const unsigned wave_gt = __builtin_amdgcn_readlane((int)wave_scan(mine_gt), 63), wave_eq = __builtin_amdgcn_readlane((int)wave_scan(mine_eq), 63);
+    unsigned gt = 0, eq = 0, total_gt = wave_gt, total_eq = wave_eq;
     if constexpr (WAVES > 1) {
-      if (lane == 0) sums[1][wave] = of_wave;
+      if (lane == 0) {
+        sums[1][wave] = wave_gt;
+        sums[2][wave] = wave_eq;
+      }
       __syncthreads();
-      total = 0;
+      total_gt = total_eq = 0;
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
-        const unsigned c = sums[1][w];
-        before += w < wave ? c : 0u;
-        total += c;
+        const unsigned g = sums[1][w], e = sums[2][w];
+        gt += w < wave ? g : 0u;
+        eq += w < wave ? e : 0u;
+        total_gt += g;
+        total_eq += e;
       }
     }
-    unsigned gt = before >> 16, eq = before & 0xffffu;
     const uint64_t lower = (1ull << lane) - 1;
     for (int first = i0 - lane; first < i1; first += 64 * AT_ONCE) {   // (some steps at once, of all lanes: one by one each would wait for its numbers)
       float x[AT_ONCE];
@@ -177,7 +182,7 @@ template <int T, int N, int BITS> struct TopHeld {
         eq += (unsigned)__builtin_popcountll(all_eq);
       }
     }
-    return (total >> 16) + min(total & 0xffffu, equal);
+    return total_gt + min(total_eq, equal);
   }
 };
 

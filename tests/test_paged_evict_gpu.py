@@ -78,6 +78,16 @@ def test_many_slots(qfa, keep):
     _check(qfa, 1, 2, 64, 128, [9001], keep, first=min(3, keep), last=min(100, keep - min(3, keep)), seed=keep)
 
 
+# more slots than are brought to LDS, and more than 2^16 that are taken, that are equal, that are both
+@pytest.mark.gpu
+@pytest.mark.parametrize("length,keep,values", [(20011, 700, None), (140001, 70007, None), (140001, 70007, [0.0]), (140001, 3, [0.0]), (140001, 139000, [0.0, 1.0])])
+def test_more_slots_than_are_held(qfa, length, keep, values):
+    w = None
+    if values:
+        w = torch.tensor(values)[torch.randint(0, len(values), (1, 1, -(-length // 1024) * 1024), generator=torch.Generator().manual_seed(keep))]
+    _check(qfa, 1, 1, 64, 1024, [length], keep, first=1, last=2, weights=w, seed=keep)
+
+
 @pytest.mark.gpu
 def test_ties_and_odd_weights(qfa):
     """Equal weights go to the lowest slots; -0 equals 0; infinities are the ends, NaN lies below them; subnormals are told apart."""

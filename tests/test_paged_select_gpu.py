@@ -155,6 +155,31 @@ def test_long_tables(qfa, width):
         assert blocks[b, 0, 0].tolist() == lm.select(one, list(range(mine + 1)), mine, keep, 1, 1)
 
 
+# more blocks than are brought to LDS, most of them equal to many others, and more than 2^16 of them taken
+@pytest.mark.gpu
+@pytest.mark.parametrize("width,keep,pages", [(17001, 64, 40), (140003, 70001, 40), (140003, 5, 2), (140003, 139999, 2)])
+def test_more_blocks_than_are_held(qfa, width, keep, pages):
+    g = torch.Generator().manual_seed(width + keep)
+    page, D = 16, 64
+    q = torch.randn(1, 2, 1, D, generator=g).bfloat16()
+    cache = qfa.make_paged_cache(pages, 1, page, D, device=DEV)
+    rows = torch.randn(1, 1, pages * page, D, generator=g).to(DEV)
+    own = torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    qfa.paged_cache_append(cache, rows, rows, own, zero)
+    bounds = qfa.make_page_bounds(cache)
+    qfa.paged_bounds_update(bounds, cache, own, zero, pages * page)
+    pick = torch.randint(0, pages, (width,), generator=g)
+    starts = torch.tensor([width * page - 9], dtype=torch.int32, device=DEV)
+    blocks, scores = qfa.paged_select_blocks(q.to(DEV), cache, bounds, pick.int()[None].to(DEV), starts, keep, last=2, return_scores=True)
+    c, s, z = (t.cpu() for t in bounds)
+    one = lm.scores_of(q[0, :, 0], (c[:, 0], s[:, 0], z[:, 0]))[pick]
+    assert torch.equal(scores[0, 0, 0].cpu(), one)
+    rank = one.clone()
+    rank[0] = rank[-2:] = float("inf")
+    assert torch.equal(blocks[0, 0, 0].cpu(), rank.argsort(descending=True, stable=True)[:keep].sort().values.int())
+
+
 @pytest.mark.gpu
 def test_token_by_token(qfa):
     """Bounds kept up to date behind every append are those of the whole prompt; pages that a call does not touch stay."""
