@@ -310,7 +310,7 @@ int qfa_paged_select(const qfa_paged_cache *cache, const qfa_page_bounds *bounds
 
 int64_t qfa_attn_paged_blocks_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t keep, int page_size) {
   if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || N <= 0 || !head_dim_ok(D) || !keep_ok(keep) || !page_size_ok(page_size)) return 0;
-  if (paged_list_units(B, H, Hk, N, keep, log2_of(page_size)) > 2147483647.0) return 0;
+  if (keep > (1LL << 30) / page_size || paged_list_units(B, H, Hk, N, keep, log2_of(page_size)) > 2147483647.0) return 0;
   return paged_list_workspace_bytes(B, H, Hk, N, D, keep, log2_of(page_size));
 }
 
@@ -324,6 +324,7 @@ int qfa_attn_paged_blocks(const qfa_paged_cache *cache, const void *q, int q_dty
   if (!aligned16(o)) return set_error(QFA_EINVAL, "%s: q and o must be 16-byte aligned", who);
   if (int e = check_scale(who, sm_scale)) return e;
   if (int e = check_keep(who, keep, 0, 0)) return e;
+  if (keep > (1LL << 30) / cache->page_size) return set_error(QFA_EUNSUPPORTED, "%s: a list has room for 2^30 keys at most", who);
   if (paged_list_units(B, H, cache->H, N, keep, a.x.page_log2) > 2147483647.0)
     return set_error(QFA_EUNSUPPORTED, "%s: too many tokens times the keys of their lists for one call", who);
   if (int e = check_workspace(who, "qfa_attn_paged_blocks_workspace_bytes", workspace, workspace_bytes,

@@ -279,3 +279,13 @@ def test_argument_errors_need_no_gpu(qfa):
         assert rc == code, L.qfa_last_error()
     ws = L.qfa_attn_paged_blocks_workspace_bytes
     assert ws(1, 4, 2, 1, 128, 1 << 20, 16) > 0 and ws(1, 4, 3, 1, 128, 8, 16) == 0 and ws(1, 4, 2, 1, 128, 8, 24) == 0 and ws(1, 4, 2, 1, 128, 0, 16) == 0
+
+
+def test_lists_of_too_many_keys_need_no_gpu(qfa):
+    """The keys of a list are counted in 31 bits."""
+    from quant_flash_attn_amd import _lib
+    L, P = _lib.lib(), 0x1000
+    for page, keep in ((16, (1 << 26) + 1), (16, 1 << 28), (1 << 20, 1025)):
+        c = _lib.PagedCacheStruct(k_codes=P, k_scale=P, k_zero=P, v_codes=P, v_scale=P, v_zero=P, pages=4, H=1, page_size=page, D=64, scale_dtype=1)
+        assert L.qfa_attn_paged_blocks(ctypes.byref(c), P, 2, 64, 64, 64, P, 4, 4, 1, P, None, P, keep, P, 1, 1, 1, 0.1, P, 1 << 40, None) == -2
+        assert L.qfa_attn_paged_blocks_workspace_bytes(1, 1, 1, 1, 64, keep, page) == 0
