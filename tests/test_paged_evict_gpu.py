@@ -245,6 +245,19 @@ def test_a_serving_loop(qfa):
     assert ((weights.double().sum(-1)[:, :, None] > 2 * steps) & (weights.double().sum(-1)[:, :, None] < 2 * total)).all()
 
 
+@pytest.mark.gpu
+def test_weights_that_want_a_gradient(qfa):
+    cache = dev(_cache(12, 2, 16, 64, torch.float16, 3))
+    table, new = torch.arange(8, dtype=torch.int32, device=DEV).view(2, 4), torch.arange(8, 12, dtype=torch.int32, device=DEV).view(2, 2)
+    n, w = torch.tensor([60, 30], dtype=torch.int32, device=DEV), torch.rand(2, 2, 64, device=DEV).requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        qfa.paged_cache_evict(cache, table, n, w, 20, new)
+    with torch.no_grad():
+        first = qfa.paged_cache_evict(cache, table, n, w, 20, new)
+    for a, b in zip(first, qfa.paged_cache_evict(cache, table, n, w.detach(), 20, new)):
+        assert torch.equal(a, b) and not a.requires_grad
+
+
 def test_argument_errors_need_no_gpu(qfa):
     from quant_flash_attn_amd import _lib
     L, P = _lib.lib(), 0x1000
