@@ -17,14 +17,18 @@ constexpr int LIST_EXTRA = 12;      // units of an item beside its tiles, as the
 // works as long as for real ones.  So the columns are the four rows four times over, and of a tile of 64 keys every copy takes 16 and
 // is a softmax of its own: the score products add up in one accumulator, each 16 keys' with the queries of their copy and zeros elsewhere,
 // and a lane has four scores of 64 keys in place of eight of 32.  The probabilities enter the P.V product likewise.  The copies meet at the end,
-// as the waves do: two, so that an item costs little beside its tiles.  2 x 333 tokens, 8 key heads of 4 x 128, 2048 keys each, us: 179 against 278 of
-// paged_rows_kernel; of one block of 64 keys each 32 against 65.  With one wave to an item 180 and 20, with four 207; with one copy of the
-// rows to a workgroup's four waves and keys read in the fragments' order 278; the values through LDS as well 198.  Keys and values come from L2
-// (98 %): 2.9 GB, 16 TB/s.  The way from the L1 cache to registers is busy for 81 % of the time, its tags for 67 %, the vector pipe for 56 %, the matrix pipe
-// for 21 %: a tile takes 270 vector instructions, 128 of them the values' conversion.
+// as the waves do: two, so that an item costs little beside its tiles.  A value's bytes, offset by 128, are binary16 numbers of 2^-24 each as they stand.
+// 2 x 333 tokens, 8 key heads of 4 x 128, 2048 keys each, us: 168 against 278 of paged_rows_kernel; of one block of 64 keys each 31 against 65.  With one wave to an item
+// 180 and 20 instead of 179 and 32, with four 207; before, keys in the fragments' order, one copy of the rows to four waves 278; values in the products' order,
+// 8 bytes a lane 179, through LDS 198, 16 bytes a lane 171 (two workgroups less on a CU 197); offset by 1152 in place of 128, another instruction for two
+// values, 171.  Keys and values come from L2 (99 %): 2.9 GB, 17 TB/s.  The way from the L1 cache to registers is busy for 76 % of the time, its tags for 52 %, the
+// vector pipe for 60 %, the matrix pipe for 24 %: a tile takes 240 vector instructions, 96 of them the values' conversion.
 constexpr int FEW_ROWS = 4, FEW_TILE = 64, FEW_WAVES = 2;
 template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 256 ? 2 : 3) void paged_list_few_kernel(PagedAttnKernelArgs a) {
-  constexpr int KM = D / 64, DB = D / 16, VB = D / 16, VD = VB / 4;   // as in paged_rows_kernel
+  constexpr int KM = D / 64;
+  // A lane holds 16 bytes of a value: D / 16 lanes of 16 have a row, so that the 16 rows of the products' first operand are PARTS times the elements,
+  // each part of keys of its own: those of copies part * 4 / PARTS and on.  What a part's rows sum up for the other copies is not looked at
+  constexpr int PARTS = 256 / D, VE = 16 / PARTS, VH = D == 256 ? 2 : 1;   // loads of a tile, products
   constexpr int LPT = D / 8;
   constexpr int OFF_ONES = (FEW_ROWS + 1) * D, OFF_ST = OFF_ONES + 16, OFF_TC = OFF_ST + 3 * 16;   // (query codes; D bytes of zeros; ones)
   constexpr int TC = 512 + 512 + 256;   // [64] x (scale, zero point operand) of keys, of values, exponents of the values' scales
@@ -41,20 +45,20 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
 
   unsigned char *smem = all + wave * EACH;
   struct Tile {
-    unsigned v[16][VD];
+    u32x4 v[VE];
     unsigned ks, kz, vs, vz;   // scale (its bits) and zero point of key lane and value lane
     int ok, key[4];            // bit per 16 keys: their page exists; the position of the first of them
   };
-  const int v_off = 4 * G * D + VB * q16;
+  const int part = q16 / (16 / PARTS), v_off = 4 * G * D + 16 * (q16 % (16 / PARTS));
   // Keys are loaded into LDS as they lie, 16 bytes a lane, and read from there in the fragments' order: loaded in that order,
   // neighbouring lanes' bytes are of different rows, and each lane is an access of its own to the L1 cache.  Within a row the 16-byte
   // parts are exchanged by its number, for the banks.
-  constexpr int PARTS = D / 16, PER_LINE = PARTS < 8 ? 8 / PARTS : 1, TURNS = PARTS < 8 ? PARTS : 8;   // (rows in 128 bytes)
+  constexpr int CHUNKS = D / 16, PER_LINE = CHUNKS < 8 ? 8 / CHUNKS : 1, TURNS = CHUNKS < 8 ? CHUNKS : 8;   // (rows in 128 bytes)
   auto k_at = [](int row, int part) __attribute__((always_inline)) -> int { return row * D + 16 * (part ^ (row / PER_LINE % TURNS)); };
   unsigned char *kl = smem + OFF_K;
   int k_off[4];   // (KM of them)
 #pragma unroll
-  for (int m = 0; m < KM; ++m) k_off[m] = k_at(m * (1024 / D) + lane / PARTS, lane % PARTS) - 1024 * m;
+  for (int m = 0; m < KM; ++m) k_off[m] = k_at(m * (1024 / D) + lane / CHUNKS, lane % CHUNKS) - 1024 * m;
   const int page_parts_log2 = a.page_log2 - 4;
   unsigned *tc = reinterpret_cast<unsigned *>(smem + OFF_TC);
   const int32_t *list = a.blocks + (((int64_t)token.b * a.work.Hk + item.h) * a.work.N + token.i) * a.keep;
@@ -106,24 +110,17 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
       for (int m = 0; m < KM; ++m) __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lptr_t)(kl + 16 * D * g + 1024 * m), 16, k_off[m], 1024 * m, 0, 0);
     }
   };
-  auto load_values = [&](Tile &t) __attribute__((always_inline)) {
+  auto load_values = [&](Tile &t) __attribute__((always_inline)) {   // (of a page that is not there those of another; they count for nothing)
+    const unsigned f0 = first[0], f1 = first[1], f2 = first[2], f3 = first[3];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const rsrc_t rv = make_rsrc(a.vc + (int64_t)first[g] * D, t.ok >> g & 1 ? 16 * D : 0);
+    for (int y = 0; y < VE / 4; ++y) {
+      unsigned at;
+      if constexpr (PARTS == 1) at = first[y];
+      else if constexpr (PARTS == 2) at = y == 0 ? (part == 0 ? f0 : f2) : (part == 0 ? f1 : f3);
+      else at = part < 2 ? (part == 0 ? f0 : f1) : (part == 2 ? f2 : f3);
+      const int8_t *from = a.vc + (int64_t)at * D + v_off;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (VD == 4) {
-          const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, v_off, e * D, 0));
-#pragma unroll
-          for (int y = 0; y < 4; ++y) t.v[4 * g + e][y] = w[y];
-        } else if constexpr (VD == 2) {
-          const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rv, v_off, e * D, 0));
-          t.v[4 * g + e][0] = w[0];
-          t.v[4 * g + e][1] = w[1];
-        } else {
-          t.v[4 * g + e][0] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(rv, v_off, e * D, 0);
-        }
-      }
+      for (int e = 0; e < 4; ++e) t.v[4 * y + e] = *reinterpret_cast<const u32x4 *>(from + e * D);
     }
   };
 
@@ -171,9 +168,9 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
   const float a_i = st_a[row_of];
   const int zq = st_z[row_of], c_i = st_c[row_of];
 
-  f32x4 oacc[DB];
+  f32x4 oacc[16];
 #pragma unroll
-  for (int i = 0; i < DB; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < 16; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float ref = NO_KEY, l_run = 0.f, w_run = 0.f;   // p = 2^(a_i * u - ref)
 
   auto tile = [&](Tile &t, int i) __attribute__((always_inline)) {
@@ -183,13 +180,13 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
       w[1] = (unsigned)(int)(signed char)t.kz;
       *reinterpret_cast<u32x2 *>(tc + 2 * lane) = w;
       w[0] = __builtin_bit_cast(unsigned, scale_to_f32<S>(t.vs));
-      w[1] = 0x6400u | (t.vz ^ 0x80u);   // the binary16 number 1152 + zero point
+      w[1] = (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(unsigned short)(t.vz ^ 0x80u));   // the binary16 number 128 + zero point
       *reinterpret_cast<u32x2 *>(tc + 128 + 2 * lane) = w;
     }
     const int mine = 16 * copy + 4 * G;   // this lane's first key
-    // The keys are in LDS once no more than the 16 loads of values behind them are on their way.  (The compiler moves no load
+    // The keys are in LDS once no more than the loads of values behind them are on their way.  (The compiler moves no load
     // across a statement like this; a register that it spilled would be counted too: the build looks for scratch.)
-    asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VE) : "memory");
     i32x4 s = {0, 0, 0, 0}, rk = {0, 0, 0, 0};
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -263,31 +260,42 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
       l_run *= alpha;
       w_run *= alpha;
 #pragma unroll
-      for (int j = 0; j < DB; ++j)
+      for (int j = 0; j < 16; ++j)
 #pragma unroll
         for (int v = 0; v < 4; ++v) oacc[j][v] *= alpha;
       probs();
     }
     l_run = l_new;
     // ---- p' as binary16, offset term
-    u32x4 pf[2];
+    u32x4 pf[VH];
+#pragma unroll
+    for (int h = 0; h < VH; ++h) pf[h] = u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       const unsigned pp = pack_h2(ps[2 * y], ps[2 * y + 1]), zz = cv[y][1] | (cv[y][3] << 16);
       w_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pp), __builtin_bit_cast(f16x2, zz), w_run, false);
+      if constexpr (PARTS == 4) {
+        pf[0][y] = pp;
+      } else {
 #pragma unroll
-      for (int g = 0; g < 4; ++g) pf[g / 2][2 * (g % 2) + y] = copy == g ? pp : 0u;
+        for (int g = 0; g < 2 * VH; ++g) pf[g / 2][2 * (g % 2) + y] = copy % (2 * VH) == g ? pp : 0u;
+      }
     }
-    // ---- O^T += (1152 + codes)^T . P'^T
+    // ---- O^T += (128 + codes)^T . P'^T, the former as the binary16 numbers 2^-24 (128 + code), which are their bytes
 #pragma unroll
-    for (int j = 0; j < DB; ++j)
+    for (int e = 0; e < VE; ++e)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32x4 vf;
+      for (int y = 0; y < 4; ++y) t.v[e][y] ^= 0x80808080u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int h = 0; h < VH; ++h) {
+        u32x4 vf = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < (PARTS == 4 ? 2 : 4); ++e) {
           constexpr unsigned pick = 0x0c040c00u;
-          vf[e] = __builtin_amdgcn_perm(t.v[8 * h + 2 * e + 1][j / 4], t.v[8 * h + 2 * e][j / 4], pick + (unsigned)(j % 4) * 0x00010001u) ^ 0x64806480u;
+          const unsigned lo = t.v[8 * h + 2 * e][j / 4], hi = t.v[8 * h + 2 * e + 1][j / 4];
+          vf[e] = __builtin_amdgcn_perm(hi, lo, pick + (unsigned)(j % 4) * 0x00010001u);
         }
         oacc[j] = mfma_h16(vf, pf[h], oacc[j]);
       }
@@ -305,15 +313,17 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
   float *mg = reinterpret_cast<float *>(smem + OFF_K), *ml = reinterpret_cast<float *>(tc);
   {
     float *dst = mg + q16 * D;
+    if (4 * G / (16 / PARTS) == copy * PARTS / 4) {   // (this lane's four rows are one part's)
 #pragma unroll
-    for (int v = 0; v < 4; ++v)
+      for (int v = 0; v < 4; ++v)
 #pragma unroll
-      for (int j = 0; j < DB; j += 4) {
-        f32x4 y;
+        for (int j = 0; j < 16; j += 4) {
+          f32x4 y;
 #pragma unroll
-        for (int z = 0; z < 4; ++z) y[z] = oacc[j + z][v] - w_tot;
-        *reinterpret_cast<f32x4 *>(dst + VB * (4 * G + v) + j) = y;
-      }
+          for (int z = 0; z < 4; ++z) y[z] = __builtin_fmaf(oacc[j + z][v], 0x1p24f, -w_tot);
+          *reinterpret_cast<f32x4 *>(dst + 16 * ((4 * G + v) % (16 / PARTS)) + j) = y;
+        }
+    }
     if (G == 0) {
       ml[2 * q16] = ref;
       ml[2 * q16 + 1] = l_tot;
