@@ -558,7 +558,8 @@ int qfa_paged_select(const qfa_paged_cache *cache, const qfa_page_bounds *bounds
 /*
  * qfa_attn_paged (causal) on listed blocks: token n of sequence b and the query heads of key head h see the keys j <= starts[b] + n of the blocks
  * in blocks[b,h,n,:] (int32, dense), in any order; a block that stands there twice counts twice, numbers outside [0, width) and blocks without a page
- * are passed over.  Rows that see no key get zeros.  keep * page_size: 2^30 at most.
+ * are passed over.  Rows that see no key get zeros.  keep * page_size: 2^30 at most.  q in fp32: probabilities times scales are held in two binary16 parts,
+ * so that no rounding is coarser than 2^-22.
  *   workspace  qfa_attn_paged_blocks_workspace_bytes(...) bytes (possibly 0), 16-byte aligned, contents irrelevant; one for each call under way
  * A call repeated gives the same bits; the last bits of a row depend on B, N, H and keep, not on the other sequences.
  */

@@ -16,7 +16,19 @@ constexpr int PAGED_WGS = 256 * 2;   // two on a CU
 __device__ __forceinline__ i32x4 paged_mfma_i8(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
 // Deal: how the work is dealt -- PagedDeal, every sequence's keys from a place on, or PagedListDeal, those of listed blocks
-template <typename S, int D, typename Deal, bool STREAM> __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnKernelArgs a) {
+// the binary16 number of a small whole number; 1152 less than two of them; what two numbers have beside their binary16 parts, as such parts
+__device__ __forceinline__ unsigned half_of(int x) { return (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(short)x); }
+__device__ __forceinline__ unsigned without_offset(unsigned two) {
+  const f16x2 x = __builtin_bit_cast(f16x2, two), offset = {(_Float16)1152.f, (_Float16)1152.f};
+  return __builtin_bit_cast(unsigned, x - offset);
+}
+__device__ __forceinline__ unsigned rest_h2(float x, float y, unsigned parts) {
+  const f16x2 p = __builtin_bit_cast(f16x2, parts);
+  return pack_h2(x - (float)p[0], y - (float)p[1]);
+}
+
+// FINE: p' in two binary16 parts, 22 bits, and codes without an offset, for queries in fp32 on lists: one part is 2^-11 off, and the offset takes 10 bits of the sums
+template <typename S, int D, typename Deal, bool STREAM, bool FINE = false> __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnKernelArgs a) {
   constexpr bool SHARED = Deal::ONE_PROBLEM, LIST = Deal::LIST;
   constexpr int KM = D / 64;    // 64-wide k-steps of the score product
   constexpr int DB = D / 16;    // 16-row blocks of O^T
@@ -214,7 +226,7 @@ template <typename S, int D, typename Deal, bool STREAM> __global__ __launch_bou
       {
         u32x2 w;
         w[0] = __builtin_bit_cast(unsigned, scale_to_f32<S>(t.sc));
-        w[1] = lane < 32 ? (unsigned)(int)(signed char)t.zp : (0x6400u | (t.zp ^ 0x80u));
+        w[1] = lane < 32 ? (unsigned)(int)(signed char)t.zp : FINE ? half_of((int)(signed char)t.zp) : (0x6400u | (t.zp ^ 0x80u));
         *reinterpret_cast<u32x2 *>(tc + 2 * lane) = w;
       }
       // ---- scores of keys 16rb + 4G + v
@@ -311,12 +323,17 @@ template <typename S, int D, typename Deal, bool STREAM> __global__ __launch_bou
       }
       l_run = l_new;
       // ---- p' as binary16, offset term
-      u32x4 pf;
+      u32x4 pf, pl;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const unsigned pp = pack_h2(ps[2 * y], ps[2 * y + 1]);
         pf[y] = pp;
         w_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pp), __builtin_bit_cast(f16x2, zz[y]), w_run, false);
+        if constexpr (FINE) {
+          const unsigned rest = rest_h2(ps[2 * y], ps[2 * y + 1], pp);   // (a bit cast of a vector's element takes element 0)
+          pl[y] = rest;
+          w_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, rest), __builtin_bit_cast(f16x2, zz[y]), w_run, false);
+        }
       }
       // ---- O^T += (1152 + codes)^T . P'^T
 #pragma unroll
@@ -326,8 +343,10 @@ template <typename S, int D, typename Deal, bool STREAM> __global__ __launch_bou
         for (int e = 0; e < 4; ++e) {
           constexpr unsigned pick = 0x0c040c00u;
           vf[e] = __builtin_amdgcn_perm(t.v[2 * e + 1][j / 4], t.v[2 * e][j / 4], pick + (unsigned)(j % 4) * 0x00010001u) ^ 0x64806480u;
+          if constexpr (FINE) vf[e] = without_offset(vf[e]);
         }
         oacc[j] = mfma_h16(vf, pf, oacc[j]);
+        if constexpr (FINE) oacc[j] = mfma_h16(vf, pl, oacc[j]);
       }
     };
     // Rows of 256 elements: two tiles in registers would leave room for one workgroup on a CU (1 to 12 % slower); a tile's keys and values

@@ -24,7 +24,7 @@ constexpr int LIST_EXTRA = 12;      // units of an item beside its tiles, as the
 // values, 171.  Keys and values come from L2 (99 %): 2.9 GB, 17 TB/s.  The way from the L1 cache to registers is busy for 76 % of the time, its tags for 52 %, the
 // vector pipe for 60 %, the matrix pipe for 24 %: a tile takes 240 vector instructions, 96 of them the values' conversion.
 constexpr int FEW_ROWS = 4, FEW_TILE = 64, FEW_WAVES = 2;
-template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 256 ? 2 : 3) void paged_list_few_kernel(PagedAttnKernelArgs a) {
+template <typename S, int D, bool FINE> __global__ __launch_bounds__(64 * FEW_WAVES, D == 256 ? 2 : 3) void paged_list_few_kernel(PagedAttnKernelArgs a) {
   constexpr int KM = D / 64;
   // A lane holds 16 bytes of a value: D / 16 lanes of 16 have a row, so that the 16 rows of the products' first operand are PARTS times the elements,
   // each part of keys of its own: those of copies part * 4 / PARTS and on.  What a part's rows sum up for the other copies is not looked at
@@ -180,7 +180,7 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
       w[1] = (unsigned)(int)(signed char)t.kz;
       *reinterpret_cast<u32x2 *>(tc + 2 * lane) = w;
       w[0] = __builtin_bit_cast(unsigned, scale_to_f32<S>(t.vs));
-      w[1] = (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(unsigned short)(t.vz ^ 0x80u));   // the binary16 number 128 + zero point
+      w[1] = FINE ? half_of((int)(signed char)t.vz) : half_of((int)(t.vz ^ 0x80u));   // the binary16 number of the zero point (or of 128 + it)
       *reinterpret_cast<u32x2 *>(tc + 128 + 2 * lane) = w;
     }
     const int mine = 16 * copy + 4 * G;   // this lane's first key
@@ -267,23 +267,32 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
     }
     l_run = l_new;
     // ---- p' as binary16, offset term
-    u32x4 pf[VH];
+    u32x4 pf[VH], pl[VH];
 #pragma unroll
-    for (int h = 0; h < VH; ++h) pf[h] = u32x4{0, 0, 0, 0};
+    for (int h = 0; h < VH; ++h) pf[h] = pl[h] = u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
       const unsigned pp = pack_h2(ps[2 * y], ps[2 * y + 1]), zz = cv[y][1] | (cv[y][3] << 16);
       w_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pp), __builtin_bit_cast(f16x2, zz), w_run, false);
+      unsigned rest = 0;
+      if constexpr (FINE) {
+        rest = rest_h2(ps[2 * y], ps[2 * y + 1], pp);
+        w_run = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, rest), __builtin_bit_cast(f16x2, zz), w_run, false);
+      }
       if constexpr (PARTS == 4) {
         pf[0][y] = pp;
+        pl[0][y] = rest;
       } else {
 #pragma unroll
-        for (int g = 0; g < 2 * VH; ++g) pf[g / 2][2 * (g % 2) + y] = copy % (2 * VH) == g ? pp : 0u;
+        for (int g = 0; g < 2 * VH; ++g) {
+          pf[g / 2][2 * (g % 2) + y] = copy % (2 * VH) == g ? pp : 0u;
+          pl[g / 2][2 * (g % 2) + y] = copy % (2 * VH) == g ? rest : 0u;
+        }
       }
     }
-    // ---- O^T += (128 + codes)^T . P'^T, the former as the binary16 numbers 2^-24 (128 + code), which are their bytes
+    // ---- O^T += (128 + codes)^T . P'^T, the former as the binary16 numbers 2^-24 (128 + code), which are their bytes (FINE: codes^T . P'^T)
 #pragma unroll
-    for (int e = 0; e < VE; ++e)
+    for (int e = 0; e < VE && !FINE; ++e)
 #pragma unroll
       for (int y = 0; y < 4; ++y) t.v[e][y] ^= 0x80808080u;
 #pragma unroll
@@ -296,8 +305,10 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
           constexpr unsigned pick = 0x0c040c00u;
           const unsigned lo = t.v[8 * h + 2 * e][j / 4], hi = t.v[8 * h + 2 * e + 1][j / 4];
           vf[e] = __builtin_amdgcn_perm(hi, lo, pick + (unsigned)(j % 4) * 0x00010001u);
+          if constexpr (FINE) vf[e] = without_offset(vf[e] ^ 0x64806480u);
         }
         oacc[j] = mfma_h16(vf, pf[h], oacc[j]);
+        if constexpr (FINE) oacc[j] = mfma_h16(vf, pl[h], oacc[j]);
       }
     asm volatile("" ::: "memory");
     load_values(t);
@@ -320,7 +331,7 @@ template <typename S, int D> __global__ __launch_bounds__(64 * FEW_WAVES, D == 2
         for (int j = 0; j < 16; j += 4) {
           f32x4 y;
 #pragma unroll
-          for (int z = 0; z < 4; ++z) y[z] = __builtin_fmaf(oacc[j + z][v], 0x1p24f, -w_tot);
+          for (int z = 0; z < 4; ++z) y[z] = __builtin_fmaf(oacc[j + z][v], FINE ? 1.0f : 0x1p24f, -w_tot);
           *reinterpret_cast<f32x4 *>(dst + 16 * ((4 * G + v) % (16 / PARTS)) + j) = y;
         }
     }
@@ -453,8 +464,11 @@ double paged_list_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t kee
 }
 
 template <typename S, int D> static void launch_list(const PagedAttnKernelArgs &a, bool few, dim3 grid, hipStream_t st) {
-  if (few) paged_list_few_kernel<S, D><<<grid, dim3(64 * FEW_WAVES), 0, st>>>(a);
-  else paged_rows_kernel<S, D, PagedListDeal, false><<<grid, dim3(256), 0, st>>>(a);
+  const bool fine = a.q_dtype == QFA_F32;
+  if (few && fine) paged_list_few_kernel<S, D, true><<<grid, dim3(64 * FEW_WAVES), 0, st>>>(a);
+  else if (few) paged_list_few_kernel<S, D, false><<<grid, dim3(64 * FEW_WAVES), 0, st>>>(a);
+  else if (fine) paged_rows_kernel<S, D, PagedListDeal, false, true><<<grid, dim3(256), 0, st>>>(a);
+  else paged_rows_kernel<S, D, PagedListDeal, false, false><<<grid, dim3(256), 0, st>>>(a);
 }
 template <int D> static int launch_d(const PagedListArgs &l, hipStream_t st) {
   const PagedAttnArgs &x = l.x;

@@ -66,7 +66,7 @@ def paged_select_blocks(q: torch.Tensor, cache, bounds, page_table: torch.Tensor
 def quant_flash_attn_paged_blocks(q: torch.Tensor, cache, page_table: torch.Tensor, starts: torch.Tensor, blocks: torch.Tensor,
                                   counts: Optional[torch.Tensor] = None, sm_scale: Optional[float] = None) -> torch.Tensor:
     """quant_flash_attn_paged (causal) of every token on its own list of blocks, int32 [B,heads,N,keep]: O [B,H,N,D] of q's type, the same
-    arithmetic.  No gradient.
+    arithmetic (of fp32 queries without its 16-bit rounding of probabilities).  No gradient.
 
     A token sees the keys up to itself in the blocks of its list.  The order of a list does not matter, a block that stands in it twice
     counts twice, numbers outside the page table and blocks without a page are passed over.  Tokens that see no key, and padding, get zeros.

@@ -1,6 +1,7 @@
 """quant_flash_attn_paged_blocks against attention in 64 bits on the listed blocks (exactly the quantized operands, the queries' codes from the C
 oracle), on caches whose other rows hold any codes and scales that are NaN or infinite."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -71,6 +72,28 @@ def test_dealing(qfa, B, H, Hk, N, D, keep, keys):
 def test_types_and_layouts(qfa, dtype, scale_dtype):
     for D, layout in ((64, "bhnd"), (128, "bnhd"), (256, "bnhd")):
         _check(qfa, lm.Problem(2, 6, 3, 4, D, 64, [333, 90], dtype=dtype, scale_dtype=scale_dtype, layout=layout, seed=2), 3)
+
+
+# Queries in fp32: no 16-bit rounding is left.  The score's roundings (the query's scale, that times sm_scale and log2(e), the key's scale, the multiply-add: 4 of the score's size in
+# log2 units, as in weights_bound; they move a probability, and the sum that divides it, so twice) and 1 ulp of v_exp; p' in two binary16 parts (22 bits; 2^-25
+# where it lies 2^21 below the largest) and its product with the scale; sums in fp32 of terms of at most 255 v_scale: those of a copy of the rows, 32 roundings inside a product and
+# one for each, eight for the joining; the division and what is stored.
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,H,Hk,N,D,page,keep,keys,scale_dtype", [
+    (2, 8, 2, 1, 64, 16, 12, 400, torch.float32), (2, 20, 2, 3, 128, 32, 20, 900, torch.float32), (1, 9, 1, 2, 256, 16, 40, 800, torch.float16),
+    (3, 4, 1, 200, 128, 16, 33, 700, torch.float32), (2, 2, 2, 140, 64, 64, 7, 500, torch.bfloat16), (1, 4, 1, 1030, 256, 16, 20, 1100, torch.float32),
+    (1, 16, 1, 1, 128, 16, 260, 4500, torch.float32)])
+def test_fp32_queries(qfa, B, H, Hk, N, D, page, keep, keys, scale_dtype):
+    p = lm.Problem(B, H, Hk, N, D, page, [max(N, keys - 37 * i) for i in range(B)], dtype=torch.float32, scale_dtype=scale_dtype, seed=D + N)
+    blocks, sm = p.fake_lists(keep, D), m.sm_of(D)
+    o = qfa.quant_flash_attn_paged_blocks(dev(p.q), dev(p.cache), *p.places(), dev(blocks), sm_scale=sm)
+    want, size = _expect(p, blocks, sm)
+    qh = m.values(*m.quantized(p.q.float()))
+    score = max(float((p.rows[0][b][h // p.G] @ qh[b, h].T).abs().max()) for b in range(B) for h in range(H)) * sm / math.log(2)
+    relative = 2 * (math.log(2) * m.U32 * (4 * score + 3) + 2 * m.U32) + 2.0 ** -22 + 8 * m.U32
+    sums = (32 + keep * page / 32 + 8) * m.U32 * 255 * p.v_scale
+    assert bool(((o.cpu().double() - want).abs() <= relative * size + sums + 2 * m.U32 * want.abs() + m.TINY[torch.float32]).all())
+    assert float((o.cpu().double() - want).norm() / want.norm()) < 1e-5
 
 
 @pytest.mark.gpu
