@@ -523,14 +523,21 @@ int qfa_attn_paged_lse(const qfa_paged_cache *cache, const void *q, int q_dtype,
 
 /*
  * Bounds of the keys of a cache's pages: of every page and key head a low and a high row (the smallest and the largest value of every
- * element over the page's rows, as fp32 values scale * (code - zero_point)), each quantized by the arithmetic of qfa_quant_per_token.
- *   codes [pages,H,2,D] 16-byte aligned, scale [pages,H,2] float (8-byte), zero [pages,H,2] (2-byte), dense; H, D of the cache
+ * element over the page's rows, as fp32 values scale * (code - zero_point)), each quantized by the arithmetic of qfa_quant_per_token, but for the zero
+ * point of a row of one sign, which lies outside 8 bits:
+ *   zero_bits 16  zero points are int16 and not cut.  Where all of a row has one sign and is larger than 3/4 of its largest magnitude, the range of its codes begins
+ *                 at 3/4 of that (zero points are within [-1024, 1023] then).  What codes, scale and zero point stand for is half a step of the scale off the
+ *                 page's minima and maxima at most, beside roundings of fp32.
+ *   zero_bits 8 (or 0)  zero points are int8 and cut to [-128, 127], as those of tokens: a row's elements that lie further from zero than its span are cut to the span.
+ *                 Rows with elements of both signs are the same as above, bit for bit; others need not bound the page's keys.
+ *   codes [pages,H,2,D] 16-byte aligned, scale [pages,H,2] float (8-byte), zero [pages,H,2] (2-byte, of 16 bits 4-byte), dense; H, D of the cache
  * qfa_paged_bounds makes those of the pages in which positions starts[b] .. starts[b] + n - 1 lie, n = min(counts[b], N) (counts NULL: N), from
  * the pages' rows before starts[b] + n.  Called after every qfa_paged_append with its arguments, it keeps all of them up to date.  A
  * page that is written may stand only once in the call's page table.  No counterpart in the reference.
  */
 typedef struct {
-  int8_t *codes; float *scale; int8_t *zero;
+  int8_t *codes; float *scale; void *zero;
+  int zero_bits;
 } qfa_page_bounds;
 
 int qfa_paged_bounds(const qfa_paged_cache *cache, const qfa_page_bounds *bounds, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw,
@@ -540,8 +547,8 @@ int qfa_paged_bounds(const qfa_paged_cache *cache, const qfa_page_bounds *bounds
  * The blocks (pages) that a token's attention shall read.  A block's score for a token and key head is the largest over the query heads
  * that share the key head of
  *     s (s_high sum_d max(e_d, 0) (c_high,d - z_high) + s_low sum_d min(e_d, 0) (c_low,d - z_low)),
- * the query quantized per token (e = code - zero point, s its scale): no key of the block has a larger product with the query, but for
- * the roundings to codes.  Rounded to fp32 once, from 64 bits; what is not a number, or below -FLT_MAX, counts as -FLT_MAX.  Candidates of token n < counts[b] are the blocks
+ * the query quantized per token (e = code - zero point, s its scale): with bounds of 16-bit zero points no key of the block has a larger product with the
+ * query so quantized, but for half a step of the bounds' codes in every element, s |e_d| times s_high / 2 where e_d > 0 and s_low / 2 elsewhere.  Rounded to fp32 once, from 64 bits; what is not a number, or below -FLT_MAX, counts as -FLT_MAX.  Candidates of token n < counts[b] are the blocks
  * 0 .. (starts[b] + n) / page_size that the page table holds and whose page is in [0, pages).
  *   blocks  [B,cache->H,N,keep]: the numbers of the `keep` candidates with the largest scores (ties: the lowest number), the `first` first blocks and the
  *           `last` last ones that the token sees always among them; ascending, -1 behind.  first + last <= keep.

@@ -36,7 +36,7 @@ class PagedCacheStruct(ctypes.Structure):
 
 class PageBoundsStruct(ctypes.Structure):
     """qfa_page_bounds"""
-    _fields_ = [("codes", c_void_p), ("scale", c_void_p), ("zero", c_void_p)]
+    _fields_ = [("codes", c_void_p), ("scale", c_void_p), ("zero", c_void_p), ("zero_bits", c_int)]
 
 
 # argument lists mirror include/qfa.h one to one

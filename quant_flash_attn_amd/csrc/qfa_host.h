@@ -251,7 +251,8 @@ double paged_list_units(int64_t B, int64_t H, int64_t Hk, int64_t N, int64_t kee
 // Bounds of the pages' keys, and the blocks that they promise the largest scores of (qfa_paged_select.hip)
 struct PagedSelectArgs {
   PagedCachePtrs cache;
-  int8_t *codes; float *scale; int8_t *zero;   // the bounds: [pages, Hk, 2, D], [pages, Hk, 2]
+  int8_t *codes; float *scale; void *zero;     // the bounds: [pages, Hk, 2, D], [pages, Hk, 2]
+  int zero_bits;                               // 8: int8, 16: int16
   const int32_t *page_table, *starts, *counts;
   int64_t pages, Hk, width, stb, stw, B, H, N;
   int page_log2, scale_dtype, D, q_dtype;

@@ -102,8 +102,9 @@ static int check_slots(const char *who, const qfa_paged_cache *c, int64_t width)
 }
 static int check_bounds(const char *who, const qfa_page_bounds *b) {
   if (!b || !b->codes || !b->scale || !b->zero) return set_error(QFA_EINVAL, "%s: null bounds pointer", who);
-  if (!aligned16(b->codes) || !aligned8(b->scale) || (reinterpret_cast<uintptr_t>(b->zero) & 1u))
-    return set_error(QFA_EINVAL, "%s: the bounds' codes must be 16-byte aligned, scales 8-byte and zero points 2-byte aligned", who);
+  if (b->zero_bits != 0 && b->zero_bits != 8 && b->zero_bits != 16) return set_error(QFA_EINVAL, "%s: zero points of %d bits: 8 or 16 are needed", who, b->zero_bits);
+  if (!aligned16(b->codes) || !aligned8(b->scale) || (reinterpret_cast<uintptr_t>(b->zero) & (b->zero_bits == 16 ? 3u : 1u)))
+    return set_error(QFA_EINVAL, "%s: the bounds' codes must be 16-byte aligned, scales 8-byte and a block's two zero points together", who);
   return 0;
 }
 
@@ -270,7 +271,7 @@ int qfa_paged_bounds(const qfa_paged_cache *cache, const qfa_page_bounds *bounds
   PagedSelectArgs a;
   memset(&a, 0, sizeof(a));
   a.cache = ptrs_of(cache);
-  a.codes = bounds->codes; a.scale = bounds->scale; a.zero = bounds->zero;
+  a.codes = bounds->codes; a.scale = bounds->scale; a.zero = bounds->zero; a.zero_bits = bounds->zero_bits == 16 ? 16 : 8;
   a.page_table = page_table; a.starts = starts; a.counts = counts;
   a.pages = cache->pages; a.Hk = cache->H; a.width = width; a.stb = stb; a.stw = stw; a.B = B; a.N = N;
   a.page_log2 = log2_of(cache->page_size); a.scale_dtype = cache->scale_dtype; a.D = cache->D;
@@ -298,7 +299,7 @@ int qfa_paged_select(const qfa_paged_cache *cache, const qfa_page_bounds *bounds
   PagedSelectArgs a;
   memset(&a, 0, sizeof(a));
   a.cache = x.cache;
-  a.codes = bounds->codes; a.scale = bounds->scale; a.zero = bounds->zero;
+  a.codes = bounds->codes; a.scale = bounds->scale; a.zero = bounds->zero; a.zero_bits = bounds->zero_bits == 16 ? 16 : 8;
   a.page_table = page_table; a.starts = starts; a.counts = counts;
   a.pages = x.pages; a.Hk = x.Hk; a.width = width; a.stb = stb; a.stw = stw; a.B = B; a.H = H; a.N = N;
   a.page_log2 = x.page_log2; a.scale_dtype = x.scale_dtype; a.D = x.D; a.q_dtype = q_dtype;

@@ -66,7 +66,7 @@ template <> struct Load8<_Float16> {
 };
 
 // The row arithmetic: E (8 or 16) elements per lane, a token in LPT adjacent lanes.  Returns the lane's codes and, in
-// every lane of the token, its scale, zero point (an integer in [-128, 127]) and code sum.  `used`: false in the lanes
+// every lane of the token, its scale, zero point (an integer in [-128, 127], but for WIDE ones) and code sum.  `used`: false in the lanes
 // past the row's end (they hold a copy of elements of the row and add nothing to the sum).
 template <int E> struct QuantRow {
   unsigned codes[E / 4];
@@ -93,13 +93,20 @@ template <bool SHORT> __device__ __forceinline__ float quant_quotient(float x, f
   return q;
 }
 
-// SHORT: as above.
-template <int LPT, bool SHORT, int E> __device__ __forceinline__ QuantRow<E> quant_row(const float (&v)[E], bool used) {
+// SHORT: as above.  WIDE: a row of one sign keeps its span.  Its zero point lies outside of 8 bits, where the quantizer cuts it, so that the elements beyond the
+// span are cut too; here it is not cut, and the codes' range reaches from 3/4 of the largest magnitude at most to that, so that it stays within [-893, 892].  (A
+// range that reaches to zero would do with 8 bits, but its steps are up to four times as wide.)  Other rows are the same, bit for bit.
+template <int LPT, bool SHORT, int E, bool WIDE = false> __device__ __forceinline__ QuantRow<E> quant_row(const float (&v)[E], bool used) {
 #pragma clang fp contract(off)
   float mn = v[0], mx = v[0];
 #pragma unroll
   for (int e = 1; e < E; ++e) { mn = fminf(mn, v[e]); mx = fmaxf(mx, v[e]); }
   group_min_max<LPT>(mn, mx);
+  if constexpr (WIDE) {
+    const float low = mn;
+    mn = mn > 0.0f ? fminf(mn, 0.75f * mx) : mn;
+    mx = mx < 0.0f ? fmaxf(mx, 0.75f * low) : mx;
+  }
   float scale = (mx - mn) / 255.0f;
   scale = (scale == 0.0f) ? 1.0f : scale;
   // the shared reciprocal's range: a tiny scale, huge values and NaN take the IEEE `/`
@@ -123,7 +130,8 @@ template <int LPT, bool SHORT, int E> __device__ __forceinline__ QuantRow<E> qua
     for (int e = 0; e < E; ++e) q[e] = v[e] / scale;
   }
   const float zpf = -128.0f - qmn;
-  const float zp = fmaxf(-128.0f, fminf(127.0f, round_away(zpf)));
+  constexpr float ZP_MIN = WIDE ? -1024.0f : -128.0f, ZP_MAX = WIDE ? 1023.0f : 127.0f;
+  const float zp = fmaxf(ZP_MIN, fminf(ZP_MAX, round_away(zpf)));
   // codes leave as biased bytes: roundf(.) + 128 converted with unsigned saturation (= the clamp to
   // [-128, 127]), flipped back to two's complement with one XOR per dword
   QuantRow<E> row;

@@ -24,7 +24,7 @@ from . import _lib
 class PageBounds(NamedTuple):
     codes: torch.Tensor        # int8 [pages, heads, 2, head_dim]: the low and the high row
     scale: torch.Tensor        # fp32 [pages, heads, 2, 1]
-    zero_point: torch.Tensor   # int8 [pages, heads, 2, 1]
+    zero_point: torch.Tensor   # int16 [pages, heads, 2, 1]
 
 
 def make_page_bounds(cache) -> PageBounds:
@@ -33,13 +33,15 @@ def make_page_bounds(cache) -> PageBounds:
     device = cache[0].device
     return PageBounds(torch.zeros(pages, heads, 2, head_dim, dtype=torch.int8, device=device),
                       torch.zeros(pages, heads, 2, 1, dtype=torch.float32, device=device),
-                      torch.zeros(pages, heads, 2, 1, dtype=torch.int8, device=device))
+                      torch.zeros(pages, heads, 2, 1, dtype=torch.int16, device=device))
 
 
 def paged_bounds_update(bounds, cache, page_table: torch.Tensor, starts: torch.Tensor, N: int, counts: Optional[torch.Tensor] = None) -> None:
     """The bounds of the pages that positions starts[b] .. starts[b] + n - 1 lie in (n = N, or counts[b] of them), in place and in one launch:
-    of every element the smallest and the largest key of the page's rows before starts[b] + n, the two rows quantized per token as
-    asymmetric_quant_per_token does it.
+    of every element the smallest and the largest key of the page's rows before starts[b] + n, the two rows quantized as asymmetric_quant_per_token
+    does it, but with zero points of 16 bits: rows of one sign, which the least and the largest keys of a page often are, have theirs outside of 8.
+    (Bounds whose zero points are int8 are taken too: their rows are quantized as tokens are, and of a row of one sign what lies
+    further from zero than its span is cut, so that such bounds may fall short of their page's keys.)
 
     With the arguments of every paged_cache_append it keeps all bounds up to date (after paged_cache_evict: the new pages', from position 0
     on).  A page that is written may stand only once in the call's page table.
@@ -54,7 +56,8 @@ def paged_select_blocks(q: torch.Tensor, cache, bounds, page_table: torch.Tensor
     [B,heads,N,keep], ascending, -1 behind (all of them for padding tokens).
 
     Selected are the blocks whose keys may have the largest product with one of the query heads that share the key head: the score is
-    the sum over elements of max(q low, q high), the query quantized per token, exact but for one rounding to fp32.  Ties go to the
+    the sum over elements of max(q low, q high), the query quantized per token, exact but for one rounding to fp32: what a key of the block may
+    have at most, but for half a step of the bounds' codes.  Ties go to the
     lowest number; the `first` first and `last` last blocks that a token sees are always taken (first + last <= keep).
     return_scores: also the scores [B,heads,N,pages of a sequence], fp32, -inf for blocks that a token does not see or that have no page.
     """
