@@ -184,8 +184,8 @@ template <typename S, int D, bool FINE> __global__ __launch_bounds__(64 * FEW_WA
       *reinterpret_cast<u32x2 *>(tc + 128 + 2 * lane) = w;
     }
     const int mine = 16 * copy + 4 * G;   // this lane's first key
-    // The keys are in LDS once no more than the loads of values behind them are on their way.  (The compiler moves no load
-    // across a statement like this; a register that it spilled would be counted too: the build looks for scratch.)
+    // The keys are in LDS once no more than the loads of values behind them are on their way.  (The compiler moves no access
+    // of memory across a statement like this, or the one behind the products; a register that it spilled would be counted too.  The build looks at all of it.)
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VE) : "memory");
     i32x4 s = {0, 0, 0, 0}, rk = {0, 0, 0, 0};
 #pragma unroll
@@ -217,7 +217,9 @@ template <typename S, int D, bool FINE> __global__ __launch_bounds__(64 * FEW_WA
       for (int v = 0; v < 4; ++v)
         if (v > seen) f[v] = -INFINITY;
     }
-    load_keys(t, i + 1);   // (where the products have read)
+    // the next tile's keys go where the products have read: not before all of their reads have returned
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    load_keys(t, i + 1);
     // ---- p and its row sum, p' = p * scale_j and the largest of them
     float ps[4], mx = 0.f, l_new = 0.f;
     auto probs = [&]() __attribute__((always_inline)) {

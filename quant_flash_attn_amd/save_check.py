@@ -9,7 +9,10 @@ All lanes are on at a kernel's start (workgroups are whole waves) and wherever e
 exec while they all were; such registers are followed through copies and through the lanes of vector registers that hold spilled
 scalars.  Whatever else happens to exec counts as turning lanes off.
 
-Kernels that wait for loads by their number (COUNTING) may have no scratch at all: what the compiler spills counts among the loads.
+Kernels that wait for loads by their number (COUNTING) load keys into LDS and count the loads behind those.  They may have no scratch at all, since what the
+compiler spills counts too; on every path from the last load into LDS to such a wait there are at least as many vector memory requests as the wait leaves on
+their way; and behind such a wait, where the keys are read, LDS is loaded again only after a wait for all of its reads.  (These waits are statements that no
+access of memory is moved across.)
 
     python -m quant_flash_attn_amd.save_check FILE.s
 """
@@ -94,12 +97,63 @@ def _saved(i) -> Optional[FrozenSet[Tuple[str, int]]]:
     return i.reads or None
 
 
+def _into_lds(i) -> bool:
+    return i.op.startswith("buffer_load") and "lds" in i.text.split()
+
+
+def _left(i, counter: str) -> int:
+    """How many requests a wait in inline assembly leaves on their way; -1: it is none of that counter's."""
+    m = re.search(counter + r"\((\d+)\)", i.text) if i.inline and i.op == "s_waitcnt" else None
+    return int(m.group(1)) if m else -1
+
+
+def _counts(ins, labels) -> List[Tuple[int, str]]:
+    """What breaks a COUNTING kernel's rules: the index of an instruction, and what is wrong with it."""
+    before: Dict[int, List[int]] = {}
+    for k, i in enumerate(ins):
+        if k + 1 < len(ins) and i.op not in ("s_branch", "s_endpgm", "s_setpc_b64"):
+            before.setdefault(k + 1, []).append(k)
+        if i.target in labels:
+            before.setdefault(labels[i.target], []).append(k)
+    bad: List[Tuple[int, str]] = []
+    for k, i in enumerate(ins):
+        want = _left(i, "vmcnt")
+        if want > 0:   # back to the loads into LDS
+            todo, seen = [(k, 0)], set()
+            while todo:
+                p, n = todo.pop()
+                if (p, n) in seen:
+                    continue
+                seen.add((p, n))
+                n += not _into_lds(ins[p]) and bool(re.match(r"(global|buffer|flat|scratch)_(load|store|atomic)", ins[p].op))
+                if n >= want:
+                    continue
+                if _into_lds(ins[p]) or p == 0:
+                    bad.append((k, f"{n} requests behind the loads into LDS"))
+                    break
+                todo += [(q, n) for q in before.get(p, [])]
+        if _into_lds(i):   # back to the wait for what has been read there (or the start), not to the one in front of those reads
+            todo, seen = list(before.get(k, [])), set()
+            while todo:
+                p = todo.pop()
+                if p in seen or _left(ins[p], "lgkmcnt") == 0:
+                    continue
+                seen.add(p)
+                if _left(ins[p], "vmcnt") > 0:
+                    bad.append((k, "a load into LDS that may still be read"))
+                    break
+                todo += before.get(p, [])
+    return bad
+
+
 def check(path: str) -> List[str]:
     """What is wrong, one line each; empty: nothing."""
     bad: List[str] = []
     for name, ins, labels, scratch in _kernels(path):
         if scratch and any(k in name for k in COUNTING):
             bad.append(f"{path}: {name}: counts its loads, and has {scratch} bytes of scratch")
+        if any(k in name for k in COUNTING):
+            bad += [f"{path}:{ins[k].line}: {name}: {what}: {ins[k].text}" for k, what in _counts(ins, labels)]
         if not any(_saved(i) for i in ins):
             continue
         after: Dict[int, List[int]] = {}
