@@ -24,9 +24,9 @@ struct PagedMergeArgs {
   PagedWork own, shared;   // shared.grid 0: none
   void *o;
   int o_dtype, chunks, chunk_rows;   // chunks of rows of a sequence and key head, a power of two that divides a block
-  float *lse;                        // nullable
+  float *lse;                        // of LSE
 };
-template <int D> __global__ __launch_bounds__(256) void paged_merge_kernel(PagedMergeArgs a) {
+template <int D, bool LSE> __global__ __launch_bounds__(256) void paged_merge_kernel(PagedMergeArgs a) {
   constexpr int CL = D / 4, SLOTS = 256 / CL;
   __shared__ float red[SLOTS][D + 4];
   const int tid = threadIdx.x, d = 4 * (tid % CL), slot = tid / CL;
@@ -41,7 +41,7 @@ template <int D> __global__ __launch_bounds__(256) void paged_merge_kernel(Paged
     const int i = r / a.own.G;
     const float inv = i >= seq.tokens || x.l == 0.f ? 0.f : 1.0f / x.l;
     const int64_t row = ((int64_t)b * a.own.Hk * a.own.G + h * a.own.G + r % a.own.G) * a.own.N + i, off = row * D;
-    if (a.lse && d == 0) a.lse[row] = i >= seq.tokens || x.l == 0.f ? -INFINITY : (x.m + __log2f(x.l)) * kLn2;
+    if (LSE && d == 0) a.lse[row] = i >= seq.tokens || x.l == 0.f ? -INFINITY : (x.m + __log2f(x.l)) * kLn2;
     store4(static_cast<char *>(a.o) + off * (a.o_dtype == QFA_F32 ? 4 : 2), a.o_dtype, d,
            f32x4{mul_zero_wins(x.acc[0], inv), mul_zero_wins(x.acc[1], inv), mul_zero_wins(x.acc[2], inv), mul_zero_wins(x.acc[3], inv)});
   };
@@ -227,7 +227,9 @@ template <int D> static int launch_d(const PagedAttnArgs &x, hipStream_t st) {
   while (chunk_rows < 16 && x.B * x.Hk * ((problem[0] + chunk_rows - 1) / chunk_rows) > 1024) chunk_rows *= 2;
   const int chunks = (int)((problem[0] + chunk_rows - 1) / chunk_rows);
   const PagedMergeArgs m = {w[0], w[1], x.o, x.q_dtype, chunks, chunk_rows, x.lse};
-  paged_merge_kernel<D><<<dim3((unsigned)(x.B * x.Hk * chunks)), dim3(256), 0, st>>>(m);
+  const dim3 grid((unsigned)(x.B * x.Hk * chunks));
+  if (x.lse) paged_merge_kernel<D, true><<<grid, dim3(256), 0, st>>>(m);
+  else paged_merge_kernel<D, false><<<grid, dim3(256), 0, st>>>(m);
   return check_launch("qfa_attn_paged (merge)");
 }
 int launch_paged_attn(const PagedAttnArgs &x, hipStream_t st) {

@@ -15,7 +15,6 @@ constexpr int PAGED_WGS = 256 * 2;   // two on a CU
 
 __device__ __forceinline__ i32x4 paged_mfma_i8(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
-// Deal: how the work is dealt -- PagedDeal, every sequence's keys from a place on, or PagedListDeal, those of listed blocks
 // the binary16 number of a small whole number; 1152 less than two of them; what two numbers have beside their binary16 parts, as such parts
 __device__ __forceinline__ unsigned half_of(int x) { return (unsigned)__builtin_bit_cast(unsigned short, (_Float16)(short)x); }
 __device__ __forceinline__ unsigned without_offset(unsigned two) {
@@ -27,6 +26,7 @@ __device__ __forceinline__ unsigned rest_h2(float x, float y, unsigned parts) {
   return pack_h2(x - (float)p[0], y - (float)p[1]);
 }
 
+// Deal: how the work is dealt -- PagedDeal, every sequence's keys from a place on, or PagedListDeal, those of listed blocks.
 // FINE: p' in two binary16 parts, 22 bits, and codes without an offset, for queries in fp32 on lists: one part is 2^-11 off, and the offset takes 10 bits of the sums
 template <typename S, int D, typename Deal, bool STREAM, bool FINE = false> __global__ __launch_bounds__(256, 2) void paged_rows_kernel(PagedAttnKernelArgs a) {
   constexpr bool SHARED = Deal::ONE_PROBLEM, LIST = Deal::LIST;
@@ -43,6 +43,7 @@ template <typename S, int D, typename Deal, bool STREAM, bool FINE = false> __gl
   __shared__ __attribute__((aligned(16))) unsigned char smem[TOTAL];
 
   Deal deal(a.work, PAGED_ROWS, SKV_TILE);
+  if constexpr (LIST) deal.lists(a.list_tiles, a.list_each);
   unsigned x;
   typename Deal::Item item;
   if (!deal.find(x, item)) return;

@@ -35,7 +35,8 @@ template <typename S, int D, bool FINE> __global__ __launch_bounds__(64 * FEW_WA
   constexpr int OFF_K = OFF_TC + TC, EACH = OFF_K + FEW_TILE * D;   // a tile's keys; the copies' sums
   __shared__ __attribute__((aligned(16))) unsigned char all[FEW_WAVES * EACH];
 
-  const PagedListDeal deal(a.work, PAGED_ROWS, FEW_TILE);
+  PagedListDeal deal(a.work, PAGED_ROWS, FEW_TILE);
+  deal.lists(a.list_tiles, a.list_each);
   PagedListDeal::Item item;
   deal.item(deal.workgroup(), item);
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), q16 = lane % 16, G = lane / 16;
@@ -372,12 +373,14 @@ struct PagedListMergeArgs {
   PagedWork work;
   void *o;
   int o_dtype;
+  unsigned tiles, each;
 };
 template <int D> __global__ __launch_bounds__(256) void paged_list_merge_kernel(PagedListMergeArgs a) {
   constexpr int CL = D / 4, SLOTS = 256 / CL;
   __shared__ float red[SLOTS][D + 4];
   const int tid = threadIdx.x, d = 4 * (tid % CL), slot = tid / CL;
-  const PagedListDeal deal(a.work, PAGED_ROWS, SKV_TILE);
+  PagedListDeal deal(a.work, PAGED_ROWS, SKV_TILE);
+  deal.lists(a.tiles, a.each);
   PagedListDeal::Item it;
   deal.item(blockIdx.x, it);
   const PagedPieces mine(it.first, deal.each, it.tiles, 0, 0);
@@ -483,17 +486,17 @@ template <int D> static int launch_d(const PagedListArgs &l, hipStream_t st) {
   a.pages = x.pages; a.stb = x.stb; a.stw = x.stw; a.sqb = x.sq[0]; a.sqh = x.sq[1]; a.sqn = x.sq[2];
   a.width = (int)x.width; a.page_log2 = x.page_log2; a.q_dtype = x.q_dtype;
   a.sm_scale_log2 = x.sm_scale * kLog2e;
-  a.blocks = l.blocks; a.keep = (int)l.keep;
+  a.blocks = l.blocks; a.keep = (int)l.keep; a.list_tiles = p.tiles; a.list_each = p.each;
   float *slots = static_cast<float *>(x.workspace);
   a.work = {x.starts, x.counts, (int)x.B, (int)x.Hk, G, (int)x.N, 1, 0, (int)(x.width << x.page_log2), p.grid, PAGED_ROWS, SKV_TILE, LIST_EXTRA, nullptr,
-            slots, p.cut ? slots + 2LL * p.grid * PAGED_ROWS * D : nullptr, nullptr, nullptr, p.tiles, p.each};
+            slots, p.cut ? slots + 2LL * p.grid * PAGED_ROWS * D : nullptr, nullptr, nullptr};
   const dim3 grid((unsigned)p.grid), block(256);
   if (x.scale_dtype == QFA_F32) launch_list<float, D>(a, p.few, grid, st);
   else if (x.scale_dtype == QFA_F16) launch_list<_Float16, D>(a, p.few, grid, st);
   else launch_list<__bf16, D>(a, p.few, grid, st);
   if (int e = check_launch("qfa_attn_paged_blocks")) return e;
   if (!p.cut) return 0;
-  paged_list_merge_kernel<D><<<dim3((unsigned)items), block, 0, st>>>({a.work, x.o, x.q_dtype});
+  paged_list_merge_kernel<D><<<dim3((unsigned)items), block, 0, st>>>({a.work, x.o, x.q_dtype, p.tiles, p.each});
   return check_launch("qfa_attn_paged_blocks (merge)");
 }
 int launch_paged_list(const PagedListArgs &x, hipStream_t st) {

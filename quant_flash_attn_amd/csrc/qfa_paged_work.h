@@ -36,7 +36,6 @@ struct PagedWork {
   unsigned *first;                  // [items] the unit of an item's first tile, [items] that one's units per workgroup (own keys)
   float *slots, *slots_ml;          // [2 * grid][br][D] and (m in log2 units, l): of a piece that does not begin its item, one that does
   float *whole, *whole_ml;          // nullable: items in one piece, [problem, head, row] (null: they are normalised and stored)
-  unsigned list_tiles, list_each;   // of lists: tiles of an item, units of a workgroup
 };
 
 // A sequence's position of its first new token, and how many it brings
@@ -224,11 +223,16 @@ struct PagedListDeal {
   typedef PagedDeal<false, false> Keys;
   typedef Keys::Row Row;
   struct Item { int p, h, rb; unsigned at, tiles, first; PagedSeq s; };
+  unsigned item_tiles;
   __device__ __forceinline__ PagedListDeal(const PagedWork &a_, int br, int) : a(a_), BR(br) {
     rows = a.G;
     blocks = (rows + BR - 1) / BR;
-    per_item = a.list_tiles + (unsigned)a.extra;
-    each = a.list_each;
+  }
+  // tiles of an item, units of a workgroup: before anything else is asked
+  __device__ __forceinline__ void lists(unsigned tiles, unsigned units) {
+    item_tiles = tiles;
+    per_item = tiles + (unsigned)a.extra;
+    each = units;
     total = (unsigned)(a.B * a.N * a.Hk * blocks) * per_item;
   }
   __device__ __forceinline__ PagedSeq seq(int p) const {
@@ -247,7 +251,7 @@ struct PagedListDeal {
     it.rb = (int)(n - token * (unsigned)blocks);
     it.h = (int)(bh - b * (unsigned)a.Hk);
     it.p = (int)(b * (unsigned)a.N + token - bh * (unsigned)a.N);
-    it.tiles = a.list_tiles;
+    it.tiles = item_tiles;
     it.first = n * per_item + (unsigned)a.extra;
     it.at = 0;
     it.s = seq(it.p);
