@@ -105,8 +105,8 @@ int launch_paged_bounds(const PagedSelectArgs &a, hipStream_t st) {
 // The list of one token, by T threads (tid: which of them): the blocks with the `keep` largest scores, number(i) of block i
 template <int T, typename Top, typename Number>
 __device__ __forceinline__ void select_blocks(Top &top, const PagedSelectArgs &x, int64_t item, int64_t pos, int tid, Number number) {
-  const int64_t own = min(pos >> x.page_log2, x.width - 1), last = own - x.last;   // (a token past the table's end sees all of it)
-  const int blocks = pos < 0 ? 0 : (int)(own + 1), keep = (int)x.keep, first = (int)x.first;
+  const int blocks = pos < 0 ? 0 : (int)min((pos >> x.page_log2) + 1, x.width);   // (a token past the table's end sees all of it)
+  const int keep = (int)x.keep, first = (int)x.first, last = blocks - 1 - (int)x.last;
   int32_t *to = x.blocks + item * keep;
   unsigned taken = 0;
   if (blocks > 0)
