@@ -553,7 +553,8 @@ int qfa_paged_bounds(const qfa_paged_cache *cache, const qfa_page_bounds *bounds
  *   blocks  [B,cache->H,N,keep]: the numbers of the `keep` candidates with the largest scores (ties: the lowest number), the `first` first blocks and the
  *           `last` last ones that the token sees always among them; ascending, -1 behind.  first + last <= keep.
  *   scores  nullable, [B,cache->H,N,width]: of all candidates, -infinity elsewhere; without it a workspace of
- *           qfa_paged_select_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant, one for each call under way
+ *           qfa_paged_select_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant, one for each call under way.  Either holds 4 bytes for every token,
+ *           key head and place of the page table: a long prompt goes in pieces of its tokens
  */
 int64_t qfa_paged_select_workspace_bytes(int64_t B, int64_t Hk, int64_t N, int64_t width);
 

@@ -5,8 +5,8 @@
 // and zero points of keys and values, each to its place in the new pages: what is kept stays in order, so the last slots are the newest
 // ones again, and pages that other sequences share are not touched.
 //
-// The selection waits for its own steps (8 x 5120 slots 10 us, 512 x 3000 13), the rows are bound by HBM: 16 sequences, 32 heads of 128, 2000 rows of each,
-// codes in and out 530 MB in 107 us (5.0 TB/s); 8 heads x 4096 rows 5.7 us, a launch with three loads that wait for each other.
+// The selection waits for its own steps (8 x 5120 slots 10.7 us, 512 x 3000 13.4), the rows are bound by HBM: 16 sequences, 32 heads of 128, 2000 rows of each,
+// codes in and out 530 MB in 108 us (4.9 TB/s); 8 heads x 4096 rows 5.7 us, a launch with three loads that wait for each other.
 #include "qfa_host.h"
 #include "qfa_topk.h"
 
@@ -42,7 +42,7 @@ template <typename Top, int T> __global__ __launch_bounds__(T) void evict_select
 }
 
 // D/16 lanes hold a row; a workgroup moves some rows of one sequence and key head, of keys or of values
-constexpr int EVICT_UNROLL = 2;   // rows of a thread (1 x 8 heads x 4096 and 16 x 32 x 1900 rows of 128, us: 2 6.1 and 128, 4 6.9 and 135, 8 11.2 and 150)
+constexpr int EVICT_UNROLL = 2;   // rows of a thread (1 x 8 heads x 4096 and 16 x 32 x 1900 rows of 128, us: 2 5.7 and 108, 4 6.8 and 115, 8 11.2 and 128)
 template <typename S, int D, bool ONCE> __global__ __launch_bounds__(256) void evict_move_kernel(PagedEvictArgs x, int chunks) {
   constexpr int LPR = D / 16, ROWS = 256 / LPR;
   unsigned id = blockIdx.x;
@@ -117,7 +117,9 @@ int launch_paged_evict(const PagedEvictArgs &x, hipStream_t st) {
   const int64_t chunks = (most + rows - 1) / rows;
   if ((double)x.B * (double)x.Hk * 2 * (double)chunks > 2147483647.0) return set_error(QFA_EUNSUPPORTED, "paged_evict: too many rows for one launch");
   const int64_t slots = x.width << x.page_log2;
-  // more sequences and heads than CUs share one: 512 x 3000 slots 10.9 us with 512 threads and with 1024, 8 x 5120 9.7 and 8.1
+  // More sequences and heads than CUs share one: 512 threads and the numbers that they hold leave room for more of them.  256, 1024, 2048 and 4096 slots, us with 512 threads:  512
+  // sequences times heads 6.1, 7.2, 8.9, 12.0,  1024: 7.7, 9.6, 12.0, 16.2,  4096: 22.4, 27.9, 33.7, 48.5;  with 1024:  7.1, 9.5, 11.1, 12.0,  12.0, 15.8, 17.4, 21.0,  37.0, 51.2, 58.0, 69.0.
+  // (512 x 3000: 13.4 and 12.5.)  Few of them want all threads: 8 x 5120 slots 12.5 with 512 and 10.9 with 1024.
   if (slots <= 4096 && x.B * x.Hk > 256) launch_top<TopHeld<512, 4096, 11>, 512>(x, st);
   else if (slots <= 16384) launch_top<TopHeld<1024, 16384, 11>, 1024>(x, st);
   else launch_top<TopHeld<1024, 0, 11>, 1024>(x, st);

@@ -1,6 +1,7 @@
 // Attention of every token on a list of blocks (pages) of its sequence, those that a cheap score has selected (qfa_paged_select.hip):
 //     O = softmax(sm_scale * Q^ K^^T) V^   over the keys of the listed blocks at or before the token,
-// with the arithmetic of attention on all keys (qfa_paged_attn.hip), and its kernel, or one for few rows.  A token and key head are an item: the query heads that
+// with the arithmetic of attention on all keys (qfa_paged_attn.hip), and its kernel, or one for few rows.  Probabilities times scales are binary16 numbers for
+// queries of 16 bits, 2^-11 off relative to a sum of p |v|: a second part of them, which queries in fp32 get (FINE), takes 26 % longer for 2 x 333 tokens.  A token and key head are an item: the query heads that
 // share the key head are its rows, the list's blocks one behind the other its keys.  A half of a tile lies in one block, so what the mask
 // asks is where each half's keys begin; the list is read beside the page numbers, 32 tiles ahead.
 //
@@ -18,10 +19,10 @@ constexpr int LIST_EXTRA = 12;      // units of an item beside its tiles, as the
 // is a softmax of its own: the score products add up in one accumulator, each 16 keys' with the queries of their copy and zeros elsewhere,
 // and a lane has four scores of 64 keys in place of eight of 32.  The probabilities enter the P.V product likewise.  The copies meet at the end,
 // as the waves do: two, so that an item costs little beside its tiles.  A value's bytes, offset by 128, are binary16 numbers of 2^-24 each as they stand.
-// 2 x 333 tokens, 8 key heads of 4 x 128, 2048 keys each, us: 168 against 278 of paged_rows_kernel; of one block of 64 keys each 31 against 65.  With one wave to an item
-// 180 and 20 instead of 179 and 32, with four 207; before, keys in the fragments' order, one copy of the rows to four waves 278; values in the products' order,
-// 8 bytes a lane 179, through LDS 198, 16 bytes a lane 171 (two workgroups less on a CU 197); offset by 1152 in place of 128, another instruction for two
-// values, 171.  Keys and values come from L2 (99 %): 2.9 GB, 17 TB/s.  The way from the L1 cache to registers is busy for 76 % of the time, its tags for 52 %, the
+// 2 x 333 tokens, 8 key heads of 4 x 128, 2048 keys each, us: 165 against 291 of paged_rows_kernel (calls in a row 140 against 244, of one block of 64 keys each 28 against 64); 64 x 1 token,
+// 1024 keys: 29.1 against 29.5.  With one wave to an item 161 and 30.4, with four 190 and 29.7.  Every step against the one before it, where it was taken: values 8 bytes a lane in
+// the products' order 179, through LDS 198, 16 bytes a lane 171 (two workgroups less on a CU 197), and that with an offset of 128 in place of 1152, an instruction less for two
+// values, 168.  Keys and values come from L2 (99 %): 2.9 GB, 17 TB/s.  The way from the L1 cache to registers is busy for 76 % of the time, its tags for 52 %, the
 // vector pipe for 60 %, the matrix pipe for 24 %: a tile takes 240 vector instructions, 96 of them the values' conversion.
 constexpr int FEW_ROWS = 4, FEW_TILE = 64, FEW_WAVES = 2;
 template <typename S, int D, bool FINE> __global__ __launch_bounds__(64 * FEW_WAVES, D == 256 ? 2 : 3) void paged_list_few_kernel(PagedAttnKernelArgs a) {
@@ -432,11 +433,13 @@ template <int D> __global__ __launch_bounds__(256) void paged_list_merge_kernel(
 // tiles, us whole and cut:  64 elements 8 items T 32: 10.5, 11.7, T 48: 13.2, 11.6; 192 items T 64: 16.6, 19.6, T 256: 49, 43.8;  128: 8 items T 32: 12.4, 12.0,
 // 64 items T 32: 12.7, 12.6, T 64: 19.8, 16.1, 192 items T 128: 36.3, 39.8;  256: 8 items T 16: 11.9, 13.6, T 32: 16.4, 13.8, 64 items T 32: 18.1, 15.6,
 // 192 items T 256: 142, 151.
+// (A list's places are counted, not what stands in them: the kernel for few rows walks all of them, the other one ends at the last block that the token sees.  2 x 333 tokens from
+// position 0, us: 46.5 with lists of the 6 blocks that there are, 136 with 26 places of -1 behind them.)
 // The kernel for up to four rows is as fast or faster from 512 items on (1024 of 256 elements), and for few keys: items x keys, us of
 // paged_rows_kernel (whole or cut) and of it:  64 elements 8 x 128: 6.5, 6.2, 8 x 512: 7.9, 8.4, 256 x 512: 8.0, 8.6, 512 x 512: 11.7, 11.0,
-// 1024 x 64: 10.6, 6.2, 1024 x 4096: 106, 104;  128: 8 x 256: 7.8, 7.2, 8 x 1024: 12.4, 14.6, 128 x 4096: 29.9, 44.6, 512 x 256: 11.9, 10.2,
+// 1024 x 64: 10.6, 6.2, 1024 x 4096: 106, 104;  128: 8 x 256: 7.8, 7.2, 8 x 1024: 12.4, 14.3, 128 x 4096: 29.7, 43.6, 512 x 256: 11.4, 10.0,
 // 512 x 4096: 99.4, 100.6, 1024 x 64: 14.6, 8.4;  256: 8 x 128: 8.6, 9.3, 512 x 512: 26.6, 29.1, 512 x 2048: 97, 102, 1024 x 64: 19.2, 14.3,
-// 1024 x 2048: 189, 190, 2664 (333 tokens of one sequence) x 2048: 216, 170.
+// 1024 x 2048: 189, 190, 2664 (333 tokens of one sequence) x 2048: 200, 152.
 struct PagedListPlan {
   unsigned tiles, each;
   int grid;

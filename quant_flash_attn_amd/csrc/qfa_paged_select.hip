@@ -12,9 +12,9 @@
 //
 // Scores, then for every token and key head the `keep` best (qfa_topk.h), in one launch or two.
 //
-// Waits bound all of it, not the 2 (D + 5) bytes of a block: page number, bounds, the digits of a selection come one behind the other.  One token of 64 sequences
-// of 5 to 512 blocks, 8 key heads of 4 x 128, 34 MB: 18.2 us (2 TB/s), vector pipe 10 % busy; 333 tokens of 2 sequences of 219 blocks, 5 key heads of 4 x 64:
-// 15.8; one token of 2048 blocks: 6.0 and 8.2 for the selection.  Not faster: eight waves that take all blocks at once (22.8; with 128 registers each 32), bounds
+// Waits bound all of it, not the 2 (D + 6) bytes of a block: page number, bounds, the digits of a selection come one behind the other.  One token of 64 sequences
+// of 5 to 512 blocks, 8 key heads of 4 x 128, 34 MB: 18.5 us (2 TB/s), vector pipe 10 % busy; 333 tokens of 2 sequences of 219 blocks, 5 key heads of 4 x 64:
+// 15.6; one token of 2048 blocks: 5.9 and 8.4 for the selection.  Not faster: eight waves that take all blocks at once (22.8; with 128 registers each 32), bounds
 // brought in the order in which they lie and turned in LDS (17.6; 256 elements run out of registers).
 #include <cfloat>
 
@@ -27,7 +27,7 @@ namespace qfa {
 
 // ---------------------------------------------------------------------------------------------------------------- bounds
 // A wave takes a page and key head: D/16 lanes hold a row, each its minima and maxima of 16 elements, which meet at the end.  A launch with its waits: one token of
-// 64 sequences, 8 key heads of 128, 16 rows a page 4.5 us, 64 rows 4.9
+// 64 sequences, 8 key heads of 128, 16 rows a page 4.2 us, one token, 64 rows 5.2; of whole prompts, 131072 tokens in pages of 64, 31.6 us (4.5 TB/s), 4 x 8192 tokens in pages of 16 18
 template <typename S, int D, typename Z> __global__ __launch_bounds__(256) void page_bounds_kernel(PagedSelectArgs a, int pages_each) {
   constexpr int LPR = D / 16, RPW = 64 / LPR;
   const int lane = threadIdx.x % 64, sub = lane % LPR, rg = lane / LPR;
@@ -510,8 +510,9 @@ int launch_paged_select(const PagedSelectArgs &x, hipStream_t st) {
   const int step = few ? 256 : 64;   // blocks of a workgroup's step
   p.steps = 1;
   // Scores and selection in one launch where a workgroup can hold all blocks of its tokens, and has one step of them or enough others beside it.  Four query
-  // heads of 128 elements, us with two launches and with one: 256 blocks of 1, 8 and 32 sequences with 8 key heads 10.3, 10.6, 10.9 and 9.1, 8.9, 9.4;
-  // 1000 blocks 14.5, 15.1, 23 and 20.3, 20.7, 22.4
+  // heads of 128 elements, us with two launches and with one: 256 blocks of 1, 8 and 32 sequences with 8 key heads 9.5, 9.7, 10.2 and 8.8, 8.9, 9.1;
+  // 1000 blocks of 1, 8, 32 and 64 12.9, 14.2, 25.5, 37.7 and 19.9, 20.5, 24.6, 35.  What decides is the table's width, for the host does not know the lengths: 32 sequences of 256
+  // blocks under a table of 2048, 16384 and 32768 pages 13.0, 19.7 and 29.4
   const bool whole = x.width <= SELECT_WHOLE || (few && x.width <= SELECT_WHOLE_FEW && groups >= 256);
   if (whole) p.steps = (int)((x.width + step - 1) / step);   // (SELECT_STEPS at most)
   while (!whole && p.steps < SELECT_STEPS && groups * ((x.width + 2 * step * p.steps - 1) / (2 * step * p.steps)) >= 512) p.steps *= 2;

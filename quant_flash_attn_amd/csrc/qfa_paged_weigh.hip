@@ -10,7 +10,7 @@
 // through LDS in panels of 64, the next one on its way while one is worked on.
 //
 // Few rows are bound by reading the keys: 64 sequences of 65 to 8192 keys, 8 key heads of 4 x 128, 16 keys a page: 64 us, 4.9 TB/s (at the 5 TB/s of a large
-// copy 62 us).  128 rows on 4 x 4000 to 8000 keys, 8 key heads of 128: 18.2 us behind 4.1 of the launch in front.  All workgroups run at once and wait, for
+// copy 62 us).  128 rows on 4 x 4000 to 8000 keys, 8 key heads of 128: 18.6 us behind 4.2 of the launch in front.  All workgroups run at once and wait, for
 // page numbers, keys and one block of rows after the other: the vector pipe, seven instructions a score, is busy for 30 % of the time, the matrix pipe 6 %.
 #include "qfa_host.h"
 #include "qfa_quant_row.h"
@@ -338,6 +338,8 @@ template <typename S, int D> static int launch_sd(const PagedWeighArgs &w, hipSt
   // Keys that outgrow the last-level cache, with what else is read of it, are not to stay there.  One token, 32 sequences with 8 key heads, keys in MiB, us without
   // and with:  64 elements 128: 32.4, 36.0, 256: 58.0, 63.5, 384: 100.9, 93.3, 1024: 265, 237;  128: 256: 49.8, 55.4, 384: 90.6, 82.0, 1024: 238, 215;  256: 256: 48.7,
   // 54.6, 384: 83.2, 83.3, 1024: 217, 208.  (Non-temporal loads in the fragments' order: 64 sequences of 65 to 8192 keys 83 instead of 72 and, these, 64.)
+  // The table's slots are counted, for the host does not know the lengths, and all of them are written: 64 sequences of 65 to 1024 keys 13.0 under their own table of 1024 slots, 17.4
+  // under one of 8192 (32 MiB of weights in and out), 53.3 under one of 32768 (128 MiB); of 65 to 8192 keys 64 and, under 32768 slots, 99.5.
   const bool stream = one && (double)BH * (double)slots * D > 320.0 * (1 << 20);
   if (stream) paged_weigh_kernel<S, D, true, true><<<grid, block, 0, st>>>(p);
   else if (one) paged_weigh_kernel<S, D, true, false><<<grid, block, 0, st>>>(p);

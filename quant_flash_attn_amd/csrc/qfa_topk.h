@@ -3,7 +3,8 @@
 //
 // Up to 16384 numbers are brought to LDS once, and their first digit is counted on the way; more are read anew for every walk, eight at a time.
 // Digits are counted in LDS: the first one holds the exponent and the first bits of the mantissa, behind it few numbers are left, and the
-// search ends as soon as all that begin alike are wanted.  8 x 5120 numbers: 7.8 us; 512 x 3000: 10.9; 256 numbers or fewer by one wave each: 3.6.
+// search ends as soon as all that begin alike are wanted.  8 x 5120 numbers and a list of them: 10.7 us; 512 x 3000:
+// 13.4; scores and selection of 2 x 5 x 333 times 219 numbers, by a wave each: 15.6.
 #pragma once
 #include "qfa_paged_work.h"
 
