@@ -525,10 +525,10 @@ int qfa_attn_paged_lse(const qfa_paged_cache *cache, const void *q, int q_dtype,
  * Bounds of the keys of a cache's pages: of every page and key head a low and a high row (the smallest and the largest value of every
  * element over the page's rows, as fp32 values scale * (code - zero_point)), each quantized by the arithmetic of qfa_quant_per_token, but for the zero
  * point of a row of one sign, which lies outside 8 bits:
- *   zero_bits 16  zero points are int16 and not cut.  Where all of a row has one sign and is larger than 3/4 of its largest magnitude, the range of its codes begins
+ *   qfa_page_bounds16  zero points are int16 and not cut.  Where all of a row has one sign and is larger than 3/4 of its largest magnitude, the range of its codes begins
  *                 at 3/4 of that (zero points are within [-1024, 1023] then).  What codes, scale and zero point stand for is half a step of the scale off the
  *                 page's minima and maxima at most, beside roundings of fp32.
- *   zero_bits 8 (or 0)  zero points are int8 and cut to [-128, 127], as those of tokens: a row's elements that lie further from zero than its span are cut to the span.
+ *   qfa_page_bounds    zero points are int8 and cut to [-128, 127], as those of tokens: a row's elements that lie further from zero than its span are cut to the span.
  *                 Rows with elements of both signs are the same as above, bit for bit; others need not bound the page's keys.
  *   codes [pages,H,2,D] 16-byte aligned, scale [pages,H,2] float (8-byte), zero [pages,H,2] (2-byte, of 16 bits 4-byte), dense; H, D of the cache
  * qfa_paged_bounds makes those of the pages in which positions starts[b] .. starts[b] + n - 1 lie, n = min(counts[b], N) (counts NULL: N), from
@@ -536,19 +536,24 @@ int qfa_attn_paged_lse(const qfa_paged_cache *cache, const void *q, int q_dtype,
  * page that is written may stand only once in the call's page table.  No counterpart in the reference.
  */
 typedef struct {
-  int8_t *codes; float *scale; void *zero;
-  int zero_bits;
+  int8_t *codes; float *scale; int8_t *zero;
 } qfa_page_bounds;
+typedef struct {
+  int8_t *codes; float *scale; int16_t *zero;
+} qfa_page_bounds16;
 
 int qfa_paged_bounds(const qfa_paged_cache *cache, const qfa_page_bounds *bounds, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw,
                      const int32_t *starts, const int32_t *counts, int64_t B, int64_t N, void *stream);
+int qfa_paged_bounds16(const qfa_paged_cache *cache, const qfa_page_bounds16 *bounds, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw,
+                       const int32_t *starts, const int32_t *counts, int64_t B, int64_t N, void *stream);
 
 /*
  * The blocks (pages) that a token's attention shall read.  A block's score for a token and key head is the largest over the query heads
  * that share the key head of
  *     s (s_high sum_d max(e_d, 0) (c_high,d - z_high) + s_low sum_d min(e_d, 0) (c_low,d - z_low)),
  * the query quantized per token (e = code - zero point, s its scale): with bounds of 16-bit zero points no key of the block has a larger product with the
- * query so quantized, but for half a step of the bounds' codes in every element, s |e_d| times s_high / 2 where e_d > 0 and s_low / 2 elsewhere.  Rounded to fp32 once, from 64 bits; what is not a number, or below -FLT_MAX, counts as -FLT_MAX.  Candidates of token n < counts[b] are the blocks
+ * query so quantized, but for half a step of the bounds' codes in every element, s |e_d| times s_high / 2 where e_d > 0 and s_low / 2 elsewhere.  Rounded
+ * to fp32 once, from 64 bits; what is not a number, or below -FLT_MAX, counts as -FLT_MAX.  Candidates of token n < counts[b] are the blocks
  * 0 .. (starts[b] + n) / page_size that the page table holds and whose page is in [0, pages).
  *   blocks  [B,cache->H,N,keep]: the numbers of the `keep` candidates with the largest scores (ties: the lowest number), the `first` first blocks and the
  *           `last` last ones that the token sees always among them; ascending, -1 behind.  first + last <= keep.
@@ -562,6 +567,10 @@ int qfa_paged_select(const qfa_paged_cache *cache, const qfa_page_bounds *bounds
                      const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, int32_t *blocks,
                      float *scores, int64_t B, int64_t H, int64_t N, int64_t keep, int64_t first, int64_t last, void *workspace, int64_t workspace_bytes,
                      void *stream);
+int qfa_paged_select16(const qfa_paged_cache *cache, const qfa_page_bounds16 *bounds, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn,
+                       const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, int32_t *blocks,
+                       float *scores, int64_t B, int64_t H, int64_t N, int64_t keep, int64_t first, int64_t last, void *workspace, int64_t workspace_bytes,
+                       void *stream);
 
 /*
  * qfa_attn_paged (causal) on listed blocks: token n of sequence b and the query heads of key head h see the keys j <= starts[b] + n of the blocks

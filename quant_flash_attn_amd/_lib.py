@@ -35,8 +35,8 @@ class PagedCacheStruct(ctypes.Structure):
 
 
 class PageBoundsStruct(ctypes.Structure):
-    """qfa_page_bounds"""
-    _fields_ = [("codes", c_void_p), ("scale", c_void_p), ("zero", c_void_p), ("zero_bits", c_int)]
+    """qfa_page_bounds, qfa_page_bounds16"""
+    _fields_ = [("codes", c_void_p), ("scale", c_void_p), ("zero", c_void_p)]
 
 
 # argument lists mirror include/qfa.h one to one
@@ -90,8 +90,10 @@ _SIGNATURES = {
     "qfa_attn_paged_lse_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _L]),
     "qfa_attn_paged_lse": (c_int, [_P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _L, _L, _L, _L, _F, _I, _P, _L, _P]),
     "qfa_paged_bounds": (c_int, [_P, _P, _P, _L, _L, _L, _P, _P, _L, _L, _P]),
+    "qfa_paged_bounds16": (c_int, [_P, _P, _P, _L, _L, _L, _P, _P, _L, _L, _P]),
     "qfa_paged_select_workspace_bytes": (c_int64, [_L, _L, _L, _L]),
     "qfa_paged_select": (c_int, [_P, _P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P] + [_L] * 6 + [_P, _L, _P]),
+    "qfa_paged_select16": (c_int, [_P, _P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P] + [_L] * 6 + [_P, _L, _P]),
     "qfa_attn_paged_blocks_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I, _L, _I]),
     "qfa_attn_paged_blocks": (c_int, [_P, _P, _I, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _L, _P, _L, _L, _L, _F, _P, _L, _P]),
     "qfa_paged_weights_workspace_bytes": (c_int64, [_L, _L, _L, _L, _I]),

@@ -100,11 +100,19 @@ static int check_keep(const char *who, int64_t keep, int64_t first, int64_t last
 static int check_slots(const char *who, const qfa_paged_cache *c, int64_t width) {
   return width <= (1LL << 30) / c->page_size ? 0 : set_error(QFA_EUNSUPPORTED, "%s: a page table has room for 2^30 keys at most", who);
 }
-static int check_bounds(const char *who, const qfa_page_bounds *b) {
-  if (!b || !b->codes || !b->scale || !b->zero) return set_error(QFA_EINVAL, "%s: null bounds pointer", who);
-  if (b->zero_bits != 0 && b->zero_bits != 8 && b->zero_bits != 16) return set_error(QFA_EINVAL, "%s: zero points of %d bits: 8 or 16 are needed", who, b->zero_bits);
-  if (!aligned16(b->codes) || !aligned8(b->scale) || (reinterpret_cast<uintptr_t>(b->zero) & (b->zero_bits == 16 ? 3u : 1u)))
-    return set_error(QFA_EINVAL, "%s: the bounds' codes must be 16-byte aligned, scales 8-byte and a block's two zero points together", who);
+// Bounds with zero points of 8 or 16 bits
+struct Bounds {
+  bool given;
+  int8_t *codes; float *scale; void *zero;
+  int bits;
+};
+template <typename T> static Bounds bounds_of(const T *b) {
+  return b ? Bounds{true, b->codes, b->scale, b->zero, (int)sizeof(*b->zero) * 8} : Bounds{false, nullptr, nullptr, nullptr, 8};
+}
+static int check_bounds(const char *who, const Bounds &b) {
+  if (!b.given || !b.codes || !b.scale || !b.zero) return set_error(QFA_EINVAL, "%s: null bounds pointer", who);
+  if (!aligned16(b.codes) || !aligned8(b.scale) || reinterpret_cast<uintptr_t>(b.zero) % (unsigned)(b.bits / 4))
+    return set_error(QFA_EINVAL, "%s: the bounds' codes must be 16-byte aligned, scales 8-byte and zero points %d-byte aligned", who, b.bits / 4);
   return 0;
 }
 
@@ -154,6 +162,46 @@ static int attn_paged(const char *who, const char *query, bool with_lse, const q
   if (int e = check_workspace(who, query, workspace, workspace_bytes, paged_attn_workspace_bytes(B, H, cache->H, N, cache->D, prefix, with_lse))) return e;
   a.o = o; a.lse = lse; a.prefix = prefix; a.sm_scale = sm_scale; a.causal = causal != 0; a.workspace = workspace;
   return launch_paged_attn(a, (hipStream_t)stream);
+}
+
+static int update_bounds(const char *who, const qfa_paged_cache *cache, const Bounds &bounds, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw,
+                         const int32_t *starts, const int32_t *counts, int64_t B, int64_t N, void *stream) {
+  if (int e = check_cache(who, cache)) return e;
+  if (int e = check_places(who, cache, page_table, starts, width, stb, stw, B, N)) return e;
+  if (int e = check_bounds(who, bounds)) return e;
+  PagedSelectArgs a;
+  memset(&a, 0, sizeof(a));
+  a.cache = ptrs_of(cache);
+  a.codes = bounds.codes; a.scale = bounds.scale; a.zero = bounds.zero; a.zero_bits = bounds.bits;
+  a.page_table = page_table; a.starts = starts; a.counts = counts;
+  a.pages = cache->pages; a.Hk = cache->H; a.width = width; a.stb = stb; a.stw = stw; a.B = B; a.N = N;
+  a.page_log2 = log2_of(cache->page_size); a.scale_dtype = cache->scale_dtype; a.D = cache->D;
+  return launch_paged_bounds(a, (hipStream_t)stream);
+}
+
+static int select_blocks(const char *who, const qfa_paged_cache *cache, const Bounds &bounds, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn,
+                         const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, int32_t *blocks,
+                         float *scores, int64_t B, int64_t H, int64_t N, int64_t keep, int64_t first, int64_t last, void *workspace, int64_t workspace_bytes,
+                         void *stream) {
+  PagedAttnArgs x;
+  if (int e = fill_attn(who, &x, cache, q, q_dtype, sqb, sqh, sqn, page_table, width, stb, stw, starts, counts, B, H, N)) return e;
+  if (int e = check_bounds(who, bounds)) return e;
+  if (!blocks) return set_error(QFA_EINVAL, "%s: null pointer argument", who);
+  if (int e = check_keep(who, keep, first, last)) return e;
+  if (!scores)
+    if (int e = check_workspace(who, "qfa_paged_select_workspace_bytes", workspace, workspace_bytes, qfa_paged_select_workspace_bytes(B, cache->H, N, width)))
+      return e;
+  PagedSelectArgs a;
+  memset(&a, 0, sizeof(a));
+  a.cache = x.cache;
+  a.codes = bounds.codes; a.scale = bounds.scale; a.zero = bounds.zero; a.zero_bits = bounds.bits;
+  a.page_table = page_table; a.starts = starts; a.counts = counts;
+  a.pages = x.pages; a.Hk = x.Hk; a.width = width; a.stb = stb; a.stw = stw; a.B = B; a.H = H; a.N = N;
+  a.page_log2 = x.page_log2; a.scale_dtype = x.scale_dtype; a.D = x.D; a.q_dtype = q_dtype;
+  a.q = q; a.sq[0] = sqb; a.sq[1] = sqh; a.sq[2] = sqn;
+  a.blocks = blocks; a.scores = scores ? scores : static_cast<float *>(workspace); a.all_scores = scores != nullptr;
+  a.keep = keep; a.first = first; a.last = last;
+  return launch_paged_select(a, (hipStream_t)stream);
 }
 
 extern "C" {
@@ -264,18 +312,11 @@ int qfa_attn_paged_lse(const qfa_paged_cache *cache, const void *q, int q_dtype,
 
 int qfa_paged_bounds(const qfa_paged_cache *cache, const qfa_page_bounds *bounds, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw,
                      const int32_t *starts, const int32_t *counts, int64_t B, int64_t N, void *stream) {
-  const char *who = "paged_bounds";
-  if (int e = check_cache(who, cache)) return e;
-  if (int e = check_places(who, cache, page_table, starts, width, stb, stw, B, N)) return e;
-  if (int e = check_bounds(who, bounds)) return e;
-  PagedSelectArgs a;
-  memset(&a, 0, sizeof(a));
-  a.cache = ptrs_of(cache);
-  a.codes = bounds->codes; a.scale = bounds->scale; a.zero = bounds->zero; a.zero_bits = bounds->zero_bits == 16 ? 16 : 8;
-  a.page_table = page_table; a.starts = starts; a.counts = counts;
-  a.pages = cache->pages; a.Hk = cache->H; a.width = width; a.stb = stb; a.stw = stw; a.B = B; a.N = N;
-  a.page_log2 = log2_of(cache->page_size); a.scale_dtype = cache->scale_dtype; a.D = cache->D;
-  return launch_paged_bounds(a, (hipStream_t)stream);
+  return update_bounds("paged_bounds", cache, bounds_of(bounds), page_table, width, stb, stw, starts, counts, B, N, stream);
+}
+int qfa_paged_bounds16(const qfa_paged_cache *cache, const qfa_page_bounds16 *bounds, const int32_t *page_table, int64_t width, int64_t stb, int64_t stw,
+                       const int32_t *starts, const int32_t *counts, int64_t B, int64_t N, void *stream) {
+  return update_bounds("paged_bounds16", cache, bounds_of(bounds), page_table, width, stb, stw, starts, counts, B, N, stream);
 }
 
 int64_t qfa_paged_select_workspace_bytes(int64_t B, int64_t Hk, int64_t N, int64_t width) {
@@ -287,26 +328,15 @@ int qfa_paged_select(const qfa_paged_cache *cache, const qfa_page_bounds *bounds
                      const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, int32_t *blocks,
                      float *scores, int64_t B, int64_t H, int64_t N, int64_t keep, int64_t first, int64_t last, void *workspace, int64_t workspace_bytes,
                      void *stream) {
-  const char *who = "paged_select";
-  PagedAttnArgs x;
-  if (int e = fill_attn(who, &x, cache, q, q_dtype, sqb, sqh, sqn, page_table, width, stb, stw, starts, counts, B, H, N)) return e;
-  if (int e = check_bounds(who, bounds)) return e;
-  if (!blocks) return set_error(QFA_EINVAL, "%s: null pointer argument", who);
-  if (int e = check_keep(who, keep, first, last)) return e;
-  if (!scores)
-    if (int e = check_workspace(who, "qfa_paged_select_workspace_bytes", workspace, workspace_bytes, qfa_paged_select_workspace_bytes(B, cache->H, N, width)))
-      return e;
-  PagedSelectArgs a;
-  memset(&a, 0, sizeof(a));
-  a.cache = x.cache;
-  a.codes = bounds->codes; a.scale = bounds->scale; a.zero = bounds->zero; a.zero_bits = bounds->zero_bits == 16 ? 16 : 8;
-  a.page_table = page_table; a.starts = starts; a.counts = counts;
-  a.pages = x.pages; a.Hk = x.Hk; a.width = width; a.stb = stb; a.stw = stw; a.B = B; a.H = H; a.N = N;
-  a.page_log2 = x.page_log2; a.scale_dtype = x.scale_dtype; a.D = x.D; a.q_dtype = q_dtype;
-  a.q = q; a.sq[0] = sqb; a.sq[1] = sqh; a.sq[2] = sqn;
-  a.blocks = blocks; a.scores = scores ? scores : static_cast<float *>(workspace); a.all_scores = scores != nullptr;
-  a.keep = keep; a.first = first; a.last = last;
-  return launch_paged_select(a, (hipStream_t)stream);
+  return select_blocks("paged_select", cache, bounds_of(bounds), q, q_dtype, sqb, sqh, sqn, page_table, width, stb, stw, starts, counts, blocks, scores, B, H, N, keep, first, last,
+                       workspace, workspace_bytes, stream);
+}
+int qfa_paged_select16(const qfa_paged_cache *cache, const qfa_page_bounds16 *bounds, const void *q, int q_dtype, int64_t sqb, int64_t sqh, int64_t sqn,
+                       const int32_t *page_table, int64_t width, int64_t stb, int64_t stw, const int32_t *starts, const int32_t *counts, int32_t *blocks,
+                       float *scores, int64_t B, int64_t H, int64_t N, int64_t keep, int64_t first, int64_t last, void *workspace, int64_t workspace_bytes,
+                       void *stream) {
+  return select_blocks("paged_select16", cache, bounds_of(bounds), q, q_dtype, sqb, sqh, sqn, page_table, width, stb, stw, starts, counts, blocks, scores, B, H, N, keep, first, last,
+                       workspace, workspace_bytes, stream);
 }
 
 int64_t qfa_attn_paged_blocks_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t N, int D, int64_t keep, int page_size) {

@@ -68,7 +68,9 @@ struct Api {
   QFA_ENTRY(qfa_attn_paged_lse_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged_lse);
   QFA_ENTRY(qfa_paged_bounds);
+  QFA_ENTRY(qfa_paged_bounds16);
   QFA_ENTRY(qfa_paged_select);
+  QFA_ENTRY(qfa_paged_select16);
   QFA_ENTRY(qfa_paged_select_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged_blocks_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged_blocks);
@@ -122,7 +124,9 @@ void init(const py::dict &address) {
   QFA_ENTRY(qfa_attn_paged_lse_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged_lse);
   QFA_ENTRY(qfa_paged_bounds);
+  QFA_ENTRY(qfa_paged_bounds16);
   QFA_ENTRY(qfa_paged_select);
+  QFA_ENTRY(qfa_paged_select16);
   QFA_ENTRY(qfa_paged_select_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged_blocks_workspace_bytes);
   QFA_ENTRY(qfa_attn_paged_blocks);

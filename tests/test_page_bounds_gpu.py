@@ -152,7 +152,9 @@ def test_argument_errors_need_no_gpu(qfa):
     from quant_flash_attn_amd import _lib
     L, P = _lib.lib(), 0x1000
     cache = _lib.PagedCacheStruct(k_codes=P, k_scale=P, k_zero=P, v_codes=P, v_scale=P, v_zero=P, pages=4, H=2, page_size=16, D=64, scale_dtype=1)
-    for zero, bits in ((P, 7), (P, -16), (P, 32), (P + 2, 16), (P + 1, 8)):
-        bounds = _lib.PageBoundsStruct(P, P, zero, bits)
-        assert L.qfa_paged_bounds(ctypes.byref(cache), ctypes.byref(bounds), P, 4, 4, 1, P, None, 1, 1, None) == -1, (zero, bits)
-        assert L.qfa_paged_select(ctypes.byref(cache), ctypes.byref(bounds), P, 2, 1024, 512, 64, P, 4, 4, 1, P, None, P, None, 1, 4, 2, 2, 1, 1, P, 1 << 20, None) == -1
+    for codes, scale, zero, eight in ((P, P, P + 2, False), (P, P, P + 1, True), (P, P + 4, P, False), (P + 8, P, P, False), (P, P, None, False), (None, P, P, True)):
+        for update, select in ((L.qfa_paged_bounds, L.qfa_paged_select), (L.qfa_paged_bounds16, L.qfa_paged_select16))[not eight:]:
+            bounds = ctypes.byref(_lib.PageBoundsStruct(codes, scale, zero))
+            assert update(ctypes.byref(cache), bounds, P, 4, 4, 1, P, None, 1, 1, None) == -1, (codes, scale, zero)
+            assert select(ctypes.byref(cache), bounds, P, 2, 1024, 512, 64, P, 4, 4, 1, P, None, P, None, 1, 4, 2, 2, 1, 1, P, 1 << 20, None) == -1
+    assert L.qfa_paged_bounds16(ctypes.byref(cache), None, P, 4, 4, 1, P, None, 1, 1, None) == -1
